@@ -506,6 +506,45 @@ int warpctct_status(unsigned *bits, int clear);
  * the defaults). */
 int warpctct_joiner_linear_lattice(int from_frames);
 
+/* ---- beside the losses: layer norm ----------------------------------------
+ * No counterpart in the reference, whose callers take these operators from
+ * torch: what makes the label scores g of the joiner (a norm, a short causal
+ * convolution, a selective scan, with forms for one token at a time) and the
+ * rules that a decoder puts on the joiner's logits.  Element types are
+ * WARPCTCT_F32 / F16 / BF16; all arithmetic is fp32, a result is rounded once.
+ *
+ * out = (x - mean) / sqrt(var + eps) * weight + bias over the last dimension.
+ * x holds `rows` rows of `width` >= 1 elements that lie next to each other; row
+ * i starts at element (i / x_inner_rows) * x_outer_stride + (i % x_inner_rows) *
+ * x_inner_stride (x_inner_rows = rows for rows a fixed distance apart).  weight,
+ * bias: width elements each of weight_dtype (that of x, or WARPCTCT_F32), or
+ * NULL for 1 and 0.  out (rows, width) is dense.  stats: 3 * rows floats
+ * that the backward pass reads, or NULL.  rows < 2^31. */
+typedef struct {
+    int dtype, weight_dtype, width;
+    float eps;
+    long rows, x_inner_rows, x_outer_stride, x_inner_stride;
+    const void *x, *weight, *bias;
+    void *out;
+    float *stats;
+} warpctct_norm_t;
+int warpctct_layer_norm(const warpctct_norm_t *p, void *stream);
+
+/* Gradients for grad_out, addressed like x by the three numbers in front of it:
+ * grad_x (rows, width) dense in the type of x, grad_weight and grad_bias in
+ * weight_dtype; each may be NULL.  `out`, `bias` and `eps` of p are not used.  The column sums are
+ * added up in a fixed order, through `workspace`
+ * (warpctct_layer_norm_workspace_bytes, needed where grad_weight or grad_bias
+ * is given). */
+typedef struct {
+    long inner_rows, outer_stride, inner_stride;
+    const void *grad_out;
+    void *grad_x, *grad_weight, *grad_bias;
+} warpctct_norm_grad_t;
+size_t warpctct_layer_norm_workspace_bytes(long rows, int width);
+int warpctct_layer_norm_grad(const warpctct_norm_t *p, const warpctct_norm_grad_t *g, void *workspace,
+                             size_t workspace_bytes, void *stream);
+
 /* ---- measurement aid ------------------------------------------------------
  * No counterpart in the reference.  warpctct_profile(1) clears earlier records
  * and starts bracketing every kernel launch of the library with two HIP events

@@ -1,0 +1,64 @@
+"""Host-side argument checks of the C entry points beside the losses: wrong
+arguments are refused before any launch, empty problems are no-ops.  Nothing
+touches a device."""
+import ctypes
+
+import hip_lib
+
+EINVAL, EWORKSPACE = 1, 3
+F32, F16, BF16 = 0, 1, 2
+P = ctypes.c_void_p
+HOST = (ctypes.c_float * 64)()
+SOME = ctypes.cast(HOST, P).value       # an address that is never followed
+
+
+class Norm(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int), ("weight_dtype", ctypes.c_int), ("width", ctypes.c_int),
+                ("eps", ctypes.c_float), ("rows", ctypes.c_long), ("x_inner_rows", ctypes.c_long),
+                ("x_outer_stride", ctypes.c_long), ("x_inner_stride", ctypes.c_long), ("x", P), ("weight", P),
+                ("bias", P), ("out", P), ("stats", P)]
+
+
+class NormGrad(ctypes.Structure):
+    _fields_ = [("inner_rows", ctypes.c_long), ("outer_stride", ctypes.c_long), ("inner_stride", ctypes.c_long),
+                ("grad_out", P), ("grad_x", P), ("grad_weight", P), ("grad_bias", P)]
+
+
+def norm(**over):
+    fields = dict(dtype=F32, weight_dtype=F32, width=8, eps=1e-5, rows=4, x_inner_rows=4, x_outer_stride=0,
+                  x_inner_stride=8, x=SOME, weight=None, bias=None, out=SOME, stats=SOME)
+    fields.update(over)
+    return Norm(**fields)
+
+
+def test_layer_norm_arguments():
+    lib = hip_lib.lib()
+    call = lambda **over: lib.warpctct_layer_norm(ctypes.byref(norm(**over)), P(0))  # noqa: E731
+    assert lib.warpctct_layer_norm(P(0), P(0)) == EINVAL
+    for bad in (dict(dtype=3), dict(weight_dtype=F16), dict(width=0), dict(rows=-1), dict(rows=2 ** 31),
+                dict(x=None), dict(out=None), dict(x_inner_rows=0)):
+        assert call(**bad) == EINVAL, bad
+    assert call(rows=0, x=None, out=None) == 0
+
+
+def test_layer_norm_gradient_arguments():
+    lib = hip_lib.lib()
+    size = lib.warpctct_layer_norm_workspace_bytes
+    size.restype, size.argtypes = ctypes.c_size_t, [ctypes.c_long, ctypes.c_int]
+    assert size(4, 8) == 64 and size(-1, 8) == 0 and size(4, 0) == 0
+    assert size(1 << 20, 8) == 512 * 64      # a workgroup walks over rows: the scratch does not grow with them
+
+    def call(p=None, workspace=SOME, have=1 << 20, **over):
+        fields = dict(inner_rows=4, outer_stride=0, inner_stride=8, grad_out=SOME, grad_x=SOME, grad_weight=SOME,
+                      grad_bias=SOME)
+        fields.update(over)
+        return lib.warpctct_layer_norm_grad(ctypes.byref(p or norm()), ctypes.byref(NormGrad(**fields)),
+                                            P(workspace), ctypes.c_size_t(have), P(0))
+
+    assert call(norm(stats=None)) == EINVAL
+    assert call(grad_out=None) == EINVAL
+    assert call(inner_rows=0) == EINVAL
+    assert call(workspace=0) == EINVAL
+    assert call(have=63) == EWORKSPACE
+    assert call(grad_x=None, grad_weight=None, grad_bias=None) == 0
+    assert call(norm(rows=0), grad_weight=None, grad_bias=None) == 0

@@ -8,35 +8,9 @@
 // layout raises RuntimeError through TORCH_CHECK.  Unlike the reference there
 // is no device-to-host synchronisation (its binding.cpp:68 reads
 // (lx-ly).max() on the host) and a failed launch raises instead of exiting.
-#include <torch/extension.h>
-
-// PyTorch-ROCm presents HIP devices under the "cuda" device type; these are
-// its guard and stream accessors for that arrangement.
-#include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-
-#include <tuple>
-
-#include "warp_ctct_hip.h"
+#include "binding_common.h"
 
 namespace {
-
-#define CHECK_CONTIGUOUS(x) TORCH_CHECK((x).is_contiguous(), #x " must be contiguous")
-#define CHECK_DEVICE(x) TORCH_CHECK((x).device().is_cuda(), #x " must be located on the GPU")
-#define CHECK_FLOAT(x) \
-    TORCH_CHECK((x).scalar_type() == at::ScalarType::Float, #x " must be a Float tensor")
-#define CHECK_INT(x) \
-    TORCH_CHECK((x).scalar_type() == at::ScalarType::Int, #x " must be a Int tensor")
-
-void check_rc(int rc, const char *what) {
-    TORCH_CHECK(rc == WARPCTCT_OK, what, ": ", warpctct_error_string(rc));
-}
-
-using DeviceGuard = c10::hip::OptionalHIPGuardMasqueradingAsCUDA;
-
-void *current_stream() {
-    return static_cast<void *>(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream());
-}
 
 void check_lengths(const torch::Tensor &ys, const torch::Tensor &lx, const torch::Tensor &ly,
                    int64_t N, int64_t U) {
@@ -875,4 +849,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         },
         "Sticky status bits of the current device (synchronises with it).",
         pybind11::arg("clear") = true);
+    define_network(m);
 }

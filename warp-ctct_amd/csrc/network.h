@@ -1,0 +1,26 @@
+// Internal launch interface of the operators beside the losses (layer norm,
+// causal convolution, selective scan, rules on logits) between the C ABI
+// (network_api.hip) and their kernels.  Structs of device pointers and sizes;
+// each launcher enqueues on the given stream and returns hipGetLastError().
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "launch.h"
+#include "warp_ctct_hip.h"
+
+namespace wctct {
+
+hipError_t launch_layer_norm(const warpctct_norm_t &p, hipStream_t stream);
+// workgroups of the backward pass, each of which leaves 2 * width partial sums
+int norm_grad_groups(long rows, int width);
+hipError_t launch_layer_norm_grad(const warpctct_norm_t &p, const warpctct_norm_grad_t &g,
+                                  float *partial, hipStream_t stream);
+
+// out[column] = sum over `rows` rows of partial (rows, columns), in a fixed
+// order; the first `split` columns go to `first`, the others to `second`, in
+// the element type given for each (either pointer may be null).
+hipError_t launch_column_sums(const float *partial, long rows, int columns, int split, void *first,
+                              int first_type, void *second, int second_type, hipStream_t stream);
+
+}  // namespace wctct

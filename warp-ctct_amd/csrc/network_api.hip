@@ -1,0 +1,63 @@
+// extern "C" surface of the operators beside the losses (declared in
+// include/warp_ctct_hip.h).  Host code only: argument validation and kernel
+// launches.  No allocation, no host synchronisation, no process exit.
+#include <hip/hip_runtime.h>
+
+#include "network.h"
+#include "warp_ctct_hip.h"
+
+namespace {
+
+using namespace wctct;
+
+inline hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
+
+inline int done(hipError_t e) {
+    if (e == hipSuccess) return WARPCTCT_OK;
+    return e == hipErrorInvalidValue ? WARPCTCT_EINVAL : WARPCTCT_ELAUNCH;
+}
+
+constexpr long kMostRows = 0x7fffffffL;
+
+bool norm_ok(const warpctct_norm_t *p) {
+    return p && io_valid(p->dtype) && (p->weight_dtype == p->dtype || p->weight_dtype == WARPCTCT_F32) &&
+           p->width >= 1 && p->width <= 0x3fffffff && p->rows >= 0 && p->rows <= kMostRows &&
+           (p->rows == 0 || (p->x && p->x_inner_rows >= 1));
+}
+
+}  // namespace
+
+extern "C" {
+
+int warpctct_layer_norm(const warpctct_norm_t *p, void *stream) {
+    if (!norm_ok(p)) return WARPCTCT_EINVAL;
+    if (p->rows == 0) return WARPCTCT_OK;
+    if (!p->out) return WARPCTCT_EINVAL;
+    return done(launch_layer_norm(*p, as_stream(stream)));
+}
+
+size_t warpctct_layer_norm_workspace_bytes(long rows, int width) {
+    if (rows < 0 || rows > kMostRows || width < 1) return 0;
+    const long groups = rows > 0 ? norm_grad_groups(rows, width) : 1;
+    return (size_t)groups * 2 * (size_t)width * sizeof(float);
+}
+
+int warpctct_layer_norm_grad(const warpctct_norm_t *p, const warpctct_norm_grad_t *g, void *workspace,
+                             size_t workspace_bytes, void *stream) {
+    if (!norm_ok(p) || !g) return WARPCTCT_EINVAL;
+    const bool columns = g->grad_weight || g->grad_bias;
+    if (p->rows > 0 && (!p->stats || !g->grad_out || g->inner_rows < 1)) return WARPCTCT_EINVAL;
+    if (columns && !workspace) return WARPCTCT_EINVAL;
+    if (columns && workspace_bytes < warpctct_layer_norm_workspace_bytes(p->rows, p->width))
+        return WARPCTCT_EWORKSPACE;
+    float *partial = columns ? static_cast<float *>(workspace) : nullptr;
+    if (p->rows == 0) {     // the sums of no rows: zeros
+        if (!columns) return WARPCTCT_OK;
+        return done(launch_column_sums(partial, 0, 2 * p->width, p->width, g->grad_weight, p->weight_dtype,
+                                       g->grad_bias, p->weight_dtype, as_stream(stream)));
+    }
+    if (!g->grad_x && !columns) return WARPCTCT_OK;
+    return done(launch_layer_norm_grad(*p, *g, partial, as_stream(stream)));
+}
+
+}  // extern "C"

@@ -1,0 +1,118 @@
+// Loads, stores and reductions shared by the operators that work on rows of
+// float, half or bfloat16 elements in 16-byte vectors (norm.hip, conv.hip,
+// scan.hip, adjust.hip).  All arithmetic is in fp32; a store rounds to nearest
+// even, once.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+namespace wctct {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+typedef unsigned int raw16 __attribute__((ext_vector_type(4)));
+
+// elements per 16-byte vector
+template <typename IO>
+constexpr int kVec = 16 / (int)sizeof(IO);
+
+template <typename IO>
+__device__ __forceinline__ float to_float(IO v) { return (float)v; }
+template <typename IO>
+__device__ __forceinline__ IO from_float(float v) { return (IO)v; }
+
+template <typename IO>
+__device__ __forceinline__ raw16 load16(const IO *p) { return *reinterpret_cast<const raw16 *>(p); }
+
+__device__ __forceinline__ void unpack16(const float *, raw16 v, float *x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[i]);
+}
+__device__ __forceinline__ void unpack16(const f16 *, raw16 v, float *x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned word = v[i];
+        x[2 * i] = (float)__builtin_bit_cast(f16, (unsigned short)(word & 0xffffu));
+        x[2 * i + 1] = (float)__builtin_bit_cast(f16, (unsigned short)(word >> 16));
+    }
+}
+__device__ __forceinline__ void unpack16(const bf16 *, raw16 v, float *x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(v[i] << 16);
+        x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+    }
+}
+
+// two floats rounded to nearest even into one word of 2-byte elements
+__device__ __forceinline__ unsigned pack_two(const f16 *, float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef f16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, h2));
+}
+__device__ __forceinline__ unsigned pack_two(const bf16 *, float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, b2));
+}
+__device__ __forceinline__ raw16 pack16(const float *, const float *x) {
+    return raw16{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                 __float_as_uint(x[3])};
+}
+template <typename IO>
+__device__ __forceinline__ raw16 pack16(const IO *p, const float *x) {
+    return raw16{pack_two(p, x[0], x[1]), pack_two(p, x[2], x[3]), pack_two(p, x[4], x[5]),
+                 pack_two(p, x[6], x[7])};
+}
+template <typename IO>
+__device__ __forceinline__ void load_vec(const IO *p, float *x) { unpack16(p, load16(p), x); }
+template <typename IO>
+__device__ __forceinline__ void store_vec(IO *p, const float *x) {
+    *reinterpret_cast<raw16 *>(p) = pack16(p, x);
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __uint_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E;        // quad_perm [1,0,3,2], [2,3,0,1]
+constexpr int kDppRor4 = 0x124, kDppRor8 = 0x128;      // rotations within 16 lanes
+
+// v of lane l plus v of lane l ^ 16 / l ^ 32, in every lane
+__device__ __forceinline__ float add_xor16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float add_xor32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Sum over the wavefront, the same bits in every lane: each step adds the two
+// halves of a pair of lanes.  (The rotation by 8 comes before that by 4, which
+// pairs lanes l and l ^ 4 only once l and l ^ 8 hold the same.)
+__device__ __forceinline__ float wave_sum(float v) {
+    v += dpp<kDppXor1>(v);
+    v += dpp<kDppXor2>(v);
+    v += dpp<kDppRor8>(v);
+    v += dpp<kDppRor4>(v);
+    return add_xor32(add_xor16(v));
+}
+
+__device__ __forceinline__ float sigmoid(float v) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
+}
+
+// Rows of a tensor whose leading dimensions are addressed by two strides (in
+// elements): row i starts at (i / inner) * outer_stride + (i % inner) * inner_stride.
+struct RowAddress {
+    unsigned inner;      // rows per outer index; 0: all rows lie inner_stride apart
+    long outer_stride, inner_stride;
+    __device__ __forceinline__ long at(unsigned row) const {
+        if (inner == 0u) return (long)row * inner_stride;
+        const unsigned o = row / inner;
+        return (long)o * outer_stride + (long)(row - o * inner) * inner_stride;
+    }
+};
+
+}  // namespace wctct

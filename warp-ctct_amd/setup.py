@@ -34,7 +34,7 @@ class BuildWithHip(BuildExtension):
 
 ext = CppExtension(
     name="warp_ctct._C",
-    sources=["csrc/binding.cpp"],
+    sources=["csrc/binding.cpp", "csrc/binding_network.cpp"],
     include_dirs=[os.path.join(HERE, "..", "include"), os.path.join(ROCM, "include")],
     define_macros=[("__HIP_PLATFORM_AMD__", "1"), ("USE_ROCM", "1")],
     extra_compile_args=["-O2", "-std=c++17"],

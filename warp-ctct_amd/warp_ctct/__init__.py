@@ -22,10 +22,13 @@ except ImportError as exc:  # pragma: no cover - exercised only on a broken inst
         "(needs hipcc, --offload-arch=gfx950)"
     ) from exc
 
+from .network import layer_norm  # noqa: E402,F401
+
 # The reference exports exactly these two (warp_ctct/__init__.py:17), so that
 # `from warp_ctct import *` binds the same names.  ctct_loss_with_logits,
-# ctct_loss_compact and label_range_violated are additions of this build and are
-# reached by name (warp_ctct.ctct_loss_with_logits, ...).
+# ctct_loss_compact, label_range_violated and the operators of network.py are
+# additions of this build and are reached by name
+# (warp_ctct.ctct_loss_with_logits, ...).
 __all__ = ["ctct_loss", "ctct_simple_loss"]
 
 
