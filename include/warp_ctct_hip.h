@@ -545,6 +545,59 @@ size_t warpctct_layer_norm_workspace_bytes(long rows, int width);
 int warpctct_layer_norm_grad(const warpctct_norm_t *p, const warpctct_norm_grad_t *g, void *workspace,
                              size_t workspace_bytes, void *stream);
 
+/* ---- beside the losses: short causal convolution ---------------------------
+ * Every channel e of x (N, L, E) with its own K <= WARPCTCT_CONV_MAX_TAPS taps:
+ *   out[n][t][e] = act(bias[e] + sum_k weight[e][k] * x[n][t - (K-1) + k][e]),
+ * act the identity or, with silu != 0, v / (1 + e^-v).  x[n][t] lies at element
+ * n * x_n + t * x_t, its channels next to each other.  In front of x lie the K-1
+ * rows of initial (N, K-1, E), NULL for zeros.  Of sequence n the first
+ * lengths[n] steps count (NULL: all L; a value outside [0, L] is clamped): the
+ * others are not read, and out is zero there.  last (N, K-1, E), may be NULL:
+ * the K-1 inputs before step lengths[n], the `initial` of a call that goes on
+ * from there.  weight (E, K), bias (E, may be NULL): float.  out, initial, last:
+ * dense, in the type of x.  N <= 65535. */
+enum { WARPCTCT_CONV_MAX_TAPS = 8 };
+typedef struct {
+    int dtype, N, L, E, K, silu;
+    long x_n, x_t;
+    const void *x;
+    const float *weight, *bias;
+    const int *lengths;
+    const void *initial;
+    void *out, *last;
+} warpctct_conv_t;
+int warpctct_causal_conv(const warpctct_conv_t *p, void *stream);
+
+/* Gradients for grad_out (addressed like x by grad_n, grad_t) and, if not NULL,
+ * grad_last (N, K-1, E): grad_x (N, L, E) and grad_initial (N, K-1, E; may be
+ * NULL) dense in the type of x, grad_weight (E, K) and grad_bias (E) float, each
+ * of which may be NULL; these two are added up in a fixed order through
+ * `workspace`.  `out` and `last` of p are not used. */
+typedef struct {
+    long grad_n, grad_t;
+    const void *grad_out, *grad_last;
+    void *grad_x, *grad_initial;
+    float *grad_weight, *grad_bias;
+} warpctct_conv_grad_t;
+size_t warpctct_causal_conv_workspace_bytes(int N, int L, int E, int K);
+int warpctct_causal_conv_grad(const warpctct_conv_t *p, const warpctct_conv_grad_t *g, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
+/* One step for N sequences at once: x (N, E), rows x_n elements apart; state
+ * (N, K-1, E) dense, updated in place; out (N, E) dense.  A sequence whose
+ * advance[n] is 0 (advance may be NULL) keeps its state, and its row of out is
+ * zero: a hypothesis that took blank does not move its prediction network on. */
+typedef struct {
+    int dtype, N, E, K, silu;
+    long x_n;
+    const void *x;
+    void *state;
+    const float *weight, *bias;
+    const unsigned char *advance;
+    void *out;
+} warpctct_conv_step_t;
+int warpctct_causal_conv_step(const warpctct_conv_step_t *p, void *stream);
+
 /* ---- measurement aid ------------------------------------------------------
  * No counterpart in the reference.  warpctct_profile(1) clears earlier records
  * and starts bracketing every kernel launch of the library with two HIP events

@@ -62,3 +62,65 @@ def test_layer_norm_gradient_arguments():
     assert call(have=63) == EWORKSPACE
     assert call(grad_x=None, grad_weight=None, grad_bias=None) == 0
     assert call(norm(rows=0), grad_weight=None, grad_bias=None) == 0
+
+
+class Conv(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_int) for k in ("dtype", "N", "L", "E", "K", "silu")] + [
+        ("x_n", ctypes.c_long), ("x_t", ctypes.c_long), ("x", P), ("weight", P), ("bias", P), ("lengths", P),
+        ("initial", P), ("out", P), ("last", P)]
+
+
+class ConvGrad(ctypes.Structure):
+    _fields_ = [("grad_n", ctypes.c_long), ("grad_t", ctypes.c_long)] + [
+        (k, P) for k in ("grad_out", "grad_last", "grad_x", "grad_initial", "grad_weight", "grad_bias")]
+
+
+class ConvStep(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_int) for k in ("dtype", "N", "E", "K", "silu")] + [("x_n", ctypes.c_long)] + [
+        (k, P) for k in ("x", "state", "weight", "bias", "advance", "out")]
+
+
+def conv(**over):
+    fields = dict(dtype=BF16, N=2, L=5, E=4, K=4, silu=1, x_n=20, x_t=4, x=SOME, weight=SOME, out=SOME)
+    fields.update(over)
+    return Conv(**fields)
+
+
+def test_causal_conv_arguments():
+    lib = hip_lib.lib()
+    call = lambda **over: lib.warpctct_causal_conv(ctypes.byref(conv(**over)), P(0))  # noqa: E731
+    assert lib.warpctct_causal_conv(P(0), P(0)) == EINVAL
+    for bad in (dict(dtype=-1), dict(N=-1), dict(N=65536), dict(L=-1), dict(E=0), dict(K=0), dict(K=9), dict(x=None),
+                dict(weight=None), dict(out=None), dict(E=1 << 29), dict(L=1 << 30, E=1 << 20)):
+        assert call(**bad) == EINVAL, bad
+    assert call(N=0, x=None, weight=None, out=None) == 0
+
+
+def test_causal_conv_gradient_and_step_arguments():
+    lib = hip_lib.lib()
+    size = lib.warpctct_causal_conv_workspace_bytes
+    size.restype = ctypes.c_size_t
+    assert size(2, 5, 4, 4) == 2 * 20 * 4 and size(2, 5, 4, 9) == 0 and size(-1, 5, 4, 4) == 0
+    assert size(0, 5, 4, 4) == 0
+
+    def call(p=None, workspace=SOME, have=1 << 20, **over):
+        fields = dict(grad_n=20, grad_t=4, grad_out=SOME, grad_x=SOME, grad_weight=SOME, grad_bias=SOME)
+        fields.update(over)
+        return lib.warpctct_causal_conv_grad(ctypes.byref(p or conv()), ctypes.byref(ConvGrad(**fields)),
+                                             P(workspace), ctypes.c_size_t(have), P(0))
+
+    assert call(conv(K=9)) == EINVAL
+    assert call(grad_out=None) == EINVAL and call(grad_x=None) == EINVAL
+    assert call(workspace=0) == EINVAL and call(have=159) == EWORKSPACE
+    assert call(conv(N=0), grad_weight=None, grad_bias=None) == 0
+
+    def step(**over):
+        fields = dict(dtype=F16, N=2, E=4, K=4, silu=0, x_n=4, x=SOME, state=SOME, weight=SOME, out=SOME)
+        fields.update(over)
+        return lib.warpctct_causal_conv_step(ctypes.byref(ConvStep(**fields)), P(0))
+
+    assert lib.warpctct_causal_conv_step(P(0), P(0)) == EINVAL
+    for bad in (dict(dtype=4), dict(N=-1), dict(E=0), dict(K=0), dict(K=9), dict(x=None), dict(state=None),
+                dict(weight=None), dict(out=None)):
+        assert step(**bad) == EINVAL, bad
+    assert step(N=0, x=None, state=None) == 0

@@ -595,13 +595,6 @@ std::tuple<torch::Tensor, torch::Tensor> log_matmul_backward(
 // SimpleCTCTLoss / LogMMExp chain (:55-85, :36-52, :195-225) and of the caller's
 // log_softmax in front of ctct_loss.
 
-// labels and lengths as contiguous int32 (the reference casts with .int(),
-// warp_ctct/__init__.py:135-136); tensors that already are cost nothing
-torch::Tensor as_int32(const torch::Tensor &t) {
-    if (t.scalar_type() == at::ScalarType::Int && t.is_contiguous()) return t;
-    return t.to(at::ScalarType::Int).contiguous();
-}
-
 torch::Tensor upstream(const torch::Tensor &grad_output) {
     return grad_output.reshape({-1}).to(at::ScalarType::Float).contiguous();
 }

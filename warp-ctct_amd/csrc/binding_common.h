@@ -30,5 +30,12 @@ inline void *current_stream() {
     return static_cast<void *>(c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream());
 }
 
+// labels and lengths as contiguous int32 (the reference casts with .int(),
+// warp_ctct/__init__.py:135-136); tensors that already are cost nothing
+inline torch::Tensor as_int32(const torch::Tensor &t) {
+    if (t.scalar_type() == at::ScalarType::Int && t.is_contiguous()) return t;
+    return t.to(at::ScalarType::Int).contiguous();
+}
+
 // The operators beside the losses (binding_network.cpp).
 void define_network(pybind11::module &m);

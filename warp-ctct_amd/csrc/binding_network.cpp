@@ -1,4 +1,5 @@
-// The operators beside the losses, for torch: layer norm.  Each is differentiable where it has a backward pass; without gradients to
+// The operators beside the losses, for torch: layer norm and the causal
+// convolution, the latter also one step at a time.  Each is differentiable where it has a backward pass; without gradients to
 // track it goes straight to the C ABI.  Arguments are checked here (RuntimeError
 // through TORCH_CHECK); nothing synchronises with the host.
 #include "binding_common.h"
@@ -198,10 +199,208 @@ torch::Tensor layer_norm(const torch::Tensor &input, Maybe weight, Maybe bias, c
     return std::get<0>(norm_forward(call, false));
 }
 
+// ---- what the operators along time share ---------------------------------------
+
+int int_size(const torch::Tensor &t, int64_t d, const char *what) {
+    TORCH_CHECK(t.size(d) <= 0x7fffffff, what, ": a dimension is too large");
+    return static_cast<int>(t.size(d));
+}
+
+// a tensor whose last dimension is dense (a copy, if it is not)
+torch::Tensor dense_last(const torch::Tensor &t) {
+    return t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+torch::Tensor lengths_of(const Maybe &lengths, const torch::Tensor &x, const char *what) {
+    if (!given(lengths)) return torch::Tensor();
+    TORCH_CHECK(lengths->dim() == 1 && lengths->size(0) == x.size(0) && !lengths->is_floating_point(), what,
+                ": lengths must be whole numbers, one for each sequence");
+    check_on(*lengths, x, "lengths");
+    return as_int32(*lengths);
+}
+
+torch::Tensor flags_of(const Maybe &advance, const torch::Tensor &x, const char *what) {
+    if (!given(advance)) return torch::Tensor();
+    TORCH_CHECK(advance->dim() == 1 && advance->size(0) == x.size(0) &&
+                    advance->scalar_type() == at::ScalarType::Bool,
+                what, ": advance must be truth values, one for each sequence");
+    check_on(*advance, x, "advance");
+    return advance->contiguous();
+}
+
+// A step updates its state in place and has no backward pass.
+void refuse_gradient(std::initializer_list<const Maybe *> inputs, const char *what) {
+    for (const Maybe *t : inputs)
+        TORCH_CHECK(!tracked(*t), what, ": not differentiable; call it under torch.no_grad()");
+}
+
+// ---- causal convolution ----------------------------------------------------------
+
+struct ConvInputs {
+    torch::Tensor x, weight, bias, lengths, initial;
+    warpctct_conv_t call() const {
+        warpctct_conv_t p = {};
+        p.dtype = type_of(x);
+        p.N = static_cast<int>(x.size(0));
+        p.L = static_cast<int>(x.size(1));
+        p.E = static_cast<int>(x.size(2));
+        p.K = static_cast<int>(weight.size(1));
+        p.x_n = x.stride(0);
+        p.x_t = x.stride(1);
+        p.x = x.data_ptr();
+        p.weight = floats(weight);
+        p.bias = floats(bias);
+        p.lengths = lengths.defined() ? lengths.data_ptr<int>() : nullptr;
+        p.initial = ptr(initial);
+        return p;
+    }
+};
+
+tensor_list conv_forward(const ConvInputs &in, bool silu, bool want_state) {
+    const DeviceGuard guard(device_of(in.x));
+    auto p = in.call();
+    p.silu = silu ? 1 : 0;
+    tensor_list outs = {torch::empty(in.x.sizes(), in.x.options())};
+    if (want_state) outs.push_back(torch::empty({p.N, p.K - 1, p.E}, in.x.options()));
+    p.out = outs[0].data_ptr();
+    p.last = want_state ? outs[1].data_ptr() : nullptr;
+    check_rc(warpctct_causal_conv(&p, current_stream()), "causal_conv");
+    return outs;
+}
+
+class CausalConv : public torch::autograd::Function<CausalConv> {
+   public:
+    static tensor_list forward(AutogradContext *ctx, const torch::Tensor &x, const torch::Tensor &weight,
+                               const Maybe &bias, const Maybe &initial, const Maybe &lengths, const bool silu,
+                               const bool want_state, const bool track_weight, const bool track_bias,
+                               const bool track_initial) {
+        const auto plain = [](const Maybe &t) { return given(t) ? *t : torch::Tensor(); };
+        const ConvInputs in = {x, weight, plain(bias), plain(lengths), plain(initial)};
+        ctx->save_for_backward({in.x, in.weight, in.bias, in.lengths, in.initial});
+        ctx->saved_data["silu"] = silu;
+        ctx->saved_data["track"] = std::vector<int64_t>{track_weight, track_bias, track_initial};
+        ctx->set_materialize_grads(false);
+        return conv_forward(in, silu, want_state);
+    }
+
+    static tensor_list backward(AutogradContext *ctx, tensor_list grad_outputs) {
+        refuse_second_derivative("causal_conv");
+        const auto saved = ctx->get_saved_variables();
+        const ConvInputs in = {saved[0], saved[1], saved[2], saved[3], saved[4]};
+        const auto track = ctx->saved_data["track"].toIntVector();
+        const DeviceGuard guard(device_of(in.x));
+        auto p = in.call();
+        p.silu = ctx->saved_data["silu"].toBool() ? 1 : 0;
+        const torch::Tensor up = grad_outputs[0].defined() ? dense_last(grad_outputs[0])
+                                                           : torch::zeros(in.x.sizes(), in.x.options());
+        torch::Tensor glast;
+        if (grad_outputs.size() > 1 && grad_outputs[1].defined()) glast = grad_outputs[1].contiguous();
+        const auto f32 = in.x.options().dtype(at::ScalarType::Float);
+        torch::Tensor gx = torch::empty(in.x.sizes(), in.x.options()), gw, gb, ginitial, workspace;
+        if (track[0]) gw = torch::empty({p.E, p.K}, f32);
+        if (track[1]) gb = torch::empty({p.E}, f32);
+        if (track[2]) ginitial = torch::empty(in.initial.sizes(), in.x.options());
+        if (track[0] || track[1])
+            workspace = bytes_like(in.x, warpctct_causal_conv_workspace_bytes(p.N, p.L, p.E, p.K));
+        warpctct_conv_grad_t g = {};
+        g.grad_n = up.stride(0);
+        g.grad_t = up.stride(1);
+        g.grad_out = up.data_ptr();
+        g.grad_last = ptr(glast);
+        g.grad_x = gx.data_ptr();
+        g.grad_initial = ginitial.defined() ? ginitial.data_ptr() : nullptr;
+        g.grad_weight = floats(gw);
+        g.grad_bias = floats(gb);
+        check_rc(warpctct_causal_conv_grad(&p, &g, workspace.defined() ? workspace.data_ptr() : nullptr,
+                                           workspace.defined() ? workspace.numel() : 0, current_stream()),
+                 "causal_conv");
+        return {gx, gw, gb, ginitial, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(),
+                torch::Tensor(), torch::Tensor()};
+    }
+};
+
+// weight (E, K) and bias (E), in float32
+void check_taps(const torch::Tensor &weight, const Maybe &bias, const torch::Tensor &x, const char *what) {
+    TORCH_CHECK(weight.dim() == 2 && weight.size(0) == x.size(-1) && weight.size(1) >= 1 &&
+                    weight.size(1) <= WARPCTCT_CONV_MAX_TAPS,
+                what, ": weight must be (channels, taps) with 1 to ", static_cast<int>(WARPCTCT_CONV_MAX_TAPS),
+                " taps");
+    check_on(weight, x, "weight");
+    if (!given(bias)) return;
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == x.size(-1), what, ": bias must have one element a channel");
+    check_on(*bias, x, "bias");
+}
+torch::Tensor as_float(const torch::Tensor &t) { return t.to(at::ScalarType::Float).contiguous(); }
+
+tensor_list causal_conv(const torch::Tensor &input, const torch::Tensor &weight, const Maybe &bias,
+                        const Maybe &lengths, const Maybe &initial, const bool silu, const bool want_state) {
+    CHECK_DEVICE(input);
+    TORCH_CHECK(input.dim() == 3 && input.size(2) >= 1, "causal_conv: the input must be (batch, time, channels)");
+    const torch::Tensor x = dense_last(native(input));
+    check_taps(weight, bias, x, "causal_conv");
+    const int L = int_size(x, 1, "causal_conv"), E = int_size(x, 2, "causal_conv");
+    TORCH_CHECK(x.size(0) <= 65535 && static_cast<long>(L) * E < (1L << 38),
+                "causal_conv: at most 65535 sequences of fewer than 2^38 elements");
+    ConvInputs in = {x, as_float(weight), given(bias) ? as_float(*bias) : torch::Tensor(),
+                     lengths_of(lengths, x, "causal_conv"), torch::Tensor()};
+    if (given(initial)) {
+        TORCH_CHECK(initial->dim() == 3 && initial->size(0) == x.size(0) &&
+                        initial->size(1) == weight.size(1) - 1 && initial->size(2) == E &&
+                        initial->scalar_type() == x.scalar_type(),
+                    "causal_conv: initial_state must be (batch, taps - 1, channels) in the input's type");
+        check_on(*initial, x, "initial_state");
+        in.initial = initial->contiguous();
+    }
+    const bool tw = tracked(in.weight), tb = tracked(in.bias), ti = tracked(in.initial);
+    if (!(tracked(in.x) || tw || tb || ti)) return conv_forward(in, silu, want_state);
+    const auto maybe = [](const torch::Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); };
+    return CausalConv::apply(in.x, in.weight, maybe(in.bias), maybe(in.initial), maybe(in.lengths), silu, want_state,
+                             tw, tb, ti);
+}
+
+torch::Tensor causal_conv_step(const torch::Tensor &input, torch::Tensor state, const torch::Tensor &weight,
+                               const Maybe &bias, const bool silu, const Maybe &advance) {
+    CHECK_DEVICE(input);
+    TORCH_CHECK(input.dim() == 2 && input.size(1) >= 1, "causal_conv_step: the input must be (batch, channels)");
+    const torch::Tensor x = dense_last(native(input));
+    check_taps(weight, bias, x, "causal_conv_step");
+    const Maybe all[4] = {x, state, weight, bias};
+    refuse_gradient({&all[0], &all[1], &all[2], &all[3]}, "causal_conv_step");
+    TORCH_CHECK(state.dim() == 3 && state.size(0) == x.size(0) && state.size(1) == weight.size(1) - 1 &&
+                    state.size(2) == x.size(1) && state.scalar_type() == x.scalar_type() && state.is_contiguous(),
+                "causal_conv_step: state must be (batch, taps - 1, channels), dense, in the input's type");
+    check_on(state, x, "state");
+    const torch::Tensor go = flags_of(advance, x, "causal_conv_step");
+    const torch::Tensor w = as_float(weight), b = given(bias) ? as_float(*bias) : torch::Tensor();
+    const DeviceGuard guard(device_of(x));
+    auto out = torch::empty(x.sizes(), x.options());
+    warpctct_conv_step_t p = {};
+    p.dtype = type_of(x);
+    p.N = int_size(x, 0, "causal_conv_step");
+    p.E = int_size(x, 1, "causal_conv_step");
+    p.K = static_cast<int>(weight.size(1));
+    p.silu = silu ? 1 : 0;
+    p.x_n = x.stride(0);
+    p.x = x.data_ptr();
+    p.state = state.data_ptr();
+    p.weight = floats(w);
+    p.bias = floats(b);
+    p.advance = go.defined() ? reinterpret_cast<const unsigned char *>(go.data_ptr<bool>()) : nullptr;
+    p.out = out.data_ptr();
+    check_rc(warpctct_causal_conv_step(&p, current_stream()), "causal_conv_step");
+    return out;
+}
+
 }  // namespace
 
 void define_network(pybind11::module &m) {
     m.def("layer_norm", &layer_norm, "Layer norm over the last dimension, differentiable.",
           pybind11::arg("x"), pybind11::arg("weight") = pybind11::none(),
           pybind11::arg("bias") = pybind11::none(), pybind11::arg("eps") = 1e-5);
+    m.def("causal_conv", &causal_conv, "Short causal convolution along time, differentiable.",
+          pybind11::arg("x"), pybind11::arg("weight"), pybind11::arg("bias"), pybind11::arg("lengths"),
+          pybind11::arg("initial_state"), pybind11::arg("silu"), pybind11::arg("return_state"));
+    m.def("causal_conv_step", &causal_conv_step, "One step of causal_conv; updates the state in place.",
+          pybind11::arg("x"), pybind11::arg("state"), pybind11::arg("weight"), pybind11::arg("bias"),
+          pybind11::arg("silu"), pybind11::arg("advance"));
 }

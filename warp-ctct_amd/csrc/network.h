@@ -19,8 +19,19 @@ hipError_t launch_layer_norm_grad(const warpctct_norm_t &p, const warpctct_norm_
 
 // out[column] = sum over `rows` rows of partial (rows, columns), in a fixed
 // order; the first `split` columns go to `first`, the others to `second`, in
-// the element type given for each (either pointer may be null).
-hipError_t launch_column_sums(const float *partial, long rows, int columns, int split, void *first,
+// the element type given for each (either pointer may be null).  `partial`
+// holds column_sums_floats(rows, columns) floats: the rows, and behind them room
+// for a second level where there are many.
+size_t column_sums_floats(long rows, long columns);
+hipError_t launch_column_sums(float *partial, long rows, int columns, int split, void *first,
                               int first_type, void *second, int second_type, hipStream_t stream);
+
+hipError_t launch_conv(const warpctct_conv_t &p, hipStream_t stream);
+// tiles of time that a sequence is cut into by the backward pass, each of which
+// leaves (K + 1) * E partial sums per sequence
+int conv_grad_tiles(int N, int L, int E);
+hipError_t launch_conv_grad(const warpctct_conv_t &p, const warpctct_conv_grad_t &g, float *partial,
+                            hipStream_t stream);
+hipError_t launch_conv_step(const warpctct_conv_step_t &p, hipStream_t stream);
 
 }  // namespace wctct

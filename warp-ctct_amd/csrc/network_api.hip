@@ -18,11 +18,18 @@ inline int done(hipError_t e) {
 }
 
 constexpr long kMostRows = 0x7fffffffL;
+constexpr int kMostBatch = 65535;      // a grid dimension, as for the losses
 
 bool norm_ok(const warpctct_norm_t *p) {
     return p && io_valid(p->dtype) && (p->weight_dtype == p->dtype || p->weight_dtype == WARPCTCT_F32) &&
            p->width >= 1 && p->width <= 0x3fffffff && p->rows >= 0 && p->rows <= kMostRows &&
            (p->rows == 0 || (p->x && p->x_inner_rows >= 1));
+}
+
+bool conv_ok(const warpctct_conv_t *p) {
+    return p && io_valid(p->dtype) && p->N >= 0 && p->N <= kMostBatch && p->L >= 0 && p->E >= 1 && p->K >= 1 &&
+           p->K <= WARPCTCT_CONV_MAX_TAPS && (long)p->E * (p->K + 1) < (1L << 30) && (long)p->L * p->E < (1L << 38) &&
+           (p->N == 0 || (p->weight && (p->x || p->L == 0)));
 }
 
 }  // namespace
@@ -39,7 +46,7 @@ int warpctct_layer_norm(const warpctct_norm_t *p, void *stream) {
 size_t warpctct_layer_norm_workspace_bytes(long rows, int width) {
     if (rows < 0 || rows > kMostRows || width < 1) return 0;
     const long groups = rows > 0 ? norm_grad_groups(rows, width) : 1;
-    return (size_t)groups * 2 * (size_t)width * sizeof(float);
+    return column_sums_floats(groups, 2L * width) * sizeof(float);
 }
 
 int warpctct_layer_norm_grad(const warpctct_norm_t *p, const warpctct_norm_grad_t *g, void *workspace,
@@ -58,6 +65,39 @@ int warpctct_layer_norm_grad(const warpctct_norm_t *p, const warpctct_norm_grad_
     }
     if (!g->grad_x && !columns) return WARPCTCT_OK;
     return done(launch_layer_norm_grad(*p, *g, partial, as_stream(stream)));
+}
+
+int warpctct_causal_conv(const warpctct_conv_t *p, void *stream) {
+    if (!conv_ok(p)) return WARPCTCT_EINVAL;
+    if (p->N == 0) return WARPCTCT_OK;
+    if (!p->out && p->L > 0) return WARPCTCT_EINVAL;
+    return done(launch_conv(*p, as_stream(stream)));
+}
+
+size_t warpctct_causal_conv_workspace_bytes(int N, int L, int E, int K) {
+    if (N < 0 || L < 0 || E < 1 || K < 1 || K > WARPCTCT_CONV_MAX_TAPS) return 0;
+    return column_sums_floats((long)N * conv_grad_tiles(N, L, E), (long)E * (K + 1)) * sizeof(float);
+}
+
+int warpctct_causal_conv_grad(const warpctct_conv_t *p, const warpctct_conv_grad_t *g, void *workspace,
+                              size_t workspace_bytes, void *stream) {
+    if (!conv_ok(p) || !g) return WARPCTCT_EINVAL;
+    const bool columns = g->grad_weight || g->grad_bias;
+    if (p->N > 0 && p->L > 0 && (!g->grad_out || !g->grad_x)) return WARPCTCT_EINVAL;
+    const size_t need = warpctct_causal_conv_workspace_bytes(p->N, p->L, p->E, p->K);
+    if (columns && need > 0 && !workspace) return WARPCTCT_EINVAL;
+    if (columns && workspace_bytes < need) return WARPCTCT_EWORKSPACE;
+    float *partial = columns ? static_cast<float *>(workspace) : nullptr;
+    return done(launch_conv_grad(*p, *g, partial, as_stream(stream)));
+}
+
+int warpctct_causal_conv_step(const warpctct_conv_step_t *p, void *stream) {
+    if (!p || !io_valid(p->dtype) || p->N < 0 || p->E < 1 || p->K < 1 || p->K > WARPCTCT_CONV_MAX_TAPS ||
+        (long)p->N * p->E >= (1L << 38))
+        return WARPCTCT_EINVAL;
+    if (p->N == 0) return WARPCTCT_OK;
+    if (!p->x || !p->weight || !p->out || (p->K > 1 && !p->state)) return WARPCTCT_EINVAL;
+    return done(launch_conv_step(*p, as_stream(stream)));
 }
 
 }  // extern "C"

@@ -304,38 +304,6 @@ __global__ __launch_bounds__(kThreads) void norm_wide_columns_kernel(
     mine[width + k] = gb;
 }
 
-// 64 columns by 16 strands of rows; the strands are added up in order.
-constexpr int kStrands = 16;
-__device__ __forceinline__ void store_as(void *p, int type, int at, float v) {
-    if (type == kIoF32)
-        static_cast<float *>(p)[at] = v;
-    else if (type == kIoF16)
-        static_cast<f16 *>(p)[at] = (f16)v;
-    else
-        static_cast<bf16 *>(p)[at] = (bf16)v;
-}
-__global__ __launch_bounds__(64 * kStrands) void column_sums_kernel(const float *__restrict__ partial, long rows,
-                                                                    int columns, int split,
-                                                                    void *__restrict__ first, int first_type,
-                                                                    void *__restrict__ second, int second_type) {
-    __shared__ float strands[kStrands][64];
-    const int lane = threadIdx.x & 63, strand = threadIdx.x >> 6, k = blockIdx.x * 64 + lane;
-    float sum = 0.0f;
-    if (k < columns) {
-#pragma unroll 8
-        for (long r = strand; r < rows; r += kStrands) sum += partial[r * columns + k];
-    }
-    strands[strand][lane] = sum;
-    __syncthreads();
-    if (strand != 0 || k >= columns) return;
-    for (int s = 1; s < kStrands; ++s) sum += strands[s][lane];
-    if (k < split) {
-        if (first) store_as(first, first_type, k, sum);
-    } else if (second) {
-        store_as(second, second_type, k - split, sum);
-    }
-}
-
 RowAddress address(long rows, long inner_rows, long outer_stride, long inner_stride) {
     RowAddress a;
     a.inner = inner_rows >= rows ? 0u : (unsigned)inner_rows;
@@ -470,13 +438,6 @@ hipError_t launch_layer_norm_grad(const warpctct_norm_t &p, const warpctct_norm_
     if (e != hipSuccess || !partial) return e;
     return launch_column_sums(partial, norm_grad_groups(p.rows, p.width), 2 * p.width, p.width, g.grad_weight,
                               p.weight_dtype, g.grad_bias, p.weight_dtype, stream);
-}
-
-hipError_t launch_column_sums(const float *partial, long rows, int columns, int split, void *first, int first_type,
-                              void *second, int second_type, hipStream_t stream) {
-    TIMED_LAUNCH(column_sums_kernel, dim3((columns + 63) / 64), dim3(64 * kStrands), 0, stream, partial, rows,
-                 columns, split, first, first_type, second, second_type);
-    return hipGetLastError();
 }
 
 }  // namespace wctct

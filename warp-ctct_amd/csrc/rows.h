@@ -71,6 +71,35 @@ __device__ __forceinline__ void store_vec(IO *p, const float *x) {
     *reinterpret_cast<raw16 *>(p) = pack16(p, x);
 }
 
+// N elements next to each other, N * sizeof(IO) bytes aligned to themselves:
+// 1 element, 4 elements, or a 16-byte vector
+template <int N, typename IO>
+__device__ __forceinline__ void load_n(const IO *p, float *x) {
+    if constexpr (N == 1) {
+        x[0] = to_float(*p);
+    } else if constexpr (N == kVec<IO>) {
+        load_vec(p, x);
+    } else {
+        static_assert(N == 4 && sizeof(IO) == 2, "half a vector of 2-byte elements");
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        float y[8];
+        unpack16(p, raw16{v.x, v.y, 0u, 0u}, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = y[i];
+    }
+}
+template <int N, typename IO>
+__device__ __forceinline__ void store_n(IO *p, const float *x) {
+    if constexpr (N == 1) {
+        *p = from_float<IO>(x[0]);
+    } else if constexpr (N == kVec<IO>) {
+        store_vec(p, x);
+    } else {
+        static_assert(N == 4 && sizeof(IO) == 2, "half a vector of 2-byte elements");
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack_two(p, x[0], x[1]), pack_two(p, x[2], x[3]));
+    }
+}
+
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
     return __uint_as_float(

@@ -2,9 +2,10 @@
 the rules put on the joiner's logits before a token is taken from them.
 
 The losses start from scores.  These are the operators on either side of them
-that a model of the same kind runs: :func:`layer_norm` for a prediction network
-or an encoder, in training.  Hand-written HIP kernels
-like the losses', through the same binding: float32, float16 and bfloat16 are
+that a model of the same kind runs: :func:`layer_norm` and
+:func:`causal_conv` for a prediction network or an encoder, in training, and
+:func:`causal_conv_step` for decoding a token at a time.  Hand-written HIP
+kernels like the losses', through the same binding: float32, float16 and bfloat16 are
 read as they are (another type is converted to float32), sums and states are
 kept in float32, a result is rounded once.  Nothing synchronises with the host;
 work is enqueued on the current stream of the input's GPU.  A wrong shape, type
@@ -39,3 +40,55 @@ def layer_norm(x: torch.Tensor,
     Differentiable with respect to ``x``, ``weight`` and ``bias``.  The gradients
     of the parameters are added up in a fixed order: the same on every call."""
     return core.layer_norm(x, weight, bias, float(eps))
+
+
+def _activation(name: Optional[str]) -> bool:
+    if name not in (None, "silu"):
+        raise RuntimeError("activation must be None or 'silu', got %r" % (name,))
+    return name == "silu"
+
+
+def causal_conv(x: torch.Tensor,
+                weight: torch.Tensor,
+                bias: Optional[torch.Tensor] = None,
+                lengths: Optional[torch.Tensor] = None,
+                initial_state: Optional[torch.Tensor] = None,
+                activation: Optional[str] = None,
+                return_state: bool = False):
+    """A short convolution along time, every channel with its own taps:
+    ``out[n, t, e] = act(bias[e] + sum_k weight[e, k] * x[n, t - (K-1) + k, e])``.
+
+    Args:
+        x: (N, T, E).  A view with a dense last dimension is read in place.
+        weight: (E, K), K from 1 to 8; the last tap is the current step's.
+        bias: (E,) or None.
+        lengths: (N,) steps of each sequence; the steps behind them are not read
+            and their outputs (and gradients) are zero.  None: all T.
+        initial_state: (N, K-1, E), the inputs in front of ``x``, in the type of
+            ``x``.  None: zeros.
+        activation: None or ``'silu'``.
+        return_state: also return (N, K-1, E), the last K-1 inputs of every
+            sequence: the ``initial_state`` of a call that goes on from there, and
+            the ``state`` of :func:`causal_conv_step`.
+
+    Returns out (N, T, E), or ``(out, state)``.  Differentiable with respect to
+    ``x``, ``weight``, ``bias`` and ``initial_state``, through both results; the
+    gradients of the parameters are added up in a fixed order."""
+    got = core.causal_conv(x, weight, bias, lengths, initial_state, _activation(activation), bool(return_state))
+    return (got[0], got[1]) if return_state else got[0]
+
+
+def causal_conv_step(x: torch.Tensor,
+                     state: torch.Tensor,
+                     weight: torch.Tensor,
+                     bias: Optional[torch.Tensor] = None,
+                     activation: Optional[str] = None,
+                     advance: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One step of :func:`causal_conv` for N sequences: ``x`` (N, E) comes in,
+    ``state`` (N, K-1, E) moves on in place, out (N, E) is returned.
+
+    ``advance`` (N,) bool, None for all: a sequence that does not advance keeps
+    its state, and its row of the result is zero (a hypothesis that took blank
+    keeps the output of its last label).  Not differentiable: call it under
+    ``torch.no_grad()``."""
+    return core.causal_conv_step(x, state, weight, bias, _activation(activation), advance)
