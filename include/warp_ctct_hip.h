@@ -598,6 +598,34 @@ typedef struct {
 } warpctct_conv_step_t;
 int warpctct_causal_conv_step(const warpctct_conv_step_t *p, void *stream);
 
+/* ---- beside the losses: rules on logits ------------------------------------
+ * logits (N, V), rows logits_n elements apart -> out (N, V) dense, may be the
+ * same memory where the rows are V apart.  With count[n][v] = how often v stands
+ * among the first tokens_lengths[n] (NULL: H; clamped into [0, H]) of tokens
+ * (N, H; int32, or int64 with tokens_64; rows tokens_n apart; NULL: none; values
+ * outside [0, V) count for nothing), in float32:
+ *   l = logits[n][v]
+ *   where count > 0:  l = l > 0 ? l / repetition : l * repetition
+ *                     l = l - presence - frequency * count
+ *   l = l + bias[n * bias_n + v]       (bias NULL: 0; bias_n 0: one for all rows)
+ *   out = allowed ? l : -infinity
+ * repetitions / presences / frequencies: one for each row, or NULL for the
+ * values in front of them.  allowed: bytes, or with allowed_packed 32-bit words
+ * of which bit v % 32 of word v / 32 is that of column v; row n allowed_n bytes
+ * or words further on (0: one for all rows); NULL: everything.  A row that
+ * allows nothing is -infinity throughout.  N <= 65535, V <= 2^30. */
+typedef struct {
+    int dtype, N, V, H, tokens_64, bias_dtype, allowed_packed;
+    float repetition, presence, frequency;
+    long logits_n, tokens_n, bias_n, allowed_n;
+    const void *logits, *tokens;
+    const int *tokens_lengths;
+    const float *repetitions, *presences, *frequencies;
+    const void *bias, *allowed;
+    void *out;
+} warpctct_adjust_t;
+int warpctct_adjust_logits(const warpctct_adjust_t *p, void *stream);
+
 /* ---- measurement aid ------------------------------------------------------
  * No counterpart in the reference.  warpctct_profile(1) clears earlier records
  * and starts bracketing every kernel launch of the library with two HIP events

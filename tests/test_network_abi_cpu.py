@@ -124,3 +124,26 @@ def test_causal_conv_gradient_and_step_arguments():
                 dict(weight=None), dict(out=None)):
         assert step(**bad) == EINVAL, bad
     assert step(N=0, x=None, state=None) == 0
+
+
+class Adjust(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_int) for k in ("dtype", "N", "V", "H", "tokens_64", "bias_dtype", "allowed_packed")] + [
+        (k, ctypes.c_float) for k in ("repetition", "presence", "frequency")] + [
+        (k, ctypes.c_long) for k in ("logits_n", "tokens_n", "bias_n", "allowed_n")] + [
+        (k, P) for k in ("logits", "tokens", "tokens_lengths", "repetitions", "presences", "frequencies", "bias",
+                         "allowed", "out")]
+
+
+def test_adjust_logits_arguments():
+    lib = hip_lib.lib()
+
+    def call(**over):
+        fields = dict(dtype=F32, N=2, V=8, H=0, repetition=1.0, logits_n=8, logits=SOME, out=SOME)
+        fields.update(over)
+        return lib.warpctct_adjust_logits(ctypes.byref(Adjust(**fields)), P(0))
+
+    assert lib.warpctct_adjust_logits(P(0), P(0)) == EINVAL
+    for bad in (dict(dtype=3), dict(N=-1), dict(N=65536), dict(V=0), dict(V=(1 << 30) + 1), dict(H=-1),
+                dict(bias=SOME, bias_dtype=3), dict(logits=None), dict(out=None)):
+        assert call(**bad) == EINVAL, bad
+    assert call(N=0, logits=None, out=None) == 0

@@ -1,5 +1,5 @@
 // The operators beside the losses, for torch: layer norm and the causal
-// convolution, the latter also one step at a time.  Each is differentiable where it has a backward pass; without gradients to
+// convolution, the latter also one step at a time, and the rules on logits.  Each is differentiable where it has a backward pass; without gradients to
 // track it goes straight to the C ABI.  Arguments are checked here (RuntimeError
 // through TORCH_CHECK); nothing synchronises with the host.
 #include "binding_common.h"
@@ -391,6 +391,102 @@ torch::Tensor causal_conv_step(const torch::Tensor &input, torch::Tensor state, 
     return out;
 }
 
+// ---- rules on logits ---------------------------------------------------------------
+
+// a penalty: one number for all rows, or a tensor with one for each
+struct Penalty {
+    float all = 0.0f;
+    torch::Tensor each;
+    Penalty(const pybind11::object &given, const torch::Tensor &logits, const char *name) {
+        if (!THPVariable_Check(given.ptr())) {
+            all = given.cast<float>();
+            return;
+        }
+        const auto t = given.cast<torch::Tensor>();
+        TORCH_CHECK(t.dim() == 1 && t.size(0) == logits.size(0), "adjust_logits: ", name,
+                    " must be a number or one for each row");
+        check_on(t, logits, name);
+        refuse_if_tracked(t, name);
+        each = t.to(at::ScalarType::Float).contiguous();
+    }
+    static void refuse_if_tracked(const torch::Tensor &t, const char *name) {
+        TORCH_CHECK(!tracked(t), "adjust_logits: not differentiable (", name, "); call it under torch.no_grad()");
+    }
+};
+
+torch::Tensor adjust_logits(const torch::Tensor &input, const Maybe &tokens, const Maybe &tokens_lengths,
+                            const pybind11::object &repetition, const pybind11::object &presence,
+                            const pybind11::object &frequency, const Maybe &bias, const Maybe &allowed) {
+    CHECK_DEVICE(input);
+    TORCH_CHECK(input.dim() == 2 && input.size(1) >= 1 && input.size(1) <= (1L << 30) && input.size(0) <= 65535,
+                "adjust_logits: the logits must be (rows, vocabulary), at most 65535 rows of at most 2^30");
+    Penalty::refuse_if_tracked(input, "logits");
+    const torch::Tensor x = dense_last(native(input));
+    const int64_t N = x.size(0), V = x.size(1);
+    warpctct_adjust_t p = {};
+    p.dtype = type_of(x);
+    p.N = static_cast<int>(N);
+    p.V = static_cast<int>(V);
+    p.logits_n = x.stride(0);
+    p.logits = x.data_ptr();
+    const Penalty rep(repetition, x, "repetition_penalty"), pre(presence, x, "presence_penalty"),
+        fre(frequency, x, "frequency_penalty");
+    TORCH_CHECK(rep.each.defined() || rep.all > 0.0f, "adjust_logits: repetition_penalty must be positive");
+    p.repetition = rep.all;
+    p.presence = pre.all;
+    p.frequency = fre.all;
+    p.repetitions = floats(rep.each);
+    p.presences = floats(pre.each);
+    p.frequencies = floats(fre.each);
+    torch::Tensor history, lengths, b, mask;
+    if (given(tokens)) {
+        const auto type = tokens->scalar_type();
+        TORCH_CHECK(tokens->dim() == 2 && tokens->size(0) == N && !tokens->is_floating_point() &&
+                        type != at::ScalarType::Bool && tokens->size(1) <= 0x7fffffff,
+                    "adjust_logits: tokens must be whole numbers, (rows, history)");
+        check_on(*tokens, x, "tokens");
+        const bool taken = type == at::ScalarType::Int || type == at::ScalarType::Long;
+        history = dense_last(taken ? *tokens : tokens->to(at::ScalarType::Int));
+        p.H = static_cast<int>(history.size(1));
+        p.tokens_64 = history.scalar_type() == at::ScalarType::Long ? 1 : 0;
+        p.tokens_n = history.stride(0);
+        p.tokens = history.data_ptr();
+        if (given(tokens_lengths)) {
+            lengths = lengths_of(tokens_lengths, x, "adjust_logits");
+            p.tokens_lengths = lengths.data_ptr<int>();
+        }
+    } else {
+        TORCH_CHECK(!given(tokens_lengths), "adjust_logits: tokens_lengths without tokens");
+    }
+    const auto rows_of = [&](const torch::Tensor &t, int64_t width, const char *name) {
+        TORCH_CHECK((t.dim() == 1 || (t.dim() == 2 && t.size(0) == N)) && t.size(-1) == width, "adjust_logits: ",
+                    name, " must have ", width, " columns, for all rows or for each");
+        check_on(t, x, name);
+        return dense_last(t);
+    };
+    if (given(bias)) {
+        Penalty::refuse_if_tracked(*bias, "bias");
+        b = rows_of(native(*bias), V, "bias");
+        p.bias_dtype = type_of(b);
+        p.bias_n = b.dim() == 2 ? b.stride(0) : 0;
+        p.bias = b.data_ptr();
+    }
+    if (given(allowed)) {
+        const bool packed = allowed->scalar_type() == at::ScalarType::Int;
+        TORCH_CHECK(packed || allowed->scalar_type() == at::ScalarType::Bool,
+                    "adjust_logits: allowed must be truth values, or int32 words of 32 bits each");
+        mask = rows_of(*allowed, packed ? (V + 31) / 32 : V, "allowed");
+        p.allowed_packed = packed ? 1 : 0;
+        p.allowed_n = mask.dim() == 2 ? mask.stride(0) : 0;
+        p.allowed = mask.data_ptr();
+    }
+    const DeviceGuard guard(device_of(x));
+    auto out = torch::empty(x.sizes(), x.options());
+    p.out = out.data_ptr();
+    check_rc(warpctct_adjust_logits(&p, current_stream()), "adjust_logits");
+    return out;
+}
+
 }  // namespace
 
 void define_network(pybind11::module &m) {
@@ -403,4 +499,8 @@ void define_network(pybind11::module &m) {
     m.def("causal_conv_step", &causal_conv_step, "One step of causal_conv; updates the state in place.",
           pybind11::arg("x"), pybind11::arg("state"), pybind11::arg("weight"), pybind11::arg("bias"),
           pybind11::arg("silu"), pybind11::arg("advance"));
+    m.def("adjust_logits", &adjust_logits, "Penalties, biases and masks on logits.", pybind11::arg("logits"),
+          pybind11::arg("tokens"), pybind11::arg("tokens_lengths"), pybind11::arg("repetition_penalty"),
+          pybind11::arg("presence_penalty"), pybind11::arg("frequency_penalty"), pybind11::arg("bias"),
+          pybind11::arg("allowed"));
 }

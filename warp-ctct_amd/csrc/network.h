@@ -34,4 +34,6 @@ hipError_t launch_conv_grad(const warpctct_conv_t &p, const warpctct_conv_grad_t
                             hipStream_t stream);
 hipError_t launch_conv_step(const warpctct_conv_step_t &p, hipStream_t stream);
 
+hipError_t launch_adjust(const warpctct_adjust_t &p, hipStream_t stream);
+
 }  // namespace wctct

@@ -4,8 +4,8 @@ the rules put on the joiner's logits before a token is taken from them.
 The losses start from scores.  These are the operators on either side of them
 that a model of the same kind runs: :func:`layer_norm` and
 :func:`causal_conv` for a prediction network or an encoder, in training, and
-:func:`causal_conv_step` for decoding a token at a time.  Hand-written HIP
-kernels like the losses', through the same binding: float32, float16 and bfloat16 are
+:func:`causal_conv_step` for decoding a token at a time; :func:`adjust_logits`
+before a token is taken.  Hand-written HIP kernels like the losses', through the same binding: float32, float16 and bfloat16 are
 read as they are (another type is converted to float32), sums and states are
 kept in float32, a result is rounded once.  Nothing synchronises with the host;
 work is enqueued on the current stream of the input's GPU.  A wrong shape, type
@@ -16,7 +16,7 @@ on the same leaves must be gone before a backward pass is captured.
 
 The reference has no counterpart: its callers take these from torch.
 """
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
@@ -92,3 +92,39 @@ def causal_conv_step(x: torch.Tensor,
     keeps the output of its last label).  Not differentiable: call it under
     ``torch.no_grad()``."""
     return core.causal_conv_step(x, state, weight, bias, _activation(activation), advance)
+
+
+def adjust_logits(logits: torch.Tensor,
+                  tokens: Optional[torch.Tensor] = None,
+                  tokens_lengths: Optional[torch.Tensor] = None,
+                  repetition_penalty: Union[float, torch.Tensor] = 1.0,
+                  presence_penalty: Union[float, torch.Tensor] = 0.0,
+                  frequency_penalty: Union[float, torch.Tensor] = 0.0,
+                  bias: Optional[torch.Tensor] = None,
+                  allowed: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The rules that a decoder puts on logits before it takes a token, in one
+    pass: penalties for the tokens a row holds already, then a bias, then a mask.
+    For every column ``v`` that stands ``count > 0`` times among a row's tokens::
+
+        l = l / repetition_penalty if l > 0 else l * repetition_penalty
+        l = l - presence_penalty - frequency_penalty * count
+
+    then ``l + bias``, and minus infinity where ``allowed`` is not set.
+
+    Args:
+        logits: (N, V).
+        tokens: (N, H) whole numbers, or None; values outside [0, V) (padding)
+            count for nothing.
+        tokens_lengths: (N,) how many of a row's tokens count.  None: all H.
+        repetition_penalty, presence_penalty, frequency_penalty: a number, or
+            (N,) with one for each row.  A repetition penalty is positive.
+        bias: (V,) or (N, V): of an outer language model, of words to be heard.
+        allowed: what a grammar lets follow: (V,) or (N, V) bool, or the same in
+            bits, int32 (ceil(V/32),) or (N, ceil(V/32)) with bit ``v % 32`` of
+            word ``v // 32`` for column ``v``.  A row that allows nothing comes
+            out as minus infinity throughout.
+
+    Returns a new (N, V) tensor of the type of ``logits``.  Not differentiable:
+    call it under ``torch.no_grad()`` where an input requires a gradient."""
+    return core.adjust_logits(logits, tokens, tokens_lengths, repetition_penalty, presence_penalty,
+                              frequency_penalty, bias, allowed)
