@@ -598,6 +598,71 @@ typedef struct {
 } warpctct_conv_step_t;
 int warpctct_causal_conv_step(const warpctct_conv_step_t *p, void *stream);
 
+/* ---- beside the losses: selective scan --------------------------------------
+ * Every channel e of x (N, L, E) drives S <= WARPCTCT_SCAN_MAX_STATES states:
+ *   d = softplus(dt[n][t][e] + dt_bias[e])        (softplus 0: the sum itself)
+ *   h[s] = exp(d a[e][s]) h[s] + d x[n][t][e] b[n][t][g][s]
+ *   out[n][t][e] = (sum_s c[n][t][g][s] h[s] + skip[e] x[n][t][e]) silu(gate[n][t][e])
+ * with g = e / (E / G) the channel's group (E a multiple of G), silu(v) =
+ * v / (1 + e^-v); skip, dt_bias NULL: 0, gate NULL: no factor.  x, dt, gate, b, c
+ * in one type; element (n, t, e) of x lies at n x_n + t x_t + e, so for dt and
+ * gate, (n, t, g, s) of b at n b_n + t b_t + g b_g + s, so for c.  a (E, S),
+ * skip, dt_bias (E): float, dense.  Of sequence n the first lengths[n] steps
+ * count (NULL: all; clamped into [0, L]): the others are not read and out is zero
+ * there.  initial (N, E, S; NULL: zeros) holds the states in front of the first
+ * step, last (N, E, S; may be NULL) receives those behind the last one that
+ * counts.  out (N, L, E) dense.
+ * keep (warpctct_selective_scan_keep_bytes, 16-byte aligned; NULL without a
+ * backward pass) receives the states in front of every WARPCTCT_SCAN_TILE steps.
+ * N <= 65535. */
+enum { WARPCTCT_SCAN_MAX_STATES = 64, WARPCTCT_SCAN_TILE = 16 };
+typedef struct {
+    int dtype, N, L, E, S, G, softplus;
+    long x_n, x_t, dt_n, dt_t, gate_n, gate_t, b_n, b_t, b_g, c_n, c_t, c_g;
+    const void *x, *dt, *gate, *b, *c;
+    const float *a, *skip, *dt_bias;
+    const int *lengths;
+    const float *initial;
+    void *out;
+    float *last;
+} warpctct_scan_t;
+size_t warpctct_selective_scan_keep_bytes(int N, int L, int E, int S);
+int warpctct_selective_scan(const warpctct_scan_t *p, void *keep, size_t keep_bytes, void *stream);
+
+/* Gradients for grad_out (addressed like x by grad_n, grad_t) and, if not NULL,
+ * grad_last (N, E, S): in the type of x and dense grad_x, grad_dt, grad_gate
+ * (N, L, E; the last NULL without a gate), grad_b, grad_c (N, L, G, S); in float
+ * grad_a (E, S), grad_skip_bias (2, E: those of skip and of dt_bias, formed
+ * whether or not there is one) and grad_initial (N, E, S; may be NULL).  keep as
+ * the forward call left it; `out` and `last` of p are not used.  Sums over
+ * channels, steps and sequences are added up in a fixed order through
+ * `workspace` (warpctct_selective_scan_workspace_bytes, 16-byte aligned). */
+typedef struct {
+    long grad_n, grad_t;
+    const void *grad_out;
+    const float *grad_last;
+    void *grad_x, *grad_dt, *grad_gate, *grad_b, *grad_c;
+    float *grad_a, *grad_skip_bias, *grad_initial;
+} warpctct_scan_grad_t;
+size_t warpctct_selective_scan_workspace_bytes(int N, int L, int E, int S, int G);
+int warpctct_selective_scan_grad(const warpctct_scan_t *p, const warpctct_scan_grad_t *g, const void *keep,
+                                 size_t keep_bytes, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One step for N sequences at once: x, dt, gate (N, E) rows x_n, dt_n, gate_n
+ * apart, b, c (N, G, S), state (N, E, S) float, dense, updated in place, out
+ * (N, E) dense.  A sequence whose advance[n] is 0 (advance may be NULL) keeps its
+ * state, and its row of out is zero. */
+typedef struct {
+    int dtype, N, E, S, G, softplus;
+    long x_n, dt_n, gate_n, b_n, b_g, c_n, c_g;
+    const void *x, *dt, *gate, *b, *c;
+    const float *a, *skip, *dt_bias;
+    float *state;
+    const unsigned char *advance;
+    void *out;
+} warpctct_scan_step_t;
+int warpctct_selective_scan_step(const warpctct_scan_step_t *p, void *stream);
+
 /* ---- beside the losses: rules on logits ------------------------------------
  * logits (N, V), rows logits_n elements apart -> out (N, V) dense, may be the
  * same memory where the rows are V apart.  With count[n][v] = how often v stands

@@ -147,3 +147,89 @@ def test_adjust_logits_arguments():
                 dict(bias=SOME, bias_dtype=3), dict(logits=None), dict(out=None)):
         assert call(**bad) == EINVAL, bad
     assert call(N=0, logits=None, out=None) == 0
+
+
+SCAN_SIZES = ("dtype", "N", "L", "E", "S", "G", "softplus")
+SCAN_STRIDES = ("x_n", "x_t", "dt_n", "dt_t", "gate_n", "gate_t", "b_n", "b_t", "b_g", "c_n", "c_t", "c_g")
+
+
+class Scan(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_int) for k in SCAN_SIZES] + [(k, ctypes.c_long) for k in SCAN_STRIDES] + [
+        (k, P) for k in ("x", "dt", "gate", "b", "c", "a", "skip", "dt_bias", "lengths", "initial", "out", "last")]
+
+
+class ScanGrad(ctypes.Structure):
+    _fields_ = [("grad_n", ctypes.c_long), ("grad_t", ctypes.c_long)] + [
+        (k, P) for k in ("grad_out", "grad_last", "grad_x", "grad_dt", "grad_gate", "grad_b", "grad_c", "grad_a",
+                         "grad_skip_bias", "grad_initial")]
+
+
+class ScanStep(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_int) for k in ("dtype", "N", "E", "S", "G", "softplus")] + [
+        (k, ctypes.c_long) for k in ("x_n", "dt_n", "gate_n", "b_n", "b_g", "c_n", "c_g")] + [
+        (k, P) for k in ("x", "dt", "gate", "b", "c", "a", "skip", "dt_bias", "state", "advance", "out")]
+
+
+ALIGNED = SOME + 15 & ~15
+
+
+def scan(**over):
+    fields = dict(dtype=F32, N=2, L=20, E=8, S=16, G=2, x=SOME, dt=SOME, b=SOME, c=SOME, a=SOME, out=SOME)
+    fields.update(over)
+    return Scan(**fields)
+
+
+BAD_SCANS = (dict(dtype=3), dict(N=-1), dict(N=65536), dict(L=-1), dict(E=0), dict(E=9), dict(S=0), dict(S=65),
+             dict(G=0), dict(x=None), dict(dt=None), dict(a=None), dict(b=None), dict(c=None), dict(E=(1 << 24) + 2))
+
+
+def test_selective_scan_arguments():
+    lib = hip_lib.lib()
+    size = lib.warpctct_selective_scan_keep_bytes
+    size.restype = ctypes.c_size_t
+    assert size(2, 20, 8, 16) == 2 * 2 * 8 * 16 * 4 and size(2, 20, 8, 5) == 2 * 2 * 8 * 8 * 4
+    assert size(2, 0, 8, 16) == 0 and size(2, 20, 8, 65) == 0
+
+    def call(keep=0, have=0, **over):
+        return lib.warpctct_selective_scan(ctypes.byref(scan(**over)), P(keep), ctypes.c_size_t(have), P(0))
+
+    assert lib.warpctct_selective_scan(P(0), P(0), ctypes.c_size_t(0), P(0)) == EINVAL
+    for bad in BAD_SCANS + (dict(out=None),):
+        assert call(**bad) == EINVAL, bad
+    assert call(keep=ALIGNED, have=2047) == EWORKSPACE
+    assert call(keep=ALIGNED + 4, have=1 << 20) == EINVAL
+    assert call(N=0, x=None, dt=None, b=None, c=None, a=None, out=None) == 0
+
+
+def test_selective_scan_gradient_and_step_arguments():
+    lib = hip_lib.lib()
+    size = lib.warpctct_selective_scan_workspace_bytes
+    size.restype = ctypes.c_size_t
+    need = size(2, 20, 8, 16, 2)
+    assert need >= 4 * (2 * 2 * 2 * 16 * 32 + 2 * 8 * 18) and size(2, 20, 9, 16, 2) == 0
+
+    def call(p=None, keep=ALIGNED, kept=1 << 20, workspace=ALIGNED, have=1 << 20, **over):
+        fields = dict(grad_out=SOME, grad_x=SOME, grad_dt=SOME, grad_b=SOME, grad_c=SOME, grad_a=SOME,
+                      grad_skip_bias=SOME)
+        fields.update(over)
+        return lib.warpctct_selective_scan_grad(ctypes.byref(p or scan()), ctypes.byref(ScanGrad(**fields)), P(keep),
+                                                ctypes.c_size_t(kept), P(workspace), ctypes.c_size_t(have), P(0))
+
+    for bad in BAD_SCANS:
+        assert call(scan(**bad)) == EINVAL, bad
+    for bad in ("grad_out", "grad_x", "grad_dt", "grad_b", "grad_c", "grad_a", "grad_skip_bias"):
+        assert call(**{bad: None}) == EINVAL, bad
+    assert call(scan(gate=SOME)) == EINVAL
+    assert call(keep=0) == EINVAL and call(workspace=0) == EINVAL and call(workspace=ALIGNED + 4) == EINVAL
+    assert call(kept=2047) == EWORKSPACE and call(have=need - 1) == EWORKSPACE
+
+    def step(**over):
+        fields = dict(dtype=F16, N=2, E=8, S=16, G=1, x=SOME, dt=SOME, b=SOME, c=SOME, a=SOME, state=SOME, out=SOME)
+        fields.update(over)
+        return lib.warpctct_selective_scan_step(ctypes.byref(ScanStep(**fields)), P(0))
+
+    assert lib.warpctct_selective_scan_step(P(0), P(0)) == EINVAL
+    for bad in (dict(dtype=3), dict(N=-1), dict(E=0), dict(S=65), dict(G=3), dict(x=None), dict(dt=None), dict(a=None),
+                dict(b=None), dict(c=None), dict(state=None), dict(out=None)):
+        assert step(**bad) == EINVAL, bad
+    assert step(N=0, x=None, state=None) == 0

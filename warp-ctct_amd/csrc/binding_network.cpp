@@ -1,7 +1,8 @@
-// The operators beside the losses, for torch: layer norm and the causal
-// convolution, the latter also one step at a time, and the rules on logits.  Each is differentiable where it has a backward pass; without gradients to
-// track it goes straight to the C ABI.  Arguments are checked here (RuntimeError
-// through TORCH_CHECK); nothing synchronises with the host.
+// The operators beside the losses, for torch: layer norm, the causal convolution
+// and the selective scan (the latter two also one step at a time), and the rules
+// on logits.  Each is differentiable where it has a backward pass; without
+// gradients to track it goes straight to the C ABI.  Arguments are checked here
+// (RuntimeError through TORCH_CHECK); nothing synchronises with the host.
 #include "binding_common.h"
 
 namespace {
@@ -391,6 +392,254 @@ torch::Tensor causal_conv_step(const torch::Tensor &input, torch::Tensor state, 
     return out;
 }
 
+// ---- selective scan ----------------------------------------------------------------
+
+struct ScanInputs {
+    torch::Tensor x, dt, a, b, c, skip, gate, dt_bias, lengths, initial;
+    warpctct_scan_t call() const {
+        warpctct_scan_t p = {};
+        p.dtype = type_of(x);
+        p.N = static_cast<int>(x.size(0));
+        p.L = static_cast<int>(x.size(1));
+        p.E = static_cast<int>(x.size(2));
+        p.S = static_cast<int>(a.size(1));
+        p.G = static_cast<int>(b.size(2));
+        p.x_n = x.stride(0);
+        p.x_t = x.stride(1);
+        p.dt_n = dt.stride(0);
+        p.dt_t = dt.stride(1);
+        if (gate.defined()) {
+            p.gate_n = gate.stride(0);
+            p.gate_t = gate.stride(1);
+        }
+        p.b_n = b.stride(0);
+        p.b_t = b.stride(1);
+        p.b_g = b.stride(2);
+        p.c_n = c.stride(0);
+        p.c_t = c.stride(1);
+        p.c_g = c.stride(2);
+        p.x = x.data_ptr();
+        p.dt = dt.data_ptr();
+        p.gate = ptr(gate);
+        p.b = b.data_ptr();
+        p.c = c.data_ptr();
+        p.a = floats(a);
+        p.skip = floats(skip);
+        p.dt_bias = floats(dt_bias);
+        p.lengths = lengths.defined() ? lengths.data_ptr<int>() : nullptr;
+        p.initial = floats(initial);
+        return p;
+    }
+};
+
+// out, the last states if wanted, and what the backward pass needs
+std::tuple<tensor_list, torch::Tensor> scan_forward(const ScanInputs &in, bool softplus, bool want_state,
+                                                    bool for_backward) {
+    const DeviceGuard guard(device_of(in.x));
+    auto p = in.call();
+    p.softplus = softplus ? 1 : 0;
+    tensor_list outs = {torch::empty(in.x.sizes(), in.x.options())};
+    if (want_state)
+        outs.push_back(torch::empty({p.N, p.E, p.S}, in.x.options().dtype(at::ScalarType::Float)));
+    p.out = outs[0].data_ptr();
+    p.last = want_state ? floats(outs[1]) : nullptr;
+    torch::Tensor keep;
+    if (for_backward) keep = bytes_like(in.x, warpctct_selective_scan_keep_bytes(p.N, p.L, p.E, p.S));
+    check_rc(warpctct_selective_scan(&p, keep.defined() ? keep.data_ptr() : nullptr, keep.defined() ? keep.numel() : 0,
+                                     current_stream()),
+             "selective_scan");
+    return std::make_tuple(outs, keep);
+}
+
+class SelectiveScan : public torch::autograd::Function<SelectiveScan> {
+   public:
+    static tensor_list forward(AutogradContext *ctx, const torch::Tensor &x, const torch::Tensor &dt,
+                               const torch::Tensor &a, const torch::Tensor &b, const torch::Tensor &c,
+                               const Maybe &skip, const Maybe &gate, const Maybe &dt_bias, const Maybe &initial,
+                               const Maybe &lengths, const bool softplus, const bool want_state,
+                               const bool track_initial) {
+        const auto plain = [](const Maybe &t) { return given(t) ? *t : torch::Tensor(); };
+        const ScanInputs in = {x, dt, a, b, c, plain(skip), plain(gate), plain(dt_bias), plain(lengths),
+                               plain(initial)};
+        auto got = scan_forward(in, softplus, want_state, true);
+        ctx->save_for_backward({in.x, in.dt, in.a, in.b, in.c, in.skip, in.gate, in.dt_bias, in.lengths, in.initial,
+                                std::get<1>(got)});
+        ctx->saved_data["softplus"] = softplus;
+        ctx->saved_data["track_initial"] = track_initial;
+        ctx->set_materialize_grads(false);
+        return std::get<0>(got);
+    }
+
+    static tensor_list backward(AutogradContext *ctx, tensor_list grad_outputs) {
+        refuse_second_derivative("selective_scan");
+        const auto s = ctx->get_saved_variables();
+        const ScanInputs in = {s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9]};
+        const torch::Tensor &x = in.x, &keep = s[10];
+        const DeviceGuard guard(device_of(x));
+        auto p = in.call();
+        p.softplus = ctx->saved_data["softplus"].toBool() ? 1 : 0;
+        const torch::Tensor up =
+            grad_outputs[0].defined() ? dense_last(grad_outputs[0]) : torch::zeros(x.sizes(), x.options());
+        torch::Tensor glast;
+        if (grad_outputs.size() > 1 && grad_outputs[1].defined()) glast = grad_outputs[1].contiguous();
+        const auto f32 = x.options().dtype(at::ScalarType::Float);
+        torch::Tensor gx = torch::empty(x.sizes(), x.options()), gdt = torch::empty(x.sizes(), x.options()), gz,
+                      gb = torch::empty(in.b.sizes(), x.options()), gc = torch::empty(in.c.sizes(), x.options()),
+                      ga = torch::empty({p.E, p.S}, f32), two = torch::empty({2, p.E}, f32), ginitial;
+        if (in.gate.defined()) gz = torch::empty(x.sizes(), x.options());
+        if (ctx->saved_data["track_initial"].toBool()) ginitial = torch::empty({p.N, p.E, p.S}, f32);
+        auto workspace = bytes_like(x, warpctct_selective_scan_workspace_bytes(p.N, p.L, p.E, p.S, p.G));
+        warpctct_scan_grad_t g = {};
+        g.grad_n = up.stride(0);
+        g.grad_t = up.stride(1);
+        g.grad_out = up.data_ptr();
+        g.grad_last = floats(glast);
+        g.grad_x = gx.data_ptr();
+        g.grad_dt = gdt.data_ptr();
+        g.grad_gate = gz.defined() ? gz.data_ptr() : nullptr;
+        g.grad_b = gb.data_ptr();
+        g.grad_c = gc.data_ptr();
+        g.grad_a = floats(ga);
+        g.grad_skip_bias = floats(two);
+        g.grad_initial = floats(ginitial);
+        check_rc(warpctct_selective_scan_grad(&p, &g, keep.data_ptr(), keep.numel(), workspace.data_ptr(),
+                                              workspace.numel(), current_stream()),
+                 "selective_scan");
+        return {gx, gdt, ga, gb, gc, in.skip.defined() ? two.select(0, 0) : torch::Tensor(), gz,
+                in.dt_bias.defined() ? two.select(0, 1) : torch::Tensor(), ginitial, torch::Tensor(),
+                torch::Tensor(), torch::Tensor(), torch::Tensor()};
+    }
+};
+
+// b or c: (..., S) shared by all channels, or (..., G, S)
+torch::Tensor groups_of(const torch::Tensor &t, const torch::Tensor &x, int64_t S, const char *name,
+                        const char *what) {
+    const int64_t lead = x.dim() - 1;
+    TORCH_CHECK(t.dim() == lead + 1 || t.dim() == lead + 2, what, ": ", name, " has the wrong number of dimensions");
+    auto v = native(t);
+    if (v.dim() == lead + 1) v = v.unsqueeze(lead);
+    for (int64_t d = 0; d < lead; ++d)
+        TORCH_CHECK(v.size(d) == x.size(d), what, ": ", name, " must have the input's batch and time");
+    TORCH_CHECK(v.size(lead) >= 1 && x.size(-1) % v.size(lead) == 0 && v.size(-1) == S, what, ": ", name,
+                " must be (..., groups, states), the channels a multiple of the groups");
+    TORCH_CHECK(v.scalar_type() == x.scalar_type(), what, ": ", name, " must have the input's type");
+    check_on(v, x, name);
+    return dense_last(v);
+}
+
+torch::Tensor like_input(const torch::Tensor &t, const torch::Tensor &x, const char *name, const char *what) {
+    const auto v = native(t);
+    TORCH_CHECK(v.sizes() == x.sizes() && v.scalar_type() == x.scalar_type(), what, ": ", name,
+                " must have the input's shape and type");
+    check_on(v, x, name);
+    return dense_last(v);
+}
+
+torch::Tensor per_channel(const Maybe &t, const torch::Tensor &x, const char *name, const char *what) {
+    if (!given(t)) return torch::Tensor();
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == x.size(-1), what, ": ", name, " must have one element a channel");
+    check_on(*t, x, name);
+    return as_float(*t);
+}
+
+// x, dt, a, b, c, skip, gate, dt_bias, checked and in the types of the C ABI
+ScanInputs scan_inputs(const torch::Tensor &input, const torch::Tensor &dt, const torch::Tensor &a,
+                       const torch::Tensor &b, const torch::Tensor &c, const Maybe &skip, const Maybe &gate,
+                       const Maybe &dt_bias, const char *what) {
+    ScanInputs in;
+    in.x = dense_last(native(input));
+    TORCH_CHECK(a.dim() == 2 && a.size(0) == in.x.size(-1) && a.size(1) >= 1 &&
+                    a.size(1) <= WARPCTCT_SCAN_MAX_STATES,
+                what, ": a must be (channels, states) with 1 to ", static_cast<int>(WARPCTCT_SCAN_MAX_STATES),
+                " states");
+    check_on(a, in.x, "a");
+    TORCH_CHECK(in.x.size(-1) <= (1 << 24), what, ": at most 2^24 channels");
+    in.a = as_float(a);
+    in.dt = like_input(dt, in.x, "dt", what);
+    in.b = groups_of(b, in.x, a.size(1), "b", what);
+    in.c = groups_of(c, in.x, a.size(1), "c", what);
+    TORCH_CHECK(in.b.sizes() == in.c.sizes(), what, ": b and c must have the same groups");
+    in.skip = per_channel(skip, in.x, "skip", what);
+    in.dt_bias = per_channel(dt_bias, in.x, "dt_bias", what);
+    if (given(gate)) in.gate = like_input(*gate, in.x, "gate", what);
+    return in;
+}
+
+tensor_list selective_scan(const torch::Tensor &input, const torch::Tensor &dt, const torch::Tensor &a,
+                           const torch::Tensor &b, const torch::Tensor &c, const Maybe &skip, const Maybe &gate,
+                           const Maybe &dt_bias, const bool softplus, const Maybe &lengths, const Maybe &initial,
+                           const bool want_state) {
+    const char *what = "selective_scan";
+    CHECK_DEVICE(input);
+    TORCH_CHECK(input.dim() == 3 && input.size(2) >= 1, "selective_scan: the input must be (batch, time, channels)");
+    TORCH_CHECK(input.size(0) <= 65535 && input.size(1) < (1L << 30),
+                "selective_scan: at most 65535 sequences of fewer than 2^30 steps");
+    ScanInputs in = scan_inputs(input, dt, a, b, c, skip, gate, dt_bias, what);
+    in.lengths = lengths_of(lengths, in.x, what);
+    if (given(initial)) {
+        TORCH_CHECK(initial->dim() == 3 && initial->size(0) == in.x.size(0) && initial->size(1) == in.x.size(2) &&
+                        initial->size(2) == a.size(1) && initial->scalar_type() == at::ScalarType::Float,
+                    "selective_scan: initial_state must be (batch, channels, states) in float32");
+        check_on(*initial, in.x, "initial_state");
+        in.initial = initial->contiguous();
+    }
+    bool track = false;
+    for (const auto *t : {&in.x, &in.dt, &in.a, &in.b, &in.c, &in.skip, &in.gate, &in.dt_bias, &in.initial})
+        track = track || tracked(*t);
+    if (!track) return std::get<0>(scan_forward(in, softplus, want_state, false));
+    const auto maybe = [](const torch::Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); };
+    return SelectiveScan::apply(in.x, in.dt, in.a, in.b, in.c, maybe(in.skip), maybe(in.gate), maybe(in.dt_bias),
+                                maybe(in.initial), maybe(in.lengths), softplus, want_state, tracked(in.initial));
+}
+
+torch::Tensor selective_scan_step(const torch::Tensor &input, torch::Tensor state, const torch::Tensor &dt,
+                                  const torch::Tensor &a, const torch::Tensor &b, const torch::Tensor &c,
+                                  const Maybe &skip, const Maybe &gate, const Maybe &dt_bias, const bool softplus,
+                                  const Maybe &advance) {
+    const char *what = "selective_scan_step";
+    CHECK_DEVICE(input);
+    TORCH_CHECK(input.dim() == 2 && input.size(1) >= 1, "selective_scan_step: the input must be (batch, channels)");
+    const Maybe all[6] = {input, state, dt, a, b, c};
+    refuse_gradient({&all[0], &all[1], &all[2], &all[3], &all[4], &all[5], &skip, &gate, &dt_bias}, what);
+    const ScanInputs in = scan_inputs(input, dt, a, b, c, skip, gate, dt_bias, what);
+    const torch::Tensor &x = in.x;
+    TORCH_CHECK(state.dim() == 3 && state.size(0) == x.size(0) && state.size(1) == x.size(1) &&
+                    state.size(2) == a.size(1) && state.scalar_type() == at::ScalarType::Float &&
+                    state.is_contiguous(),
+                "selective_scan_step: state must be (batch, channels, states), dense, in float32");
+    check_on(state, x, "state");
+    const torch::Tensor go = flags_of(advance, x, what);
+    const DeviceGuard guard(device_of(x));
+    auto out = torch::empty(x.sizes(), x.options());
+    warpctct_scan_step_t p = {};
+    p.dtype = type_of(x);
+    p.N = int_size(x, 0, what);
+    p.E = int_size(x, 1, what);
+    p.S = static_cast<int>(a.size(1));
+    p.G = static_cast<int>(in.b.size(1));
+    p.softplus = softplus ? 1 : 0;
+    p.x_n = x.stride(0);
+    p.dt_n = in.dt.stride(0);
+    p.gate_n = in.gate.defined() ? in.gate.stride(0) : 0;
+    p.b_n = in.b.stride(0);
+    p.b_g = in.b.stride(1);
+    p.c_n = in.c.stride(0);
+    p.c_g = in.c.stride(1);
+    p.x = x.data_ptr();
+    p.dt = in.dt.data_ptr();
+    p.gate = ptr(in.gate);
+    p.b = in.b.data_ptr();
+    p.c = in.c.data_ptr();
+    p.a = floats(in.a);
+    p.skip = floats(in.skip);
+    p.dt_bias = floats(in.dt_bias);
+    p.state = floats(state);
+    p.advance = go.defined() ? reinterpret_cast<const unsigned char *>(go.data_ptr<bool>()) : nullptr;
+    p.out = out.data_ptr();
+    check_rc(warpctct_selective_scan_step(&p, current_stream()), what);
+    return out;
+}
+
 // ---- rules on logits ---------------------------------------------------------------
 
 // a penalty: one number for all rows, or a tensor with one for each
@@ -503,4 +752,12 @@ void define_network(pybind11::module &m) {
           pybind11::arg("tokens"), pybind11::arg("tokens_lengths"), pybind11::arg("repetition_penalty"),
           pybind11::arg("presence_penalty"), pybind11::arg("frequency_penalty"), pybind11::arg("bias"),
           pybind11::arg("allowed"));
+    m.def("selective_scan", &selective_scan, "Selective state space scan, differentiable.", pybind11::arg("x"),
+          pybind11::arg("dt"), pybind11::arg("a"), pybind11::arg("b"), pybind11::arg("c"), pybind11::arg("skip"),
+          pybind11::arg("gate"), pybind11::arg("dt_bias"), pybind11::arg("softplus"), pybind11::arg("lengths"),
+          pybind11::arg("initial_state"), pybind11::arg("return_state"));
+    m.def("selective_scan_step", &selective_scan_step, "One step of selective_scan; updates the state in place.",
+          pybind11::arg("x"), pybind11::arg("state"), pybind11::arg("dt"), pybind11::arg("a"), pybind11::arg("b"),
+          pybind11::arg("c"), pybind11::arg("skip"), pybind11::arg("gate"), pybind11::arg("dt_bias"),
+          pybind11::arg("softplus"), pybind11::arg("advance"));
 }

@@ -32,6 +32,16 @@ bool conv_ok(const warpctct_conv_t *p) {
            (p->N == 0 || (p->weight && (p->x || p->L == 0)));
 }
 
+bool scan_sizes_ok(int dtype, int N, int L, int E, int S, int G) {
+    return io_valid(dtype) && N >= 0 && N <= kMostBatch && L >= 0 && E >= 1 && E <= (1 << 24) && S >= 1 &&
+           S <= WARPCTCT_SCAN_MAX_STATES && G >= 1 && E % G == 0 && (long)L * G * S < (1L << 36) &&
+           L <= 0x7fffffff - WARPCTCT_SCAN_TILE;
+}
+bool scan_ok(const warpctct_scan_t *p) {
+    return p && scan_sizes_ok(p->dtype, p->N, p->L, p->E, p->S, p->G) &&
+           (p->N == 0 || (p->a && (p->L == 0 || (p->x && p->dt && p->b && p->c))));
+}
+
 }  // namespace
 
 extern "C" {
@@ -107,6 +117,55 @@ int warpctct_adjust_logits(const warpctct_adjust_t *p, void *stream) {
     if (p->N == 0) return WARPCTCT_OK;
     if (!p->logits || !p->out) return WARPCTCT_EINVAL;
     return done(launch_adjust(*p, as_stream(stream)));
+}
+
+size_t warpctct_selective_scan_keep_bytes(int N, int L, int E, int S) {
+    if (!scan_sizes_ok(WARPCTCT_F32, N, L, E, S, 1)) return 0;
+    return scan_keep_floats(N, L, E, S) * sizeof(float);
+}
+
+int warpctct_selective_scan(const warpctct_scan_t *p, void *keep, size_t keep_bytes, void *stream) {
+    if (!scan_ok(p)) return WARPCTCT_EINVAL;
+    if (p->N == 0) return WARPCTCT_OK;
+    if (p->L > 0 && !p->out) return WARPCTCT_EINVAL;
+    if (keep && (keep_bytes < scan_keep_floats(p->N, p->L, p->E, p->S) * sizeof(float))) return WARPCTCT_EWORKSPACE;
+    if (reinterpret_cast<uintptr_t>(keep) & 15u) return WARPCTCT_EINVAL;
+    return done(launch_scan(*p, static_cast<float *>(keep), as_stream(stream)));
+}
+
+size_t warpctct_selective_scan_workspace_bytes(int N, int L, int E, int S, int G) {
+    if (!scan_sizes_ok(WARPCTCT_F32, N, L, E, S, G)) return 0;
+    warpctct_scan_t p = {};
+    p.N = N;
+    p.L = L;
+    p.E = E;
+    p.S = S;
+    p.G = G;
+    return scan_grad_floats(p) * sizeof(float);
+}
+
+int warpctct_selective_scan_grad(const warpctct_scan_t *p, const warpctct_scan_grad_t *g, const void *keep,
+                                 size_t keep_bytes, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!scan_ok(p) || !g || !g->grad_a || !g->grad_skip_bias) return WARPCTCT_EINVAL;
+    if (p->N > 0 && p->L > 0 &&
+        (!g->grad_out || !g->grad_x || !g->grad_dt || !g->grad_b || !g->grad_c || (p->gate && !g->grad_gate) || !keep ||
+         !workspace))
+        return WARPCTCT_EINVAL;
+    if ((reinterpret_cast<uintptr_t>(keep) | reinterpret_cast<uintptr_t>(workspace)) & 15u) return WARPCTCT_EINVAL;
+    if (keep_bytes < scan_keep_floats(p->N, p->L, p->E, p->S) * sizeof(float) ||
+        workspace_bytes < scan_grad_floats(*p) * sizeof(float))
+        return WARPCTCT_EWORKSPACE;
+    return done(launch_scan_grad(*p, *g, static_cast<const float *>(keep), static_cast<float *>(workspace),
+                                 as_stream(stream)));
+}
+
+int warpctct_selective_scan_step(const warpctct_scan_step_t *p, void *stream) {
+    // (the batch is no grid dimension here)
+    if (!p || p->N < 0 || !scan_sizes_ok(p->dtype, 0, 1, p->E, p->S, p->G) || (long)p->N * p->E >= (1L << 34))
+        return WARPCTCT_EINVAL;
+    if (p->N == 0) return WARPCTCT_OK;
+    if (!p->x || !p->dt || !p->a || !p->b || !p->c || !p->state || !p->out) return WARPCTCT_EINVAL;
+    return done(launch_scan_step(*p, as_stream(stream)));
 }
 
 }  // extern "C"

@@ -1,0 +1,660 @@
+// Selective state space scan and its backward pass.  Channel e has S states,
+//   d_t = softplus(dt_t + dt_bias)  (or the sum itself)
+//   h_t[s] = exp(d_t a[s]) h_{t-1}[s] + d_t x_t b_t[s]
+//   y_t = sum_s c_t[s] h_t[s] + skip x_t,   out_t = y_t silu(gate_t)
+// and, with gy = g silu(gate) and k_t[s] = exp(d_t a[s]),
+//   gh_t[s] = c_t[s] gy_t + k_{t+1}[s] gh_{t+1}[s]
+//   gc_t[s] = sum_e gy_t h_t[s],  gb_t[s] = sum_e gh_t[s] d_t x_t
+//   gx_t = skip gy_t + d_t sum_s gh_t[s] b_t[s]
+//   gd_t = x_t sum_s gh_t[s] b_t[s] + sum_s a[s] gh_t[s] k_t[s] h_{t-1}[s]
+//   ga[s] = sum_t d_t gh_t[s] k_t[s] h_{t-1}[s],  gskip = sum_t gy_t x_t
+// b and c are shared by the channels of a group.
+//
+// Bound by arithmetic: a state and a step cost an exponential (four issue slots)
+// and four multiply-adds forwards, more than twice that backwards, against 8
+// bytes a channel and a step of 2-byte elements for 16 states.  A channel lies on
+// kLanes lanes next to each other, four states on each, so that the states'
+// products are independent work of a lane and their sum a few lane exchanges.  A
+// workgroup takes 256 / kLanes channels of one group and one sequence and walks
+// down time in tiles of 16 steps: what depends on the step and the channel alone
+// (softplus, silu, the products with x) is computed once an element, by threads
+// that load and store the tile's rows in wide pieces, and handed over in LDS.
+// States, sums and exponents are fp32.
+#include "network.h"
+#include "rows.h"
+
+// products are fused into sums where fmaf says so
+#pragma clang fp contract(off)
+
+namespace wctct {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kSteps = WARPCTCT_SCAN_TILE;      // of a tile
+constexpr int kStates = 4;                      // of a lane
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// log(1 + e^v) and its derivative.  log1p(q), q = e^-|v| in [0, 1], is
+// 2 atanh(q / (2 + q)), whose argument is at most 1/3: eight terms of the
+// series leave a relative error of 3e-9, where log2(1 + q) on the transcendental
+// unit would lose q itself to the rounding of the sum.
+struct Softplus {
+    float value, slope;
+};
+__device__ __forceinline__ Softplus softplus(float v) {
+    const float q = exp2_hw(-kLog2e * fabsf(v));
+    const float r = q * __builtin_amdgcn_rcpf(2.0f + q), r2 = r * r;
+    float s = 1.0f / 15.0f;
+    s = fmaf(s, r2, 1.0f / 13.0f);
+    s = fmaf(s, r2, 1.0f / 11.0f);
+    s = fmaf(s, r2, 1.0f / 9.0f);
+    s = fmaf(s, r2, 1.0f / 7.0f);
+    s = fmaf(s, r2, 1.0f / 5.0f);
+    s = fmaf(s, r2, 1.0f / 3.0f);
+    s = fmaf(s, r2, 1.0f);
+    Softplus p;
+    p.value = fmaxf(v, 0.0f) + 2.0f * r * s;
+    if (v != v) p.value = v;
+    const float inv = __builtin_amdgcn_rcpf(1.0f + q);
+    p.slope = v >= 0.0f ? inv : q * inv;
+    return p;
+}
+
+// Sum over the kLanes lanes of a channel, the same in all of them.
+template <int LANES>
+__device__ __forceinline__ float channel_sum(float v) {
+    if constexpr (LANES >= 2) v += dpp<kDppXor1>(v);
+    if constexpr (LANES >= 4) v += dpp<kDppXor2>(v);
+    if constexpr (LANES >= 8) v += dpp<0x141 /* row_half_mirror */>(v);
+    if constexpr (LANES >= 16) v += dpp<kDppRor8>(v);
+    return v;
+}
+
+__device__ __forceinline__ float swap_add32(float a, float b) {      // lanes < 32: a's sum, others: b's
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float swap_add16(float a, float b) {      // even rows of 16: a's, odd rows: b's
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Four values summed over the channels of a wavefront (lanes kLanes apart): row r
+// of 16 lanes receives value (r & 1) * 2 + (r >> 1).  Halving the values while
+// doubling the distance takes 6 exchanges for the first two steps, not 8.
+template <int LANES>
+__device__ __forceinline__ float sum_over_channels(const float (&v)[kStates]) {
+    float s = swap_add16(swap_add32(v[0], v[1]), swap_add32(v[2], v[3]));
+    if constexpr (LANES <= 8) s += dpp<kDppRor8>(s);
+    if constexpr (LANES <= 4) s += dpp<kDppRor4>(s);
+    if constexpr (LANES <= 2) s += dpp<kDppXor2>(s);
+    if constexpr (LANES <= 1) s += dpp<kDppXor1>(s);
+    return s;
+}
+
+// Where a workgroup works: sequence n, channels [first, end) of group g.
+struct Place {
+    int n, g, block, first, end, len;
+};
+template <int LANES>
+__device__ __forceinline__ Place place_of(const warpctct_scan_t &p) {
+    constexpr int CH = kThreads / LANES;
+    const int per = p.E / p.G, blocks = (per + CH - 1) / CH;
+    Place w;
+    w.n = blockIdx.y;
+    w.block = blockIdx.x;
+    w.g = blockIdx.x / blocks;
+    w.first = w.g * per + (blockIdx.x - w.g * blocks) * CH;
+    w.end = (w.g + 1) * per;
+    w.len = p.lengths ? min(max(p.lengths[w.n], 0), p.L) : p.L;
+    return w;
+}
+
+// A thread's elements of a tile: EPT channels next to each other of one step.
+template <int LANES>
+struct Elements {
+    static constexpr int CH = kThreads / LANES, EPT = kSteps / LANES;
+    int j, c;        // step in the tile, first channel in the workgroup
+    __device__ __forceinline__ Elements() {
+        const int at = threadIdx.x * EPT;
+        j = at / CH;
+        c = at % CH;
+    }
+};
+
+// N elements of a row, in the widest pieces where `wide`; those at or past `have`
+// read as zero and are not written.
+template <int N, typename IO>
+__device__ __forceinline__ void load_row(const IO *p, int have, bool wide, float (&v)[N]) {
+    constexpr int piece = N < 4 ? 1 : (N < kVec<IO> ? 4 : kVec<IO>);
+    if (wide && have >= N) {
+#pragma unroll
+        for (int i = 0; i < N; i += piece) load_n<piece>(p + i, v + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i < have ? to_float(p[i]) : 0.0f;
+    }
+}
+template <int N, typename IO>
+__device__ __forceinline__ void store_row(IO *p, int have, bool wide, const float (&v)[N]) {
+    constexpr int piece = N < 4 ? 1 : (N < kVec<IO> ? 4 : kVec<IO>);
+    if (wide && have >= N) {
+#pragma unroll
+        for (int i = 0; i < N; i += piece) store_n<piece>(p + i, v + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < have) p[i] = from_float<IO>(v[i]);
+    }
+}
+
+// The tile's rows of b and c, kSteps x 2 SP values, by all threads.
+template <int LANES>
+struct Shared {
+    static constexpr int SP = kStates * LANES;
+    static constexpr int PER = (2 * kSteps * SP + kThreads - 1) / kThreads;
+};
+template <int LANES, typename IO>
+__device__ __forceinline__ void load_bc(const warpctct_scan_t &p, const Place &w, int t0,
+                                        float (&v)[Shared<LANES>::PER]) {
+    constexpr int SP = Shared<LANES>::SP;
+    const IO *b = static_cast<const IO *>(p.b) + (long)w.n * p.b_n + (long)w.g * p.b_g;
+    const IO *c = static_cast<const IO *>(p.c) + (long)w.n * p.c_n + (long)w.g * p.c_g;
+#pragma unroll
+    for (int i = 0; i < Shared<LANES>::PER; ++i) {
+        const int at = i * kThreads + threadIdx.x, j = at / (2 * SP), k = at % (2 * SP);
+        const int s = k % SP, t = t0 + j;
+        v[i] = 0.0f;
+        if (j < kSteps && t < w.len && s < p.S)
+            v[i] = to_float(k < SP ? b[(long)t * p.b_t + s] : c[(long)t * p.c_t + s]);
+    }
+}
+
+template <typename IO, int LANES>
+__global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float *__restrict__ keep, bool wide) {
+    constexpr int CH = kThreads / LANES, EPT = Elements<LANES>::EPT, SP = Shared<LANES>::SP, PER = Shared<LANES>::PER;
+    __shared__ float2 steps[kSteps][CH];           // d, d x
+    __shared__ __align__(16) float bc[kSteps][2 * SP];
+    __shared__ float ys[kSteps][CH];
+    const Place w = place_of<LANES>(p);
+    const Elements<LANES> el;
+    // as a lane: a channel and four of its states
+    const int ch = threadIdx.x / LANES, q = threadIdx.x % LANES, e = w.first + ch;
+    const bool live = e < w.end;
+    float a[kStates], h[kStates];
+    const long state = ((long)w.n * p.E + e) * p.S + q * kStates;
+#pragma unroll
+    for (int i = 0; i < kStates; ++i) {
+        const bool in = live && q * kStates + i < p.S;
+        a[i] = in ? p.a[(long)e * p.S + q * kStates + i] * kLog2e : 0.0f;
+        h[i] = in && p.initial ? p.initial[state + i] : 0.0f;
+    }
+    // as a thread of elements: its channels' parameters and rows
+    const int e0 = w.first + el.c, have = max(0, min(EPT, w.end - e0));
+    float skip[EPT], bias[EPT];
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+        skip[i] = p.skip && i < have ? p.skip[e0 + i] : 0.0f;
+        bias[i] = p.dt_bias && i < have ? p.dt_bias[e0 + i] : 0.0f;
+    }
+    const IO *xs = static_cast<const IO *>(p.x) + (long)w.n * p.x_n + e0;
+    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + e0;
+    const IO *zs = p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + e0 : nullptr;
+    IO *out = static_cast<IO *>(p.out) + (long)w.n * p.L * p.E + e0;
+
+    float x[EPT], d[EPT], z[EPT], side[PER];
+    auto request = [&](int t0) {
+        const int t = t0 + el.j, n = t < w.len ? have : 0;
+        load_row<EPT>(xs + (long)t * p.x_t, n, wide, x);
+        load_row<EPT>(ds + (long)t * p.dt_t, n, wide, d);
+        if (zs) load_row<EPT>(zs + (long)t * p.gate_t, n, wide, z);
+        load_bc<LANES, IO>(p, w, t0, side);
+    };
+    request(0);
+    for (int t0 = 0; t0 < w.len; t0 += kSteps) {
+        const bool on = t0 + el.j < w.len;
+        float xk[EPT], zk[EPT];
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+            float v = d[i] + bias[i];
+            if (p.softplus) v = softplus(v).value;
+            if (!(on && i < have)) v = 0.0f;       // a step that leaves the state as it is
+            steps[el.j][el.c + i] = make_float2(v, v * x[i]);
+            xk[i] = x[i];
+            zk[i] = z[i];
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int at = i * kThreads + threadIdx.x;
+            if (at < 2 * kSteps * SP) bc[at / (2 * SP)][at % (2 * SP)] = side[i];
+        }
+        __syncthreads();
+        if (t0 + kSteps < w.len) request(t0 + kSteps);
+        if (keep && live)
+            *reinterpret_cast<float4 *>(
+                keep + (((long)w.n * ((p.L + kSteps - 1) / kSteps) + t0 / kSteps) * p.E + e) * SP + q * kStates) =
+                make_float4(h[0], h[1], h[2], h[3]);
+        for (int j0 = 0; j0 < kSteps && t0 + j0 < w.len; j0 += 4) {
+#pragma unroll
+            for (int j1 = 0; j1 < 4; ++j1) {
+                const int j = j0 + j1;
+                const float2 s = steps[j][ch];
+                const float4 b4 = *reinterpret_cast<const float4 *>(&bc[j][q * kStates]);
+                const float4 c4 = *reinterpret_cast<const float4 *>(&bc[j][SP + q * kStates]);
+                const float b[4] = {b4.x, b4.y, b4.z, b4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
+                float y = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kStates; ++i) {
+                    h[i] = fmaf(exp2_hw(s.x * a[i]), h[i], s.y * b[i]);
+                    y = fmaf(c[i], h[i], y);
+                }
+                y = channel_sum<LANES>(y);
+                if (q == 0) ys[j][ch] = y;
+            }
+        }
+        __syncthreads();
+        if (on) {
+            float o[EPT];
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) {
+                o[i] = fmaf(skip[i], xk[i], ys[el.j][el.c + i]);
+                if (zs) o[i] *= zk[i] * sigmoid(zk[i]);
+            }
+            store_row<EPT>(out + (long)(t0 + el.j) * p.E, have, wide, o);
+        }
+    }
+    // the steps that do not count
+    const float zero[EPT] = {};
+    for (int t = w.len + el.j; t < p.L; t += kSteps) store_row<EPT>(out + (long)t * p.E, have, wide, zero);
+    if (p.last && live) {
+#pragma unroll
+        for (int i = 0; i < kStates; ++i)
+            if (q * kStates + i < p.S) p.last[state + i] = h[i];
+    }
+}
+
+// The backward pass walks up time.  A tile's states are computed again from the
+// one that the forward pass kept in front of it, into registers, together with
+// the factors k; then the tile is walked backwards with gh in registers.  gb and
+// gc, sums over channels, are added up within a wavefront by lane exchanges,
+// within the workgroup in LDS, and leave as partial sums of the workgroup (row:
+// 2 SP floats a step); the sums over time stay in registers until the end.
+template <typename IO, int LANES>
+__global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t p, warpctct_scan_grad_t g,
+                                                                const float *__restrict__ keep,
+                                                                float *__restrict__ part_bc,
+                                                                float *__restrict__ part_sums, bool wide) {
+    constexpr int CH = kThreads / LANES, EPT = Elements<LANES>::EPT, SP = Shared<LANES>::SP, PER = Shared<LANES>::PER;
+    constexpr int WAVES = kThreads / 64;
+    // d, d x, gy, and y without the skip; on the way back the first two give way
+    // to sum gh b and sum a gh k h (a channel's lanes lie in one wavefront, which
+    // has read a step before it overwrites it)
+    __shared__ float4 steps[kSteps][CH];
+    __shared__ __align__(16) float bc[kSteps][2 * SP];
+    __shared__ float sums[WAVES][kSteps][2 * SP];   // gb, gc of a wavefront
+    const Place w = place_of<LANES>(p);
+    const Elements<LANES> el;
+    const int ch = threadIdx.x / LANES, q = threadIdx.x % LANES, e = w.first + ch;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool live = e < w.end;
+    const int tiles = (p.L + kSteps - 1) / kSteps;
+    float a[kStates], carry[kStates], ga[kStates];
+    const long state = ((long)w.n * p.E + e) * p.S + q * kStates;
+#pragma unroll
+    for (int i = 0; i < kStates; ++i) {
+        const bool in = live && q * kStates + i < p.S;
+        a[i] = in ? p.a[(long)e * p.S + q * kStates + i] : 0.0f;
+        carry[i] = in && g.grad_last ? g.grad_last[state + i] : 0.0f;
+        ga[i] = 0.0f;
+    }
+    const int e0 = w.first + el.c, have = max(0, min(EPT, w.end - e0));
+    float skip[EPT], bias[EPT], gskip[EPT], gbias[EPT];
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+        skip[i] = p.skip && i < have ? p.skip[e0 + i] : 0.0f;
+        bias[i] = p.dt_bias && i < have ? p.dt_bias[e0 + i] : 0.0f;
+        gskip[i] = gbias[i] = 0.0f;
+    }
+    const IO *xs = static_cast<const IO *>(p.x) + (long)w.n * p.x_n + e0;
+    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + e0;
+    const IO *zs = p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + e0 : nullptr;
+    const IO *us = static_cast<const IO *>(g.grad_out) + (long)w.n * g.grad_n + e0;
+    const long rows = (long)w.n * p.L * p.E + e0;
+    IO *gx = static_cast<IO *>(g.grad_x) + rows, *gd = static_cast<IO *>(g.grad_dt) + rows;
+    IO *gz = p.gate ? static_cast<IO *>(g.grad_gate) + rows : nullptr;
+
+    const float zero[EPT] = {};
+    for (int t = w.len + el.j; t < p.L; t += kSteps) {
+        store_row<EPT>(gx + (long)t * p.E, have, wide, zero);
+        store_row<EPT>(gd + (long)t * p.E, have, wide, zero);
+        if (gz) store_row<EPT>(gz + (long)t * p.E, have, wide, zero);
+    }
+    for (int tile = (w.len + kSteps - 1) / kSteps - 1; tile >= 0; --tile) {
+        const int t0 = tile * kSteps, t = t0 + el.j;
+        const bool on = t < w.len;
+        float x[EPT], raw[EPT], z[EPT], u[EPT], side[PER];
+        load_row<EPT>(xs + (long)t * p.x_t, on ? have : 0, wide, x);
+        load_row<EPT>(ds + (long)t * p.dt_t, on ? have : 0, wide, raw);
+        load_row<EPT>(us + (long)t * g.grad_t, on ? have : 0, wide, u);
+        if (zs) load_row<EPT>(zs + (long)t * p.gate_t, on ? have : 0, wide, z);
+        load_bc<LANES, IO>(p, w, t0, side);
+        float h0[kStates] = {};
+        if (live) {
+            const float4 v = *reinterpret_cast<const float4 *>(keep + (((long)w.n * tiles + tile) * p.E + e) * SP +
+                                                               q * kStates);
+            h0[0] = v.x, h0[1] = v.y, h0[2] = v.z, h0[3] = v.w;
+        }
+        float d[EPT], slope[EPT], gy[EPT], silu[EPT], dsilu[EPT];
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+            const float v = raw[i] + bias[i];
+            d[i] = v;
+            slope[i] = 1.0f;
+            if (p.softplus) {
+                const Softplus s = softplus(v);
+                d[i] = s.value;
+                slope[i] = s.slope;
+            }
+            if (!(on && i < have)) d[i] = 0.0f;
+            silu[i] = 1.0f;
+            dsilu[i] = 0.0f;
+            if (zs) {
+                const float s = sigmoid(z[i]);
+                silu[i] = z[i] * s;
+                dsilu[i] = s * fmaf(z[i], 1.0f - s, 1.0f);
+            }
+            gy[i] = u[i] * silu[i];
+            if (!(on && i < have)) gy[i] = 0.0f;
+            steps[el.j][el.c + i] = make_float4(d[i], d[i] * x[i], gy[i], 0.0f);
+            gskip[i] = fmaf(gy[i], x[i], gskip[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int at = i * kThreads + threadIdx.x;
+            if (at < 2 * kSteps * SP) bc[at / (2 * SP)][at % (2 * SP)] = side[i];
+        }
+        __syncthreads();
+        float k[kSteps][kStates], h[kSteps][kStates];
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            const float4 s = steps[j][ch];
+            const float4 b4 = *reinterpret_cast<const float4 *>(&bc[j][q * kStates]);
+            const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+            for (int i = 0; i < kStates; ++i) {
+                k[j][i] = exp2_hw(s.x * (a[i] * kLog2e));
+                h[j][i] = fmaf(k[j][i], j ? h[j - 1][i] : h0[i], s.y * b[i]);
+            }
+            if (zs) {
+                const float4 c4 = *reinterpret_cast<const float4 *>(&bc[j][SP + q * kStates]);
+                float y = c4.x * h[j][0];
+                y = fmaf(c4.y, h[j][1], y);
+                y = fmaf(c4.z, h[j][2], y);
+                y = fmaf(c4.w, h[j][3], y);
+                y = channel_sum<LANES>(y);
+                if (q == 0) steps[j][ch].w = y;
+            }
+        }
+#pragma unroll
+        for (int j = kSteps - 1; j >= 0; --j) {
+            const float4 s = steps[j][ch];
+            const float4 b4 = *reinterpret_cast<const float4 *>(&bc[j][q * kStates]);
+            const float4 c4 = *reinterpret_cast<const float4 *>(&bc[j][SP + q * kStates]);
+            const float b[4] = {b4.x, b4.y, b4.z, b4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
+            float ghb = 0.0f, akh = 0.0f, vb[kStates], vc[kStates];
+#pragma unroll
+            for (int i = 0; i < kStates; ++i) {
+                const float gh = fmaf(c[i], s.z, carry[i]);
+                ghb = fmaf(gh, b[i], ghb);
+                vb[i] = gh * s.y;
+                vc[i] = h[j][i] * s.z;
+                carry[i] = gh * k[j][i];
+                const float r = carry[i] * (j ? h[j - 1][i] : h0[i]);
+                akh = fmaf(a[i], r, akh);
+                ga[i] = fmaf(s.x, r, ga[i]);
+            }
+            ghb = channel_sum<LANES>(ghb);
+            akh = channel_sum<LANES>(akh);
+            if (q == 0) *reinterpret_cast<float2 *>(&steps[j][ch]) = make_float2(ghb, akh);
+            const float sb = sum_over_channels<LANES>(vb), sc = sum_over_channels<LANES>(vc);
+            if ((lane & 15) < LANES) {
+                const int row = lane >> 4, s_at = (lane % LANES) * kStates + (row & 1) * 2 + (row >> 1);
+                sums[wave][j][s_at] = sb;
+                sums[wave][j][SP + s_at] = sc;
+            }
+        }
+        __syncthreads();
+        if (on) {
+            float ox[EPT], od[EPT], oz[EPT];
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) {
+                const float4 s = steps[el.j][el.c + i];
+                ox[i] = fmaf(d[i], s.x, skip[i] * gy[i]);
+                od[i] = fmaf(x[i], s.x, s.y) * slope[i];
+                if (i < have) gbias[i] += od[i];
+                if (zs) oz[i] = u[i] * fmaf(skip[i], x[i], s.w) * dsilu[i];
+            }
+            store_row<EPT>(gx + (long)t * p.E, have, wide, ox);
+            store_row<EPT>(gd + (long)t * p.E, have, wide, od);
+            if (gz) store_row<EPT>(gz + (long)t * p.E, have, wide, oz);
+        }
+        float *to = part_bc + (((long)w.n * gridDim.x + w.block) * tiles + tile) * (kSteps * 2 * SP);
+        for (int at = threadIdx.x; at < kSteps * 2 * SP; at += kThreads) {
+            float s = 0.0f;
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) s += sums[v][at / (2 * SP)][at % (2 * SP)];
+            to[at] = s;
+        }
+    }
+    if (g.grad_initial && live) {
+#pragma unroll
+        for (int i = 0; i < kStates; ++i)
+            if (q * kStates + i < p.S) g.grad_initial[state + i] = carry[i];
+    }
+    // the sums over time: a row of E S + 2 E floats for every sequence
+    float *mine = part_sums + (size_t)w.n * p.E * (p.S + 2);
+    if (live) {
+#pragma unroll
+        for (int i = 0; i < kStates; ++i)
+            if (q * kStates + i < p.S) mine[(long)e * p.S + q * kStates + i] = ga[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) steps[el.j][el.c + i] = make_float4(gskip[i], gbias[i], 0.0f, 0.0f);
+    __syncthreads();
+    for (int c = threadIdx.x; c < CH; c += kThreads) {
+        if (w.first + c >= w.end) continue;
+        float s = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            s += steps[j][c].x;
+            b += steps[j][c].y;
+        }
+        mine[(long)p.E * p.S + w.first + c] = s;
+        mine[(long)p.E * p.S + p.E + w.first + c] = b;
+    }
+}
+
+// gb, gc (N, L, G, S): the workgroups' partial sums of a group added up, zero
+// behind a sequence.  A thread has one value.
+template <typename IO>
+__global__ __launch_bounds__(kThreads) void scan_grad_bc_kernel(warpctct_scan_t p, warpctct_scan_grad_t g,
+                                                                const float *__restrict__ part_bc, int blocks,
+                                                                int SP) {
+    const int n = blockIdx.y, GS = p.G * p.S;
+    const long i = (long)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= (long)p.L * 2 * GS) return;
+    const int t = (int)(i / (2 * GS)), k = (int)(i - (long)t * 2 * GS), v = k % GS, grp = v / p.S, s = v % p.S;
+    const int tiles = (p.L + kSteps - 1) / kSteps;
+    const int len = p.lengths ? min(max(p.lengths[n], 0), p.L) : p.L;
+    float sum = 0.0f;
+    if (t < len) {
+        const float *from = part_bc + (((long)n * blocks * p.G + (long)grp * blocks) * tiles * kSteps + t) * (2 * SP) +
+                            (k < GS ? 0 : SP) + s;
+        for (int b = 0; b < blocks; ++b) sum += from[(long)b * tiles * kSteps * 2 * SP];
+    }
+    IO *to = static_cast<IO *>(k < GS ? g.grad_b : g.grad_c);
+    to[((long)n * p.L + t) * GS + v] = from_float<IO>(sum);
+}
+
+// One step of N sequences; a channel lies on kLanes lanes.
+template <typename IO, int LANES>
+__global__ __launch_bounds__(kThreads) void scan_step_kernel(warpctct_scan_step_t p) {
+    const long i0 = ((long)blockIdx.x * kThreads + threadIdx.x) / LANES;
+    if (i0 >= (long)p.N * p.E) return;             // all lanes of a channel
+    const int n = (int)(i0 / p.E), e = (int)(i0 - (long)n * p.E), q = threadIdx.x % LANES;
+    IO *out = static_cast<IO *>(p.out) + (long)n * p.E + e;
+    if (p.advance && !p.advance[n]) {
+        if (q == 0) *out = from_float<IO>(0.0f);
+        return;
+    }
+    const float x = to_float(static_cast<const IO *>(p.x)[(long)n * p.x_n + e]);
+    float d = to_float(static_cast<const IO *>(p.dt)[(long)n * p.dt_n + e]) + (p.dt_bias ? p.dt_bias[e] : 0.0f);
+    if (p.softplus) d = softplus(d).value;
+    const int grp = e / (p.E / p.G);
+    const IO *b = static_cast<const IO *>(p.b) + (long)n * p.b_n + (long)grp * p.b_g + q * kStates;
+    const IO *c = static_cast<const IO *>(p.c) + (long)n * p.c_n + (long)grp * p.c_g + q * kStates;
+    float *h = p.state + i0 * p.S + q * kStates;
+    const float *a = p.a + (long)e * p.S + q * kStates;
+    const float dx = d * x;
+    float y = 0.0f;
+    if (p.S == kStates * LANES && (reinterpret_cast<uintptr_t>(p.state) & 15u) == 0 &&
+        (reinterpret_cast<uintptr_t>(p.a) & 15u) == 0) {
+        const float4 h4 = *reinterpret_cast<const float4 *>(h), a4 = *reinterpret_cast<const float4 *>(a);
+        float hv[4] = {h4.x, h4.y, h4.z, h4.w};
+        const float av[4] = {a4.x, a4.y, a4.z, a4.w};
+#pragma unroll
+        for (int i = 0; i < kStates; ++i) {
+            hv[i] = fmaf(exp2_hw(d * (av[i] * kLog2e)), hv[i], dx * to_float(b[i]));
+            y = fmaf(to_float(c[i]), hv[i], y);
+        }
+        *reinterpret_cast<float4 *>(h) = make_float4(hv[0], hv[1], hv[2], hv[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kStates; ++i) {
+            if (q * kStates + i >= p.S) continue;
+            const float hv = fmaf(exp2_hw(d * (a[i] * kLog2e)), h[i], dx * to_float(b[i]));
+            y = fmaf(to_float(c[i]), hv, y);
+            h[i] = hv;
+        }
+    }
+    y = channel_sum<LANES>(y);
+    if (q != 0) return;
+    if (p.skip) y = fmaf(p.skip[e], x, y);
+    if (p.gate) {
+        const float z = to_float(static_cast<const IO *>(p.gate)[(long)n * p.gate_n + e]);
+        y *= z * sigmoid(z);
+    }
+    *out = from_float<IO>(y);
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int lanes_of(int S) {
+    int lanes = 1;
+    while (lanes * kStates < S) lanes *= 2;
+    return lanes;
+}
+int blocks_of(const warpctct_scan_t &p) {      // of a group
+    const int ch = kThreads / lanes_of(p.S);
+    return (p.E / p.G + ch - 1) / ch;
+}
+
+// Rows may be read and written in 16-byte pieces: so are they spaced and aligned,
+// and every group starts at a multiple of 16 bytes.
+template <typename IO>
+bool rows_wide(const warpctct_scan_t &p) {
+    constexpr int V = kVec<IO>;
+    return p.E % V == 0 && (p.E / p.G) % V == 0 && p.x_n % V == 0 && p.x_t % V == 0 && p.dt_n % V == 0 &&
+           p.dt_t % V == 0 && p.gate_n % V == 0 && p.gate_t % V == 0 && aligned16(p.x) && aligned16(p.dt) &&
+           aligned16(p.gate) && aligned16(p.out);
+}
+
+template <typename IO, int LANES>
+hipError_t start(const warpctct_scan_t &p, float *keep, hipStream_t stream) {
+    auto kernel = scan_kernel<IO, LANES>;
+    TIMED_LAUNCH(kernel, dim3(p.G * blocks_of(p), p.N), dim3(kThreads), 0, stream, p, keep, rows_wide<IO>(p));
+    return hipGetLastError();
+}
+
+template <typename IO, int LANES>
+hipError_t start(const warpctct_scan_t &p, const warpctct_scan_grad_t &g, const float *keep, float *part_bc,
+                 float *part_sums, hipStream_t stream) {
+    constexpr int V = kVec<IO>;
+    const bool wide = rows_wide<IO>(p) && g.grad_n % V == 0 && g.grad_t % V == 0 && aligned16(g.grad_out) &&
+                      aligned16(g.grad_x) && aligned16(g.grad_dt) && aligned16(g.grad_gate);
+    const int blocks = blocks_of(p);
+    if (p.N == 0) return hipSuccess;
+    auto kernel = scan_grad_kernel<IO, LANES>;
+    TIMED_LAUNCH(kernel, dim3(p.G * blocks, p.N), dim3(kThreads), 0, stream, p, g, keep, part_bc, part_sums, wide);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.L == 0) return e;
+    auto join = scan_grad_bc_kernel<IO>;
+    const long values = (long)p.L * 2 * p.G * p.S;
+    TIMED_LAUNCH(join, dim3((unsigned)((values + kThreads - 1) / kThreads), p.N), dim3(kThreads), 0, stream, p, g,
+                 part_bc, blocks, Shared<LANES>::SP);
+    return hipGetLastError();
+}
+
+template <typename IO, int LANES>
+hipError_t start(const warpctct_scan_step_t &p, hipStream_t stream) {
+    const long threads = (long)p.N * p.E * LANES;
+    auto kernel = scan_step_kernel<IO, LANES>;
+    TIMED_LAUNCH(kernel, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, p);
+    return hipGetLastError();
+}
+
+template <typename IO, typename... Args>
+hipError_t by_states(int S, const Args &...args) {
+    switch (lanes_of(S)) {
+        case 1: return start<IO, 1>(args...);
+        case 2: return start<IO, 2>(args...);
+        case 4: return start<IO, 4>(args...);
+        case 8: return start<IO, 8>(args...);
+        case 16: return start<IO, 16>(args...);
+        default: return hipErrorInvalidValue;
+    }
+}
+template <typename... Args>
+hipError_t by_type(int dtype, int S, const Args &...args) {
+    if (dtype == kIoF32) return by_states<float>(S, args...);
+    if (dtype == kIoF16) return by_states<f16>(S, args...);
+    return by_states<bf16>(S, args...);
+}
+
+size_t part_bc_floats(const warpctct_scan_t &p) {
+    const size_t tiles = (p.L + kSteps - 1) / kSteps, SP = kStates * lanes_of(p.S);
+    return (size_t)p.N * p.G * blocks_of(p) * tiles * kSteps * 2 * SP;
+}
+
+}  // namespace
+
+size_t scan_keep_floats(int N, int L, int E, int S) {
+    return (size_t)N * ((L + kSteps - 1) / kSteps) * E * (kStates * lanes_of(S));
+}
+
+size_t scan_grad_floats(const warpctct_scan_t &p) {
+    return part_bc_floats(p) + column_sums_floats(p.N, (long)p.E * (p.S + 2));
+}
+
+hipError_t launch_scan(const warpctct_scan_t &p, float *keep, hipStream_t stream) {
+    return by_type(p.dtype, p.S, p, keep, stream);
+}
+
+hipError_t launch_scan_grad(const warpctct_scan_t &p, const warpctct_scan_grad_t &g, const float *keep,
+                            float *workspace, hipStream_t stream) {
+    float *part_bc = workspace, *part_sums = workspace + part_bc_floats(p);
+    const hipError_t e = by_type(p.dtype, p.S, p, g, keep, part_bc, part_sums, stream);
+    if (e != hipSuccess) return e;
+    // (the skip's and the bias's gradients lie next to each other)
+    return launch_column_sums(part_sums, p.N, p.E * (p.S + 2), p.E * p.S, g.grad_a, kIoF32, g.grad_skip_bias, kIoF32,
+                              stream);
+}
+
+hipError_t launch_scan_step(const warpctct_scan_step_t &p, hipStream_t stream) {
+    return by_type(p.dtype, p.S, p, stream);
+}
+
+}  // namespace wctct

@@ -22,7 +22,8 @@ except ImportError as exc:  # pragma: no cover - exercised only on a broken inst
         "(needs hipcc, --offload-arch=gfx950)"
     ) from exc
 
-from .network import adjust_logits, causal_conv, causal_conv_step, layer_norm  # noqa: E402,F401
+from .network import (adjust_logits, causal_conv, causal_conv_step, layer_norm,  # noqa: E402,F401
+                      selective_scan, selective_scan_step)
 
 # The reference exports exactly these two (warp_ctct/__init__.py:17), so that
 # `from warp_ctct import *` binds the same names.  ctct_loss_with_logits,

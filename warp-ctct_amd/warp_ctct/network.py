@@ -2,10 +2,11 @@
 the rules put on the joiner's logits before a token is taken from them.
 
 The losses start from scores.  These are the operators on either side of them
-that a model of the same kind runs: :func:`layer_norm` and
-:func:`causal_conv` for a prediction network or an encoder, in training, and
-:func:`causal_conv_step` for decoding a token at a time; :func:`adjust_logits`
-before a token is taken.  Hand-written HIP kernels like the losses', through the same binding: float32, float16 and bfloat16 are
+that a model of the same kind runs: :func:`layer_norm`,
+:func:`causal_conv` and :func:`selective_scan` for a prediction network or an
+encoder, in training and over prompts, :func:`causal_conv_step` and
+:func:`selective_scan_step` for decoding a token at a time;
+:func:`adjust_logits` before a token is taken.  Hand-written HIP kernels like the losses', through the same binding: float32, float16 and bfloat16 are
 read as they are (another type is converted to float32), sums and states are
 kept in float32, a result is rounded once.  Nothing synchronises with the host;
 work is enqueued on the current stream of the input's GPU.  A wrong shape, type
@@ -92,6 +93,69 @@ def causal_conv_step(x: torch.Tensor,
     keeps the output of its last label).  Not differentiable: call it under
     ``torch.no_grad()``."""
     return core.causal_conv_step(x, state, weight, bias, _activation(activation), advance)
+
+
+def selective_scan(x: torch.Tensor,
+                   dt: torch.Tensor,
+                   a: torch.Tensor,
+                   b: torch.Tensor,
+                   c: torch.Tensor,
+                   skip: Optional[torch.Tensor] = None,
+                   gate: Optional[torch.Tensor] = None,
+                   dt_bias: Optional[torch.Tensor] = None,
+                   softplus: bool = False,
+                   lengths: Optional[torch.Tensor] = None,
+                   initial_state: Optional[torch.Tensor] = None,
+                   return_state: bool = False):
+    """Selective state space scan: every channel drives S states of its own::
+
+        d = softplus(dt + dt_bias)            # softplus=False: the sum itself
+        h[s] = exp(d * a[s]) * h[s] + d * x * b[s]
+        out = (sum_s c[s] * h[s] + skip * x) * silu(gate)
+
+    Args:
+        x, dt, gate: (N, T, E) in one type; gate may be None.  Views with a dense
+            last dimension (the halves of one projection) are read in place.
+        a: (E, S), S up to 64; converted to float32 like skip and dt_bias.
+        b, c: (N, T, S), or (N, T, G, S) for G groups of E/G channels next to each
+            other, in the type of ``x``.
+        skip, dt_bias: (E,) or None.
+        lengths: (N,) steps of each sequence; the steps behind them are not read
+            and their outputs (and gradients) are zero.  None: all T.
+        initial_state: (N, E, S) float32, the states in front of the first step.
+            None: zeros.
+        return_state: also return the states behind the last step of every
+            sequence, (N, E, S) float32: the ``initial_state`` of a call that goes
+            on from there, and the ``state`` of :func:`selective_scan_step`.
+
+    Returns out (N, T, E), or ``(out, state)``.  Differentiable with respect to
+    everything but ``lengths``, through both results; every sum is added up in a
+    fixed order.  Where a gradient is tracked, the states in front of every 16
+    steps are kept for it: T/16 * N * E * S floats."""
+    got = core.selective_scan(x, dt, a, b, c, skip, gate, dt_bias, bool(softplus), lengths, initial_state,
+                              bool(return_state))
+    return (got[0], got[1]) if return_state else got[0]
+
+
+def selective_scan_step(x: torch.Tensor,
+                        state: torch.Tensor,
+                        dt: torch.Tensor,
+                        a: torch.Tensor,
+                        b: torch.Tensor,
+                        c: torch.Tensor,
+                        skip: Optional[torch.Tensor] = None,
+                        gate: Optional[torch.Tensor] = None,
+                        dt_bias: Optional[torch.Tensor] = None,
+                        softplus: bool = False,
+                        advance: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One step of :func:`selective_scan` for N sequences: ``x``, ``dt``, ``gate``
+    (N, E), ``b``, ``c`` (N, S) or (N, G, S); ``state`` (N, E, S) float32 moves on
+    in place, out (N, E) is returned.
+
+    ``advance`` (N,) bool, None for all: a sequence that does not advance keeps
+    its state, and its row of the result is zero.  Not differentiable: call it
+    under ``torch.no_grad()``."""
+    return core.selective_scan_step(x, state, dt, a, b, c, skip, gate, dt_bias, bool(softplus), advance)
 
 
 def adjust_logits(logits: torch.Tensor,
