@@ -614,6 +614,8 @@ int warpctct_causal_conv_step(const warpctct_conv_step_t *p, void *stream);
  * counts.  out (N, L, E) dense.
  * keep (warpctct_selective_scan_keep_bytes, 16-byte aligned; NULL without a
  * backward pass) receives the states in front of every WARPCTCT_SCAN_TILE steps.
+ * workspace: warpctct_selective_scan_workspace_bytes(..., 0), 16-byte aligned (0
+ * bytes, may be NULL, unless few long sequences are cut into chunks).
  * N <= 65535. */
 enum { WARPCTCT_SCAN_MAX_STATES = 64, WARPCTCT_SCAN_TILE = 16 };
 typedef struct {
@@ -627,7 +629,9 @@ typedef struct {
     float *last;
 } warpctct_scan_t;
 size_t warpctct_selective_scan_keep_bytes(int N, int L, int E, int S);
-int warpctct_selective_scan(const warpctct_scan_t *p, void *keep, size_t keep_bytes, void *stream);
+size_t warpctct_selective_scan_workspace_bytes(int N, int L, int E, int S, int G, int backward);
+int warpctct_selective_scan(const warpctct_scan_t *p, void *keep, size_t keep_bytes, void *workspace,
+                            size_t workspace_bytes, void *stream);
 
 /* Gradients for grad_out (addressed like x by grad_n, grad_t) and, if not NULL,
  * grad_last (N, E, S): in the type of x and dense grad_x, grad_dt, grad_gate
@@ -636,7 +640,7 @@ int warpctct_selective_scan(const warpctct_scan_t *p, void *keep, size_t keep_by
  * whether or not there is one) and grad_initial (N, E, S; may be NULL).  keep as
  * the forward call left it; `out` and `last` of p are not used.  Sums over
  * channels, steps and sequences are added up in a fixed order through
- * `workspace` (warpctct_selective_scan_workspace_bytes, 16-byte aligned). */
+ * `workspace` (warpctct_selective_scan_workspace_bytes(..., 1), 16-byte aligned). */
 typedef struct {
     long grad_n, grad_t;
     const void *grad_out;
@@ -644,7 +648,6 @@ typedef struct {
     void *grad_x, *grad_dt, *grad_gate, *grad_b, *grad_c;
     float *grad_a, *grad_skip_bias, *grad_initial;
 } warpctct_scan_grad_t;
-size_t warpctct_selective_scan_workspace_bytes(int N, int L, int E, int S, int G);
 int warpctct_selective_scan_grad(const warpctct_scan_t *p, const warpctct_scan_grad_t *g, const void *keep,
                                  size_t keep_bytes, void *workspace, size_t workspace_bytes, void *stream);
 

@@ -190,14 +190,24 @@ def test_selective_scan_arguments():
     assert size(2, 20, 8, 16) == 2 * 2 * 8 * 16 * 4 and size(2, 20, 8, 5) == 2 * 2 * 8 * 8 * 4
     assert size(2, 0, 8, 16) == 0 and size(2, 20, 8, 65) == 0
 
-    def call(keep=0, have=0, **over):
-        return lib.warpctct_selective_scan(ctypes.byref(scan(**over)), P(keep), ctypes.c_size_t(have), P(0))
+    def call(keep=0, have=0, workspace=0, scratch=0, **over):
+        return lib.warpctct_selective_scan(ctypes.byref(scan(**over)), P(keep), ctypes.c_size_t(have), P(workspace),
+                                           ctypes.c_size_t(scratch), P(0))
 
-    assert lib.warpctct_selective_scan(P(0), P(0), ctypes.c_size_t(0), P(0)) == EINVAL
+    none = ctypes.c_size_t(0)
+    assert lib.warpctct_selective_scan(P(0), P(0), none, P(0), none, P(0)) == EINVAL
     for bad in BAD_SCANS + (dict(out=None),):
         assert call(**bad) == EINVAL, bad
     assert call(keep=ALIGNED, have=2047) == EWORKSPACE
     assert call(keep=ALIGNED + 4, have=1 << 20) == EINVAL
+    # few long sequences take scratch: at least the states and the sum of every chunk but one
+    size = lib.warpctct_selective_scan_workspace_bytes
+    size.restype = ctypes.c_size_t
+    need = size(1, 20000, 8, 16, 2, 0)
+    assert need >= 2 * 8 * 17 * 4 and need % (8 * 17 * 4) == 0 and size(2, 20, 8, 16, 2, 0) == 0
+    long = dict(N=1, L=20000)
+    assert call(**long) == EINVAL and call(workspace=ALIGNED, scratch=need - 1, **long) == EWORKSPACE
+    assert call(workspace=ALIGNED + 4, scratch=need, **long) == EINVAL
     assert call(N=0, x=None, dt=None, b=None, c=None, a=None, out=None) == 0
 
 
@@ -205,8 +215,8 @@ def test_selective_scan_gradient_and_step_arguments():
     lib = hip_lib.lib()
     size = lib.warpctct_selective_scan_workspace_bytes
     size.restype = ctypes.c_size_t
-    need = size(2, 20, 8, 16, 2)
-    assert need >= 4 * (2 * 2 * 2 * 16 * 32 + 2 * 8 * 18) and size(2, 20, 9, 16, 2) == 0
+    need = size(2, 20, 8, 16, 2, 1)
+    assert need >= 4 * (2 * 2 * 2 * 16 * 32 + 2 * 8 * 18) and size(2, 20, 9, 16, 2, 1) == 0
 
     def call(p=None, keep=ALIGNED, kept=1 << 20, workspace=ALIGNED, have=1 << 20, **over):
         fields = dict(grad_out=SOME, grad_x=SOME, grad_dt=SOME, grad_b=SOME, grad_c=SOME, grad_a=SOME,

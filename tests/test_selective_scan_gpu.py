@@ -181,7 +181,8 @@ def compare(case):
 
 SHAPES = [(1, 1, 1, 1, 1), (2, 1, 8, 16, 1), (2, 15, 6, 3, 2), (1, 16, 64, 16, 1), (3, 17, 65, 16, 1), (2, 33, 10, 5, 2),
           (2, 40, 260, 4, 1), (2, 50, 130, 8, 1), (1, 100, 96, 16, 3), (2, 37, 40, 20, 1), (2, 20, 34, 32, 2),
-          (1, 35, 20, 33, 1), (2, 48, 24, 64, 1), (1, 300, 16, 12, 1), (70, 18, 4, 2, 1)]
+          (1, 35, 20, 33, 1), (2, 48, 24, 64, 1), (1, 300, 16, 12, 1), (70, 18, 4, 2, 1), (140, 70, 6, 16, 1),
+          (1, 1100, 10, 16, 1)]
 
 
 @gpu

@@ -445,8 +445,11 @@ std::tuple<tensor_list, torch::Tensor> scan_forward(const ScanInputs &in, bool s
     p.last = want_state ? floats(outs[1]) : nullptr;
     torch::Tensor keep;
     if (for_backward) keep = bytes_like(in.x, warpctct_selective_scan_keep_bytes(p.N, p.L, p.E, p.S));
+    const size_t scratch = warpctct_selective_scan_workspace_bytes(p.N, p.L, p.E, p.S, p.G, 0);
+    torch::Tensor workspace;
+    if (scratch > 0) workspace = bytes_like(in.x, scratch);
     check_rc(warpctct_selective_scan(&p, keep.defined() ? keep.data_ptr() : nullptr, keep.defined() ? keep.numel() : 0,
-                                     current_stream()),
+                                     workspace.defined() ? workspace.data_ptr() : nullptr, scratch, current_stream()),
              "selective_scan");
     return std::make_tuple(outs, keep);
 }
@@ -488,7 +491,7 @@ class SelectiveScan : public torch::autograd::Function<SelectiveScan> {
                       ga = torch::empty({p.E, p.S}, f32), two = torch::empty({2, p.E}, f32), ginitial;
         if (in.gate.defined()) gz = torch::empty(x.sizes(), x.options());
         if (ctx->saved_data["track_initial"].toBool()) ginitial = torch::empty({p.N, p.E, p.S}, f32);
-        auto workspace = bytes_like(x, warpctct_selective_scan_workspace_bytes(p.N, p.L, p.E, p.S, p.G));
+        auto workspace = bytes_like(x, warpctct_selective_scan_workspace_bytes(p.N, p.L, p.E, p.S, p.G, 1));
         warpctct_scan_grad_t g = {};
         g.grad_n = up.stride(0);
         g.grad_t = up.stride(1);

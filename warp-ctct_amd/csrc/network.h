@@ -36,8 +36,10 @@ hipError_t launch_conv_step(const warpctct_conv_step_t &p, hipStream_t stream);
 
 // floats that the forward pass keeps for the backward: the states in front of every tile
 size_t scan_keep_floats(int N, int L, int E, int S);
+// floats of scratch that the two passes take (16-byte aligned)
+size_t scan_floats(const warpctct_scan_t &p);
 size_t scan_grad_floats(const warpctct_scan_t &p);
-hipError_t launch_scan(const warpctct_scan_t &p, float *keep, hipStream_t stream);
+hipError_t launch_scan(const warpctct_scan_t &p, float *keep, float *workspace, hipStream_t stream);
 hipError_t launch_scan_grad(const warpctct_scan_t &p, const warpctct_scan_grad_t &g, const float *keep,
                             float *workspace, hipStream_t stream);
 hipError_t launch_scan_step(const warpctct_scan_step_t &p, hipStream_t stream);

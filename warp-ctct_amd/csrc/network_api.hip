@@ -124,16 +124,7 @@ size_t warpctct_selective_scan_keep_bytes(int N, int L, int E, int S) {
     return scan_keep_floats(N, L, E, S) * sizeof(float);
 }
 
-int warpctct_selective_scan(const warpctct_scan_t *p, void *keep, size_t keep_bytes, void *stream) {
-    if (!scan_ok(p)) return WARPCTCT_EINVAL;
-    if (p->N == 0) return WARPCTCT_OK;
-    if (p->L > 0 && !p->out) return WARPCTCT_EINVAL;
-    if (keep && (keep_bytes < scan_keep_floats(p->N, p->L, p->E, p->S) * sizeof(float))) return WARPCTCT_EWORKSPACE;
-    if (reinterpret_cast<uintptr_t>(keep) & 15u) return WARPCTCT_EINVAL;
-    return done(launch_scan(*p, static_cast<float *>(keep), as_stream(stream)));
-}
-
-size_t warpctct_selective_scan_workspace_bytes(int N, int L, int E, int S, int G) {
+size_t warpctct_selective_scan_workspace_bytes(int N, int L, int E, int S, int G, int backward) {
     if (!scan_sizes_ok(WARPCTCT_F32, N, L, E, S, G)) return 0;
     warpctct_scan_t p = {};
     p.N = N;
@@ -141,7 +132,20 @@ size_t warpctct_selective_scan_workspace_bytes(int N, int L, int E, int S, int G
     p.E = E;
     p.S = S;
     p.G = G;
-    return scan_grad_floats(p) * sizeof(float);
+    return (backward ? scan_grad_floats(p) : scan_floats(p)) * sizeof(float);
+}
+
+int warpctct_selective_scan(const warpctct_scan_t *p, void *keep, size_t keep_bytes, void *workspace,
+                            size_t workspace_bytes, void *stream) {
+    if (!scan_ok(p)) return WARPCTCT_EINVAL;
+    if (p->N == 0) return WARPCTCT_OK;
+    if (p->L > 0 && !p->out) return WARPCTCT_EINVAL;
+    if ((reinterpret_cast<uintptr_t>(keep) | reinterpret_cast<uintptr_t>(workspace)) & 15u) return WARPCTCT_EINVAL;
+    const size_t need = scan_floats(*p) * sizeof(float);
+    if (need > 0 && !workspace) return WARPCTCT_EINVAL;
+    if ((keep && keep_bytes < scan_keep_floats(p->N, p->L, p->E, p->S) * sizeof(float)) || workspace_bytes < need)
+        return WARPCTCT_EWORKSPACE;
+    return done(launch_scan(*p, static_cast<float *>(keep), static_cast<float *>(workspace), as_stream(stream)));
 }
 
 int warpctct_selective_scan_grad(const warpctct_scan_t *p, const warpctct_scan_grad_t *g, const void *keep,

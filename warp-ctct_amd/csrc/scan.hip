@@ -20,6 +20,14 @@
 // (softplus, silu, the products with x) is computed once an element, by threads
 // that load and store the tile's rows in wide pieces, and handed over in LDS.
 // States, sums and exponents are fp32.
+//
+// Few long sequences are cut into chunks of tiles.  The states behind a chunk
+// are exp(a sum d) times those in front of it plus what it makes of zeros, so a
+// first pass takes every chunk from zeros (without c and y), a small kernel joins
+// them one after the other, and the second pass starts every chunk from its own
+// states; the reverse recurrence of gh alike.
+#include <algorithm>
+
 #include "network.h"
 #include "rows.h"
 
@@ -94,12 +102,13 @@ __device__ __forceinline__ float sum_over_channels(const float (&v)[kStates]) {
     return s;
 }
 
-// Where a workgroup works: sequence n, channels [first, end) of group g.
+// Where a workgroup works: sequence n, channels [first, end) of group g, steps
+// [from, to) of the `len` that count (chunk blockIdx.z of the sequence).
 struct Place {
-    int n, g, block, first, end, len;
+    int n, g, block, first, end, len, from, to;
 };
 template <int LANES>
-__device__ __forceinline__ Place place_of(const warpctct_scan_t &p) {
+__device__ __forceinline__ Place place_of(const warpctct_scan_t &p, int chunk_tiles) {
     constexpr int CH = kThreads / LANES;
     const int per = p.E / p.G, blocks = (per + CH - 1) / CH;
     Place w;
@@ -109,6 +118,8 @@ __device__ __forceinline__ Place place_of(const warpctct_scan_t &p) {
     w.first = w.g * per + (blockIdx.x - w.g * blocks) * CH;
     w.end = (w.g + 1) * per;
     w.len = p.lengths ? min(max(p.lengths[w.n], 0), p.L) : p.L;
+    w.from = min((int)blockIdx.z * chunk_tiles * kSteps, w.len);
+    w.to = blockIdx.z + 1 == gridDim.z ? w.len : min(w.from + chunk_tiles * kSteps, w.len);
     return w;
 }
 
@@ -172,49 +183,115 @@ __device__ __forceinline__ void load_bc(const warpctct_scan_t &p, const Place &w
     }
 }
 
-template <typename IO, int LANES>
-__global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float *__restrict__ keep, bool wide) {
+// Four steps of a tile as a lane takes them out of LDS.
+struct Four {
+    float2 s[4];                 // d, d x
+    float b[4][kStates], c[4][kStates];
+};
+template <int LANES, bool WITH_C>
+__device__ __forceinline__ void load_four(Four &f, const float2 (*steps)[kThreads / LANES],
+                                          const float (*bc)[2 * kStates * LANES], int j0, int ch, int q) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        f.s[j] = steps[j0 + j][ch];
+        *reinterpret_cast<float4 *>(f.b[j]) = *reinterpret_cast<const float4 *>(&bc[j0 + j][q * kStates]);
+        if (WITH_C)
+            *reinterpret_cast<float4 *>(f.c[j]) =
+                *reinterpret_cast<const float4 *>(&bc[j0 + j][kStates * LANES + q * kStates]);
+    }
+}
+
+// What four lanes q = 0..3 of a channel (or two, or one) hold for four steps,
+// summed over the channel's lanes: each step's sum ends on one lane (of every
+// four), which holds `kept` of them, the first of them `step`.  Three selects and
+// exchanges where a sum for every lane would take two a step, and no branch.
+template <int LANES>
+struct StepSums {
+    static constexpr int kept = LANES >= 4 ? 1 : 4 / LANES;
+    static __device__ __forceinline__ int step(int q) {
+        return LANES == 1 ? 0 : LANES == 2 ? 2 * q : (q & 1) * 2 + ((q >> 1) & 1);
+    }
+    static __device__ __forceinline__ void add(const float (&v)[4], int q, float (&r)[kept]) {
+        if constexpr (LANES == 1) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] = v[j];
+        } else {
+            const bool odd = q & 1, high = q & 2;
+            const float u0 = (odd ? v[2] : v[0]) + dpp<kDppXor1>(odd ? v[0] : v[2]);
+            const float u1 = (odd ? v[3] : v[1]) + dpp<kDppXor1>(odd ? v[1] : v[3]);
+            if constexpr (LANES == 2) {
+                r[0] = u0;
+                r[1] = u1;
+            } else {
+                float w = (high ? u1 : u0) + dpp<kDppXor2>(high ? u0 : u1);
+                // lane ^ 4: the mirror image within 8 lanes, its quads turned round
+                if constexpr (LANES >= 8) w += dpp<0x1B>(dpp<0x141>(w));
+                if constexpr (LANES >= 16) w += dpp<kDppRor8>(w);
+                r[0] = w;
+            }
+        }
+    }
+};
+
+// The first pass over chunks: where a chunk leads from zeros, and its sum of d.
+// local (N, chunks, E, SP), total (N, chunks, E).
+struct Chunks {
+    float *local, *total;
+    int tiles;                   // of a chunk
+};
+
+// CARRY: the first pass over chunks.  Otherwise from `starts` (laid out like
+// Chunks::local, the states in front of every chunk) or, without it, from
+// p.initial.
+template <typename IO, int LANES, bool CARRY>
+__global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float *__restrict__ keep, Chunks chunks,
+                                                        const float *__restrict__ starts, bool wide) {
     constexpr int CH = kThreads / LANES, EPT = Elements<LANES>::EPT, SP = Shared<LANES>::SP, PER = Shared<LANES>::PER;
     __shared__ float2 steps[kSteps][CH];           // d, d x
     __shared__ __align__(16) float bc[kSteps][2 * SP];
-    __shared__ float ys[kSteps][CH];
-    const Place w = place_of<LANES>(p);
+    __shared__ float ys[kSteps][CARRY ? 1 : CH];
+    const Place w = place_of<LANES>(p, chunks.tiles);
     const Elements<LANES> el;
     // as a lane: a channel and four of its states
     const int ch = threadIdx.x / LANES, q = threadIdx.x % LANES, e = w.first + ch;
     const bool live = e < w.end;
-    float a[kStates], h[kStates];
+    float a[kStates], h[kStates], total = 0.0f;
     const long state = ((long)w.n * p.E + e) * p.S + q * kStates;
+    const long chunk = ((long)w.n * gridDim.z + blockIdx.z) * p.E + e;
 #pragma unroll
     for (int i = 0; i < kStates; ++i) {
         const bool in = live && q * kStates + i < p.S;
         a[i] = in ? p.a[(long)e * p.S + q * kStates + i] * kLog2e : 0.0f;
-        h[i] = in && p.initial ? p.initial[state + i] : 0.0f;
+        h[i] = 0.0f;
+        if (!CARRY && in && starts)
+            h[i] = starts[chunk * SP + q * kStates + i];
+        else if (!CARRY && in && p.initial)
+            h[i] = p.initial[state + i];
     }
     // as a thread of elements: its channels' parameters and rows
     const int e0 = w.first + el.c, have = max(0, min(EPT, w.end - e0));
     float skip[EPT], bias[EPT];
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-        skip[i] = p.skip && i < have ? p.skip[e0 + i] : 0.0f;
+        skip[i] = !CARRY && p.skip && i < have ? p.skip[e0 + i] : 0.0f;
         bias[i] = p.dt_bias && i < have ? p.dt_bias[e0 + i] : 0.0f;
     }
     const IO *xs = static_cast<const IO *>(p.x) + (long)w.n * p.x_n + e0;
     const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + e0;
-    const IO *zs = p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + e0 : nullptr;
+    const IO *zs = !CARRY && p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + e0 : nullptr;
     IO *out = static_cast<IO *>(p.out) + (long)w.n * p.L * p.E + e0;
 
     float x[EPT], d[EPT], z[EPT], side[PER];
     auto request = [&](int t0) {
-        const int t = t0 + el.j, n = t < w.len ? have : 0;
+        const int t = t0 + el.j, n = t < w.to ? have : 0;
         load_row<EPT>(xs + (long)t * p.x_t, n, wide, x);
         load_row<EPT>(ds + (long)t * p.dt_t, n, wide, d);
         if (zs) load_row<EPT>(zs + (long)t * p.gate_t, n, wide, z);
         load_bc<LANES, IO>(p, w, t0, side);
     };
-    request(0);
-    for (int t0 = 0; t0 < w.len; t0 += kSteps) {
-        const bool on = t0 + el.j < w.len;
+    if (w.from < w.to) request(w.from);
+    for (int t0 = w.from; t0 < w.to; t0 += kSteps) {
+        const bool on = t0 + el.j < w.to;
         float xk[EPT], zk[EPT];
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
@@ -231,31 +308,40 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
             if (at < 2 * kSteps * SP) bc[at / (2 * SP)][at % (2 * SP)] = side[i];
         }
         __syncthreads();
-        if (t0 + kSteps < w.len) request(t0 + kSteps);
-        if (keep && live)
+        if (t0 + kSteps < w.to) request(t0 + kSteps);
+        if (!CARRY && keep && live)
             *reinterpret_cast<float4 *>(
                 keep + (((long)w.n * ((p.L + kSteps - 1) / kSteps) + t0 / kSteps) * p.E + e) * SP + q * kStates) =
                 make_float4(h[0], h[1], h[2], h[3]);
-        for (int j0 = 0; j0 < kSteps && t0 + j0 < w.len; j0 += 4) {
+        Four f[2];
+        load_four<LANES, !CARRY>(f[0], steps, bc, 0, ch, q);
 #pragma unroll
-            for (int j1 = 0; j1 < 4; ++j1) {
-                const int j = j0 + j1;
-                const float2 s = steps[j][ch];
-                const float4 b4 = *reinterpret_cast<const float4 *>(&bc[j][q * kStates]);
-                const float4 c4 = *reinterpret_cast<const float4 *>(&bc[j][SP + q * kStates]);
-                const float b[4] = {b4.x, b4.y, b4.z, b4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
-                float y = 0.0f;
+        for (int j0 = 0; j0 < kSteps; j0 += 4) {
+            if (t0 + j0 >= w.to) break;
+            const Four &g = f[(j0 / 4) & 1];
+            if (j0 + 4 < kSteps) load_four<LANES, !CARRY>(f[(j0 / 4 + 1) & 1], steps, bc, j0 + 4, ch, q);
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                y[j] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < kStates; ++i) {
-                    h[i] = fmaf(exp2_hw(s.x * a[i]), h[i], s.y * b[i]);
-                    y = fmaf(c[i], h[i], y);
+                    h[i] = fmaf(exp2_hw(g.s[j].x * a[i]), h[i], g.s[j].y * g.b[j][i]);
+                    if (!CARRY) y[j] = fmaf(g.c[j][i], h[i], y[j]);
                 }
-                y = channel_sum<LANES>(y);
-                if (q == 0) ys[j][ch] = y;
+                if (CARRY) total += g.s[j].x;
+            }
+            if (!CARRY) {
+                float r[StepSums<LANES>::kept];
+                StepSums<LANES>::add(y, q, r);
+                // (with more than four lanes a channel, groups of four write the same)
+#pragma unroll
+                for (int j = 0; j < StepSums<LANES>::kept; ++j)
+                    ys[j0 + StepSums<LANES>::step(q) + j][ch] = r[j];
             }
         }
         __syncthreads();
-        if (on) {
+        if (!CARRY && on) {
             float o[EPT];
 #pragma unroll
             for (int i = 0; i < EPT; ++i) {
@@ -265,6 +351,15 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
             store_row<EPT>(out + (long)(t0 + el.j) * p.E, have, wide, o);
         }
     }
+    if (CARRY) {
+        if (live) {
+            *reinterpret_cast<float4 *>(chunks.local + chunk * SP + q * kStates) =
+                make_float4(h[0], h[1], h[2], h[3]);
+            if (q == 0) chunks.total[chunk] = total;
+        }
+        return;
+    }
+    if (blockIdx.z + 1 != gridDim.z) return;
     // the steps that do not count
     const float zero[EPT] = {};
     for (int t = w.len + el.j; t < p.L; t += kSteps) store_row<EPT>(out + (long)t * p.E, have, wide, zero);
@@ -273,6 +368,40 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
         for (int i = 0; i < kStates; ++i)
             if (q * kStates + i < p.S) p.last[state + i] = h[i];
     }
+}
+
+// Joins chunks: turns what each makes of zeros into what stands in front of it,
+// in place; backwards for the reverse recurrence, whose end (in front of the
+// sequence) goes to `end`.  A thread has one state.
+__global__ __launch_bounds__(kThreads) void scan_join_kernel(const float *__restrict__ a, const float *__restrict__ first,
+                                                             Chunks chunks, int count, int E, int S, int SP,
+                                                             bool backwards, float *__restrict__ end) {
+    const long i = (long)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= (long)E * SP) return;
+    const int n = blockIdx.y, e = (int)(i / SP), k = (int)(i - (long)e * SP);
+    if (k >= S) return;
+    const float rate = a[(long)e * S + k] * kLog2e;
+    const long state = ((long)n * E + e) * S + k;
+    float h = first ? first[state] : 0.0f;
+    for (int c0 = 0; c0 < count; c0 += 8) {
+        float local[8], total[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (c0 + c >= count) break;
+            const int at = backwards ? count - 1 - c0 - c : c0 + c;
+            const long chunk = ((long)n * count + at) * E + e;
+            local[c] = chunks.local[chunk * SP + k];
+            total[c] = chunks.total[chunk];
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (c0 + c >= count) break;
+            const int at = backwards ? count - 1 - c0 - c : c0 + c;
+            chunks.local[(((long)n * count + at) * E + e) * SP + k] = h;
+            h = fmaf(exp2_hw(rate * total[c]), h, local[c]);
+        }
+    }
+    if (end) end[state] = h;
 }
 
 // The backward pass walks up time.  A tile's states are computed again from the
@@ -285,7 +414,8 @@ template <typename IO, int LANES>
 __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t p, warpctct_scan_grad_t g,
                                                                 const float *__restrict__ keep,
                                                                 float *__restrict__ part_bc,
-                                                                float *__restrict__ part_sums, bool wide) {
+                                                                float *__restrict__ part_sums, int chunk_tiles,
+                                                                const float *__restrict__ starts, bool wide) {
     constexpr int CH = kThreads / LANES, EPT = Elements<LANES>::EPT, SP = Shared<LANES>::SP, PER = Shared<LANES>::PER;
     constexpr int WAVES = kThreads / 64;
     // d, d x, gy, and y without the skip; on the way back the first two give way
@@ -294,7 +424,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     __shared__ float4 steps[kSteps][CH];
     __shared__ __align__(16) float bc[kSteps][2 * SP];
     __shared__ float sums[WAVES][kSteps][2 * SP];   // gb, gc of a wavefront
-    const Place w = place_of<LANES>(p);
+    const Place w = place_of<LANES>(p, chunk_tiles);
     const Elements<LANES> el;
     const int ch = threadIdx.x / LANES, q = threadIdx.x % LANES, e = w.first + ch;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -306,7 +436,11 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     for (int i = 0; i < kStates; ++i) {
         const bool in = live && q * kStates + i < p.S;
         a[i] = in ? p.a[(long)e * p.S + q * kStates + i] : 0.0f;
-        carry[i] = in && g.grad_last ? g.grad_last[state + i] : 0.0f;
+        carry[i] = 0.0f;
+        if (in && starts)
+            carry[i] = starts[(((long)w.n * gridDim.z + blockIdx.z) * p.E + e) * SP + q * kStates + i];
+        else if (in && g.grad_last)
+            carry[i] = g.grad_last[state + i];
         ga[i] = 0.0f;
     }
     const int e0 = w.first + el.c, have = max(0, min(EPT, w.end - e0));
@@ -326,14 +460,14 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     IO *gz = p.gate ? static_cast<IO *>(g.grad_gate) + rows : nullptr;
 
     const float zero[EPT] = {};
-    for (int t = w.len + el.j; t < p.L; t += kSteps) {
+    for (int t = blockIdx.z + 1 == gridDim.z ? w.len + el.j : p.L; t < p.L; t += kSteps) {
         store_row<EPT>(gx + (long)t * p.E, have, wide, zero);
         store_row<EPT>(gd + (long)t * p.E, have, wide, zero);
         if (gz) store_row<EPT>(gz + (long)t * p.E, have, wide, zero);
     }
-    for (int tile = (w.len + kSteps - 1) / kSteps - 1; tile >= 0; --tile) {
+    for (int tile = (w.to + kSteps - 1) / kSteps - 1; tile * kSteps >= w.from && tile >= 0; --tile) {
         const int t0 = tile * kSteps, t = t0 + el.j;
-        const bool on = t < w.len;
+        const bool on = t < w.to;
         float x[EPT], raw[EPT], z[EPT], u[EPT], side[PER];
         load_row<EPT>(xs + (long)t * p.x_t, on ? have : 0, wide, x);
         load_row<EPT>(ds + (long)t * p.dt_t, on ? have : 0, wide, raw);
@@ -448,13 +582,13 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
             to[at] = s;
         }
     }
-    if (g.grad_initial && live) {
+    if (g.grad_initial && !starts && live) {
 #pragma unroll
         for (int i = 0; i < kStates; ++i)
             if (q * kStates + i < p.S) g.grad_initial[state + i] = carry[i];
     }
-    // the sums over time: a row of E S + 2 E floats for every sequence
-    float *mine = part_sums + (size_t)w.n * p.E * (p.S + 2);
+    // the sums over time: a row of E S + 2 E floats for every chunk
+    float *mine = part_sums + ((size_t)w.n * gridDim.z + blockIdx.z) * p.E * (p.S + 2);
     if (live) {
 #pragma unroll
         for (int i = 0; i < kStates; ++i)
@@ -475,6 +609,79 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
         mine[(long)p.E * p.S + w.first + c] = s;
         mine[(long)p.E * p.S + p.E + w.first + c] = b;
     }
+}
+
+// The first pass of the reverse recurrence over chunks: what each makes of zeros
+// behind it, k_t gh_t of its first step, and its sum of d.
+template <typename IO, int LANES>
+__global__ __launch_bounds__(kThreads) void scan_grad_carry_kernel(warpctct_scan_t p, warpctct_scan_grad_t g,
+                                                                   Chunks chunks, bool wide) {
+    constexpr int CH = kThreads / LANES, EPT = Elements<LANES>::EPT, SP = Shared<LANES>::SP, PER = Shared<LANES>::PER;
+    __shared__ float2 steps[kSteps][CH];           // d, gy
+    __shared__ __align__(16) float bc[kSteps][2 * SP];
+    const Place w = place_of<LANES>(p, chunks.tiles);
+    const Elements<LANES> el;
+    const int ch = threadIdx.x / LANES, q = threadIdx.x % LANES, e = w.first + ch;
+    const bool live = e < w.end;
+    float a[kStates], carry[kStates], total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kStates; ++i) {
+        const bool in = live && q * kStates + i < p.S;
+        a[i] = in ? p.a[(long)e * p.S + q * kStates + i] * kLog2e : 0.0f;
+        carry[i] = 0.0f;
+    }
+    const int e0 = w.first + el.c, have = max(0, min(EPT, w.end - e0));
+    float bias[EPT];
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) bias[i] = p.dt_bias && i < have ? p.dt_bias[e0 + i] : 0.0f;
+    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + e0;
+    const IO *zs = p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + e0 : nullptr;
+    const IO *us = static_cast<const IO *>(g.grad_out) + (long)w.n * g.grad_n + e0;
+    float d[EPT], u[EPT], z[EPT], side[PER];
+    auto request = [&](int t0) {
+        const int t = t0 + el.j, n = t < w.to ? have : 0;
+        load_row<EPT>(ds + (long)t * p.dt_t, n, wide, d);
+        load_row<EPT>(us + (long)t * g.grad_t, n, wide, u);
+        if (zs) load_row<EPT>(zs + (long)t * p.gate_t, n, wide, z);
+        load_bc<LANES, IO>(p, w, t0, side);
+    };
+    const int last = w.from + (w.to - w.from - 1) / kSteps * kSteps;
+    if (w.from < w.to) request(last);
+    for (int t0 = w.from < w.to ? last : -1; t0 >= w.from; t0 -= kSteps) {
+        const bool on = t0 + el.j < w.to;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+            float v = d[i] + bias[i];
+            if (p.softplus) v = softplus(v).value;
+            if (!(on && i < have)) v = 0.0f;
+            float y = u[i];
+            if (zs) y *= z[i] * sigmoid(z[i]);
+            if (!(on && i < have)) y = 0.0f;
+            steps[el.j][el.c + i] = make_float2(v, y);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int at = i * kThreads + threadIdx.x;
+            if (at < 2 * kSteps * SP) bc[at / (2 * SP)][at % (2 * SP)] = side[i];
+        }
+        __syncthreads();
+        if (t0 - kSteps >= w.from) request(t0 - kSteps);
+#pragma unroll
+        for (int j = kSteps - 1; j >= 0; --j) {
+            const float2 s = steps[j][ch];
+            const float4 c4 = *reinterpret_cast<const float4 *>(&bc[j][SP + q * kStates]);
+            const float c[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+            for (int i = 0; i < kStates; ++i) carry[i] = exp2_hw(s.x * a[i]) * fmaf(c[i], s.y, carry[i]);
+            total += s.x;
+        }
+        __syncthreads();
+    }
+    if (!live) return;
+    const long chunk = ((long)w.n * gridDim.z + blockIdx.z) * p.E + e;
+    *reinterpret_cast<float4 *>(chunks.local + chunk * SP + q * kStates) =
+        make_float4(carry[0], carry[1], carry[2], carry[3]);
+    if (q == 0) chunks.total[chunk] = total;
 }
 
 // gb, gc (N, L, G, S): the workgroups' partial sums of a group added up, zero
@@ -572,24 +779,82 @@ bool rows_wide(const warpctct_scan_t &p) {
            aligned16(p.gate) && aligned16(p.out);
 }
 
+// Chunks that a sequence is cut into: one while its workgroups alone put a
+// wavefront on every second SIMD or more, since two passes cost twice the
+// arithmetic; otherwise as many as put two wavefronts on each, of two tiles at
+// least.
+struct Cut {
+    int count, tiles;
+};
+Cut cut_of(const warpctct_scan_t &p) {
+    const long waves = (long)p.N * p.G * blocks_of(p) * (kThreads / 64), tiles = ((long)p.L + kSteps - 1) / kSteps;
+    Cut c = {1, (int)tiles};
+    if (waves <= 0 || waves > 512 || tiles < 4) return c;
+    const long count = std::min(2048 / waves, tiles / 2);
+    c.tiles = (int)((tiles + count - 1) / count);
+    c.count = (int)((tiles + c.tiles - 1) / c.tiles);
+    return c;
+}
+size_t chunk_floats(const warpctct_scan_t &p) {
+    const Cut c = cut_of(p);
+    return c.count > 1 ? (size_t)p.N * c.count * p.E * (kStates * lanes_of(p.S) + 1) : 0;
+}
+Chunks chunks_of(const warpctct_scan_t &p, float *workspace) {
+    const Cut c = cut_of(p);
+    Chunks k;
+    k.local = workspace;
+    k.total = workspace + (c.count > 1 ? (size_t)p.N * c.count * p.E * (kStates * lanes_of(p.S)) : 0);
+    k.tiles = c.tiles;
+    return k;
+}
+hipError_t join_chunks(const warpctct_scan_t &p, const float *first, const Chunks &chunks, bool backwards, float *end,
+                       hipStream_t stream) {
+    const int SP = kStates * lanes_of(p.S);
+    const long threads = (long)p.E * SP;
+    TIMED_LAUNCH(scan_join_kernel, dim3((unsigned)((threads + kThreads - 1) / kThreads), p.N), dim3(kThreads), 0,
+                 stream, p.a, first, chunks, cut_of(p).count, p.E, p.S, SP, backwards, end);
+    return hipGetLastError();
+}
+
 template <typename IO, int LANES>
-hipError_t start(const warpctct_scan_t &p, float *keep, hipStream_t stream) {
-    auto kernel = scan_kernel<IO, LANES>;
-    TIMED_LAUNCH(kernel, dim3(p.G * blocks_of(p), p.N), dim3(kThreads), 0, stream, p, keep, rows_wide<IO>(p));
+hipError_t start(const warpctct_scan_t &p, float *keep, float *workspace, hipStream_t stream) {
+    const Cut cut = cut_of(p);
+    const Chunks chunks = chunks_of(p, workspace);
+    const dim3 grid(p.G * blocks_of(p), p.N, cut.count);
+    const bool wide = rows_wide<IO>(p);
+    if (cut.count > 1) {
+        auto carry = scan_kernel<IO, LANES, true>;
+        TIMED_LAUNCH(carry, grid, dim3(kThreads), 0, stream, p, nullptr, chunks, nullptr, wide);
+        const hipError_t e = join_chunks(p, p.initial, chunks, false, nullptr, stream);
+        if (e != hipSuccess) return e;
+    }
+    auto kernel = scan_kernel<IO, LANES, false>;
+    TIMED_LAUNCH(kernel, grid, dim3(kThreads), 0, stream, p, keep, chunks, cut.count > 1 ? chunks.local : nullptr, wide);
     return hipGetLastError();
 }
 
 template <typename IO, int LANES>
 hipError_t start(const warpctct_scan_t &p, const warpctct_scan_grad_t &g, const float *keep, float *part_bc,
-                 float *part_sums, hipStream_t stream) {
+                 float *part_sums, float *workspace, hipStream_t stream) {
     constexpr int V = kVec<IO>;
     const bool wide = rows_wide<IO>(p) && g.grad_n % V == 0 && g.grad_t % V == 0 && aligned16(g.grad_out) &&
                       aligned16(g.grad_x) && aligned16(g.grad_dt) && aligned16(g.grad_gate);
     const int blocks = blocks_of(p);
     if (p.N == 0) return hipSuccess;
+    const Cut cut = cut_of(p);
+    const Chunks chunks = chunks_of(p, workspace);
+    const dim3 grid(p.G * blocks, p.N, cut.count);
+    hipError_t e;
+    if (cut.count > 1) {
+        auto carry = scan_grad_carry_kernel<IO, LANES>;
+        TIMED_LAUNCH(carry, grid, dim3(kThreads), 0, stream, p, g, chunks, wide);
+        e = join_chunks(p, g.grad_last, chunks, true, g.grad_initial, stream);
+        if (e != hipSuccess) return e;
+    }
     auto kernel = scan_grad_kernel<IO, LANES>;
-    TIMED_LAUNCH(kernel, dim3(p.G * blocks, p.N), dim3(kThreads), 0, stream, p, g, keep, part_bc, part_sums, wide);
-    hipError_t e = hipGetLastError();
+    TIMED_LAUNCH(kernel, grid, dim3(kThreads), 0, stream, p, g, keep, part_bc, part_sums, cut.tiles,
+                 cut.count > 1 ? chunks.local : nullptr, wide);
+    e = hipGetLastError();
     if (e != hipSuccess || p.L == 0) return e;
     auto join = scan_grad_bc_kernel<IO>;
     const long values = (long)p.L * 2 * p.G * p.S;
@@ -635,22 +900,24 @@ size_t scan_keep_floats(int N, int L, int E, int S) {
     return (size_t)N * ((L + kSteps - 1) / kSteps) * E * (kStates * lanes_of(S));
 }
 
+size_t scan_floats(const warpctct_scan_t &p) { return chunk_floats(p); }
+
 size_t scan_grad_floats(const warpctct_scan_t &p) {
-    return part_bc_floats(p) + column_sums_floats(p.N, (long)p.E * (p.S + 2));
+    return part_bc_floats(p) + chunk_floats(p) + column_sums_floats((long)p.N * cut_of(p).count, (long)p.E * (p.S + 2));
 }
 
-hipError_t launch_scan(const warpctct_scan_t &p, float *keep, hipStream_t stream) {
-    return by_type(p.dtype, p.S, p, keep, stream);
+hipError_t launch_scan(const warpctct_scan_t &p, float *keep, float *workspace, hipStream_t stream) {
+    return by_type(p.dtype, p.S, p, keep, workspace, stream);
 }
 
 hipError_t launch_scan_grad(const warpctct_scan_t &p, const warpctct_scan_grad_t &g, const float *keep,
                             float *workspace, hipStream_t stream) {
-    float *part_bc = workspace, *part_sums = workspace + part_bc_floats(p);
-    const hipError_t e = by_type(p.dtype, p.S, p, g, keep, part_bc, part_sums, stream);
+    float *part_bc = workspace, *local = part_bc + part_bc_floats(p), *part_sums = local + chunk_floats(p);
+    const hipError_t e = by_type(p.dtype, p.S, p, g, keep, part_bc, part_sums, local, stream);
     if (e != hipSuccess) return e;
     // (the skip's and the bias's gradients lie next to each other)
-    return launch_column_sums(part_sums, p.N, p.E * (p.S + 2), p.E * p.S, g.grad_a, kIoF32, g.grad_skip_bias, kIoF32,
-                              stream);
+    return launch_column_sums(part_sums, (long)p.N * cut_of(p).count, p.E * (p.S + 2), p.E * p.S, g.grad_a, kIoF32,
+                              g.grad_skip_bias, kIoF32, stream);
 }
 
 hipError_t launch_scan_step(const warpctct_scan_step_t &p, hipStream_t stream) {
