@@ -613,11 +613,11 @@ int warpctct_causal_conv_step(const warpctct_conv_step_t *p, void *stream);
  * step, last (N, E, S; may be NULL) receives those behind the last one that
  * counts.  out (N, L, E) dense.
  * keep (warpctct_selective_scan_keep_bytes, 16-byte aligned; NULL without a
- * backward pass) receives the states in front of every WARPCTCT_SCAN_TILE steps.
+ * backward pass) receives the states in front of every few steps.
  * workspace: warpctct_selective_scan_workspace_bytes(..., 0), 16-byte aligned (0
  * bytes, may be NULL, unless few long sequences are cut into chunks).
  * N <= 65535. */
-enum { WARPCTCT_SCAN_MAX_STATES = 64, WARPCTCT_SCAN_TILE = 16 };
+enum { WARPCTCT_SCAN_MAX_STATES = 64 };
 typedef struct {
     int dtype, N, L, E, S, G, softplus;
     long x_n, x_t, dt_n, dt_t, gate_n, gate_t, b_n, b_t, b_g, c_n, c_t, c_g;

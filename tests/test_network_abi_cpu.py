@@ -187,7 +187,7 @@ def test_selective_scan_arguments():
     lib = hip_lib.lib()
     size = lib.warpctct_selective_scan_keep_bytes
     size.restype = ctypes.c_size_t
-    assert size(2, 20, 8, 16) == 2 * 2 * 8 * 16 * 4 and size(2, 20, 8, 5) == 2 * 2 * 8 * 8 * 4
+    assert size(2, 20, 8, 16) == 2 * 3 * 8 * 16 * 4 and size(2, 20, 8, 5) == 2 * 3 * 8 * 8 * 4
     assert size(2, 0, 8, 16) == 0 and size(2, 20, 8, 65) == 0
 
     def call(keep=0, have=0, workspace=0, scratch=0, **over):
@@ -198,7 +198,7 @@ def test_selective_scan_arguments():
     assert lib.warpctct_selective_scan(P(0), P(0), none, P(0), none, P(0)) == EINVAL
     for bad in BAD_SCANS + (dict(out=None),):
         assert call(**bad) == EINVAL, bad
-    assert call(keep=ALIGNED, have=2047) == EWORKSPACE
+    assert call(keep=ALIGNED, have=3071) == EWORKSPACE
     assert call(keep=ALIGNED + 4, have=1 << 20) == EINVAL
     # few long sequences take scratch: at least the states and the sum of every chunk but one
     size = lib.warpctct_selective_scan_workspace_bytes
@@ -231,7 +231,7 @@ def test_selective_scan_gradient_and_step_arguments():
         assert call(**{bad: None}) == EINVAL, bad
     assert call(scan(gate=SOME)) == EINVAL
     assert call(keep=0) == EINVAL and call(workspace=0) == EINVAL and call(workspace=ALIGNED + 4) == EINVAL
-    assert call(kept=2047) == EWORKSPACE and call(have=need - 1) == EWORKSPACE
+    assert call(kept=3071) == EWORKSPACE and call(have=need - 1) == EWORKSPACE
 
     def step(**over):
         fields = dict(dtype=F16, N=2, E=8, S=16, G=1, x=SOME, dt=SOME, b=SOME, c=SOME, a=SOME, state=SOME, out=SOME)

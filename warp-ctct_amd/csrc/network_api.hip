@@ -35,7 +35,7 @@ bool conv_ok(const warpctct_conv_t *p) {
 bool scan_sizes_ok(int dtype, int N, int L, int E, int S, int G) {
     return io_valid(dtype) && N >= 0 && N <= kMostBatch && L >= 0 && E >= 1 && E <= (1 << 24) && S >= 1 &&
            S <= WARPCTCT_SCAN_MAX_STATES && G >= 1 && E % G == 0 && (long)L * G * S < (1L << 36) &&
-           L <= 0x7fffffff - WARPCTCT_SCAN_TILE;
+           L <= (1 << 30);
 }
 bool scan_ok(const warpctct_scan_t *p) {
     return p && scan_sizes_ok(p->dtype, p->N, p->L, p->E, p->S, p->G) &&

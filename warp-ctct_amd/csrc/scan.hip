@@ -39,9 +39,15 @@ namespace wctct {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kSteps = WARPCTCT_SCAN_TILE;      // of a tile
+constexpr int kSteps = 16;                      // of a tile
 constexpr int kStates = 4;                      // of a lane
 constexpr float kLog2e = 1.4426950408889634f;
+
+// Steps of a tile of the backward pass, which is also how far apart the states
+// lie that the forward pass keeps for it: the states and factors of a tile take
+// 8 registers a step, 64 of them leave room for three wavefronts on a SIMD (16
+// steps: 256 registers and spills), and a thread has up to 4 elements.
+constexpr int back_steps(int lanes) { return lanes == 1 ? 4 : lanes == 16 ? 16 : 8; }
 
 __device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
 
@@ -124,9 +130,9 @@ __device__ __forceinline__ Place place_of(const warpctct_scan_t &p, int chunk_ti
 }
 
 // A thread's elements of a tile: EPT channels next to each other of one step.
-template <int LANES>
+template <int LANES, int STEPS>
 struct Elements {
-    static constexpr int CH = kThreads / LANES, EPT = kSteps / LANES;
+    static constexpr int CH = kThreads / LANES, EPT = STEPS * CH / kThreads;
     int j, c;        // step in the tile, first channel in the workgroup
     __device__ __forceinline__ Elements() {
         const int at = threadIdx.x * EPT;
@@ -161,24 +167,24 @@ __device__ __forceinline__ void store_row(IO *p, int have, bool wide, const floa
     }
 }
 
-// The tile's rows of b and c, kSteps x 2 SP values, by all threads.
-template <int LANES>
+// The tile's rows of b and c, STEPS x 2 SP values, by all threads.
+template <int LANES, int STEPS>
 struct Shared {
     static constexpr int SP = kStates * LANES;
-    static constexpr int PER = (2 * kSteps * SP + kThreads - 1) / kThreads;
+    static constexpr int PER = (2 * STEPS * SP + kThreads - 1) / kThreads;
 };
-template <int LANES, typename IO>
+template <int LANES, int STEPS, typename IO>
 __device__ __forceinline__ void load_bc(const warpctct_scan_t &p, const Place &w, int t0,
-                                        float (&v)[Shared<LANES>::PER]) {
-    constexpr int SP = Shared<LANES>::SP;
+                                        float (&v)[Shared<LANES, STEPS>::PER]) {
+    constexpr int SP = Shared<LANES, STEPS>::SP;
     const IO *b = static_cast<const IO *>(p.b) + (long)w.n * p.b_n + (long)w.g * p.b_g;
     const IO *c = static_cast<const IO *>(p.c) + (long)w.n * p.c_n + (long)w.g * p.c_g;
 #pragma unroll
-    for (int i = 0; i < Shared<LANES>::PER; ++i) {
+    for (int i = 0; i < Shared<LANES, STEPS>::PER; ++i) {
         const int at = i * kThreads + threadIdx.x, j = at / (2 * SP), k = at % (2 * SP);
         const int s = k % SP, t = t0 + j;
         v[i] = 0.0f;
-        if (j < kSteps && t < w.len && s < p.S)
+        if (j < STEPS && t < w.len && s < p.S)
             v[i] = to_float(k < SP ? b[(long)t * p.b_t + s] : c[(long)t * p.c_t + s]);
     }
 }
@@ -246,12 +252,14 @@ struct Chunks {
 template <typename IO, int LANES, bool CARRY>
 __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float *__restrict__ keep, Chunks chunks,
                                                         const float *__restrict__ starts, bool wide) {
-    constexpr int CH = kThreads / LANES, EPT = Elements<LANES>::EPT, SP = Shared<LANES>::SP, PER = Shared<LANES>::PER;
+    constexpr int CH = kThreads / LANES, SP = kStates * LANES, EPT = Elements<LANES, kSteps>::EPT;
+    constexpr int PER = Shared<LANES, kSteps>::PER;
     __shared__ float2 steps[kSteps][CH];           // d, d x
     __shared__ __align__(16) float bc[kSteps][2 * SP];
     __shared__ float ys[kSteps][CARRY ? 1 : CH];
+    constexpr int BACK = back_steps(LANES);
     const Place w = place_of<LANES>(p, chunks.tiles);
-    const Elements<LANES> el;
+    const Elements<LANES, kSteps> el;
     // as a lane: a channel and four of its states
     const int ch = threadIdx.x / LANES, q = threadIdx.x % LANES, e = w.first + ch;
     const bool live = e < w.end;
@@ -287,7 +295,7 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
         load_row<EPT>(xs + (long)t * p.x_t, n, wide, x);
         load_row<EPT>(ds + (long)t * p.dt_t, n, wide, d);
         if (zs) load_row<EPT>(zs + (long)t * p.gate_t, n, wide, z);
-        load_bc<LANES, IO>(p, w, t0, side);
+        load_bc<LANES, kSteps, IO>(p, w, t0, side);
     };
     if (w.from < w.to) request(w.from);
     for (int t0 = w.from; t0 < w.to; t0 += kSteps) {
@@ -309,15 +317,15 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
         }
         __syncthreads();
         if (t0 + kSteps < w.to) request(t0 + kSteps);
-        if (!CARRY && keep && live)
-            *reinterpret_cast<float4 *>(
-                keep + (((long)w.n * ((p.L + kSteps - 1) / kSteps) + t0 / kSteps) * p.E + e) * SP + q * kStates) =
-                make_float4(h[0], h[1], h[2], h[3]);
         Four f[2];
         load_four<LANES, !CARRY>(f[0], steps, bc, 0, ch, q);
 #pragma unroll
         for (int j0 = 0; j0 < kSteps; j0 += 4) {
             if (t0 + j0 >= w.to) break;
+            if (!CARRY && keep && live && j0 % BACK == 0)
+                *reinterpret_cast<float4 *>(
+                    keep + (((long)w.n * ((p.L + BACK - 1) / BACK) + (t0 + j0) / BACK) * p.E + e) * SP + q * kStates) =
+                    make_float4(h[0], h[1], h[2], h[3]);
             const Four &g = f[(j0 / 4) & 1];
             if (j0 + 4 < kSteps) load_four<LANES, !CARRY>(f[(j0 / 4 + 1) & 1], steps, bc, j0 + 4, ch, q);
             float y[4];
@@ -416,20 +424,22 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
                                                                 float *__restrict__ part_bc,
                                                                 float *__restrict__ part_sums, int chunk_tiles,
                                                                 const float *__restrict__ starts, bool wide) {
-    constexpr int CH = kThreads / LANES, EPT = Elements<LANES>::EPT, SP = Shared<LANES>::SP, PER = Shared<LANES>::PER;
+    constexpr int STEPS = back_steps(LANES);
+    constexpr int CH = kThreads / LANES, SP = kStates * LANES, EPT = Elements<LANES, STEPS>::EPT;
+    constexpr int PER = Shared<LANES, STEPS>::PER;
     constexpr int WAVES = kThreads / 64;
     // d, d x, gy, and y without the skip; on the way back the first two give way
     // to sum gh b and sum a gh k h (a channel's lanes lie in one wavefront, which
     // has read a step before it overwrites it)
-    __shared__ float4 steps[kSteps][CH];
-    __shared__ __align__(16) float bc[kSteps][2 * SP];
-    __shared__ float sums[WAVES][kSteps][2 * SP];   // gb, gc of a wavefront
+    __shared__ float4 steps[STEPS][CH];
+    __shared__ __align__(16) float bc[STEPS][2 * SP];
+    __shared__ float sums[WAVES][STEPS][2 * SP];   // gb, gc of a wavefront
     const Place w = place_of<LANES>(p, chunk_tiles);
-    const Elements<LANES> el;
+    const Elements<LANES, STEPS> el;
     const int ch = threadIdx.x / LANES, q = threadIdx.x % LANES, e = w.first + ch;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool live = e < w.end;
-    const int tiles = (p.L + kSteps - 1) / kSteps;
+    const int tiles = (p.L + STEPS - 1) / STEPS;
     float a[kStates], carry[kStates], ga[kStates];
     const long state = ((long)w.n * p.E + e) * p.S + q * kStates;
 #pragma unroll
@@ -460,27 +470,31 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     IO *gz = p.gate ? static_cast<IO *>(g.grad_gate) + rows : nullptr;
 
     const float zero[EPT] = {};
-    for (int t = blockIdx.z + 1 == gridDim.z ? w.len + el.j : p.L; t < p.L; t += kSteps) {
+    for (int t = blockIdx.z + 1 == gridDim.z ? w.len + el.j : p.L; t < p.L; t += STEPS) {
         store_row<EPT>(gx + (long)t * p.E, have, wide, zero);
         store_row<EPT>(gd + (long)t * p.E, have, wide, zero);
         if (gz) store_row<EPT>(gz + (long)t * p.E, have, wide, zero);
     }
-    for (int tile = (w.to + kSteps - 1) / kSteps - 1; tile * kSteps >= w.from && tile >= 0; --tile) {
-        const int t0 = tile * kSteps, t = t0 + el.j;
+    // the rows of a tile and the states in front of it are asked for while the
+    // tile behind it is worked on
+    float x[EPT], raw[EPT], z[EPT], u[EPT], side[PER];
+    float4 front = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto request = [&](int tile) {
+        const int t = tile * STEPS + el.j, n = t < w.to ? have : 0;
+        load_row<EPT>(xs + (long)t * p.x_t, n, wide, x);
+        load_row<EPT>(ds + (long)t * p.dt_t, n, wide, raw);
+        load_row<EPT>(us + (long)t * g.grad_t, n, wide, u);
+        if (zs) load_row<EPT>(zs + (long)t * p.gate_t, n, wide, z);
+        load_bc<LANES, STEPS, IO>(p, w, tile * STEPS, side);
+        if (live)
+            front = *reinterpret_cast<const float4 *>(keep + (((long)w.n * tiles + tile) * p.E + e) * SP + q * kStates);
+    };
+    const int top = (w.to + STEPS - 1) / STEPS - 1, bottom = w.from < w.to ? w.from / STEPS : top + 1;
+    if (top >= bottom) request(top);
+    for (int tile = top; tile >= bottom; --tile) {
+        const int t = tile * STEPS + el.j;
         const bool on = t < w.to;
-        float x[EPT], raw[EPT], z[EPT], u[EPT], side[PER];
-        load_row<EPT>(xs + (long)t * p.x_t, on ? have : 0, wide, x);
-        load_row<EPT>(ds + (long)t * p.dt_t, on ? have : 0, wide, raw);
-        load_row<EPT>(us + (long)t * g.grad_t, on ? have : 0, wide, u);
-        if (zs) load_row<EPT>(zs + (long)t * p.gate_t, on ? have : 0, wide, z);
-        load_bc<LANES, IO>(p, w, t0, side);
-        float h0[kStates] = {};
-        if (live) {
-            const float4 v = *reinterpret_cast<const float4 *>(keep + (((long)w.n * tiles + tile) * p.E + e) * SP +
-                                                               q * kStates);
-            h0[0] = v.x, h0[1] = v.y, h0[2] = v.z, h0[3] = v.w;
-        }
-        float d[EPT], slope[EPT], gy[EPT], silu[EPT], dsilu[EPT];
+        float xk[EPT], d[EPT], slope[EPT], uk[EPT], zk[EPT];
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
             const float v = raw[i] + bias[i];
@@ -491,91 +505,106 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
                 d[i] = s.value;
                 slope[i] = s.slope;
             }
-            if (!(on && i < have)) d[i] = 0.0f;
-            silu[i] = 1.0f;
-            dsilu[i] = 0.0f;
-            if (zs) {
-                const float s = sigmoid(z[i]);
-                silu[i] = z[i] * s;
-                dsilu[i] = s * fmaf(z[i], 1.0f - s, 1.0f);
-            }
-            gy[i] = u[i] * silu[i];
-            if (!(on && i < have)) gy[i] = 0.0f;
-            steps[el.j][el.c + i] = make_float4(d[i], d[i] * x[i], gy[i], 0.0f);
-            gskip[i] = fmaf(gy[i], x[i], gskip[i]);
+            float gy = u[i];
+            if (zs) gy *= z[i] * sigmoid(z[i]);
+            if (!(on && i < have)) d[i] = gy = 0.0f;
+            steps[el.j][el.c + i] = make_float4(d[i], d[i] * x[i], gy, 0.0f);
+            gskip[i] = fmaf(gy, x[i], gskip[i]);
+            xk[i] = x[i];
+            uk[i] = u[i];
+            zk[i] = z[i];
         }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int at = i * kThreads + threadIdx.x;
-            if (at < 2 * kSteps * SP) bc[at / (2 * SP)][at % (2 * SP)] = side[i];
+            if (at < 2 * STEPS * SP) bc[at / (2 * SP)][at % (2 * SP)] = side[i];
         }
+        const float h0[kStates] = {front.x, front.y, front.z, front.w};
         __syncthreads();
-        float k[kSteps][kStates], h[kSteps][kStates];
+        if (tile > bottom) request(tile - 1);
+        float k[STEPS][kStates], h[STEPS][kStates];
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            const float4 s = steps[j][ch];
-            const float4 b4 = *reinterpret_cast<const float4 *>(&bc[j][q * kStates]);
-            const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+        for (int j0 = 0; j0 < STEPS; j0 += 4) {
+            __builtin_amdgcn_sched_barrier(0);
+            float y[4];
 #pragma unroll
-            for (int i = 0; i < kStates; ++i) {
-                k[j][i] = exp2_hw(s.x * (a[i] * kLog2e));
-                h[j][i] = fmaf(k[j][i], j ? h[j - 1][i] : h0[i], s.y * b[i]);
+            for (int j = j0; j < j0 + 4; ++j) {
+                const float2 s = *reinterpret_cast<const float2 *>(&steps[j][ch]);
+                const float4 b4 = *reinterpret_cast<const float4 *>(&bc[j][q * kStates]);
+                const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+                for (int i = 0; i < kStates; ++i) {
+                    k[j][i] = exp2_hw(s.x * (a[i] * kLog2e));
+                    h[j][i] = fmaf(k[j][i], j ? h[j - 1][i] : h0[i], s.y * b[i]);
+                }
+                const float4 c4 = *reinterpret_cast<const float4 *>(&bc[j][SP + q * kStates]);
+                y[j - j0] = fmaf(c4.w, h[j][3], fmaf(c4.z, h[j][2], fmaf(c4.y, h[j][1], c4.x * h[j][0])));
             }
             if (zs) {
+                float r[StepSums<LANES>::kept];
+                StepSums<LANES>::add(y, q, r);
+#pragma unroll
+                for (int j = 0; j < StepSums<LANES>::kept; ++j) steps[j0 + StepSums<LANES>::step(q) + j][ch].w = r[j];
+            }
+        }
+#pragma unroll
+        for (int j0 = STEPS - 4; j0 >= 0; j0 -= 4) {
+            __builtin_amdgcn_sched_barrier(0);
+            float ghb[4], akh[4];
+#pragma unroll
+            for (int j = j0 + 3; j >= j0; --j) {
+                const float4 s = steps[j][ch];
+                const float4 b4 = *reinterpret_cast<const float4 *>(&bc[j][q * kStates]);
                 const float4 c4 = *reinterpret_cast<const float4 *>(&bc[j][SP + q * kStates]);
-                float y = c4.x * h[j][0];
-                y = fmaf(c4.y, h[j][1], y);
-                y = fmaf(c4.z, h[j][2], y);
-                y = fmaf(c4.w, h[j][3], y);
-                y = channel_sum<LANES>(y);
-                if (q == 0) steps[j][ch].w = y;
-            }
-        }
+                const float b[4] = {b4.x, b4.y, b4.z, b4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
+                float vb[kStates], vc[kStates];
+                ghb[j - j0] = akh[j - j0] = 0.0f;
 #pragma unroll
-        for (int j = kSteps - 1; j >= 0; --j) {
-            const float4 s = steps[j][ch];
-            const float4 b4 = *reinterpret_cast<const float4 *>(&bc[j][q * kStates]);
-            const float4 c4 = *reinterpret_cast<const float4 *>(&bc[j][SP + q * kStates]);
-            const float b[4] = {b4.x, b4.y, b4.z, b4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
-            float ghb = 0.0f, akh = 0.0f, vb[kStates], vc[kStates];
+                for (int i = 0; i < kStates; ++i) {
+                    const float gh = fmaf(c[i], s.z, carry[i]);
+                    ghb[j - j0] = fmaf(gh, b[i], ghb[j - j0]);
+                    vb[i] = gh * s.y;
+                    vc[i] = h[j][i] * s.z;
+                    carry[i] = gh * k[j][i];
+                    const float r = carry[i] * (j ? h[j - 1][i] : h0[i]);
+                    akh[j - j0] = fmaf(a[i], r, akh[j - j0]);
+                    ga[i] = fmaf(s.x, r, ga[i]);
+                }
+                const float sb = sum_over_channels<LANES>(vb), sc = sum_over_channels<LANES>(vc);
+                if ((lane & 15) < LANES) {
+                    const int row = lane >> 4, s_at = (lane % LANES) * kStates + (row & 1) * 2 + (row >> 1);
+                    sums[wave][j][s_at] = sb;
+                    sums[wave][j][SP + s_at] = sc;
+                }
+            }
+            float rb[StepSums<LANES>::kept], ra[StepSums<LANES>::kept];
+            StepSums<LANES>::add(ghb, q, rb);
+            StepSums<LANES>::add(akh, q, ra);
 #pragma unroll
-            for (int i = 0; i < kStates; ++i) {
-                const float gh = fmaf(c[i], s.z, carry[i]);
-                ghb = fmaf(gh, b[i], ghb);
-                vb[i] = gh * s.y;
-                vc[i] = h[j][i] * s.z;
-                carry[i] = gh * k[j][i];
-                const float r = carry[i] * (j ? h[j - 1][i] : h0[i]);
-                akh = fmaf(a[i], r, akh);
-                ga[i] = fmaf(s.x, r, ga[i]);
-            }
-            ghb = channel_sum<LANES>(ghb);
-            akh = channel_sum<LANES>(akh);
-            if (q == 0) *reinterpret_cast<float2 *>(&steps[j][ch]) = make_float2(ghb, akh);
-            const float sb = sum_over_channels<LANES>(vb), sc = sum_over_channels<LANES>(vc);
-            if ((lane & 15) < LANES) {
-                const int row = lane >> 4, s_at = (lane % LANES) * kStates + (row & 1) * 2 + (row >> 1);
-                sums[wave][j][s_at] = sb;
-                sums[wave][j][SP + s_at] = sc;
-            }
+            for (int j = 0; j < StepSums<LANES>::kept; ++j)
+                *reinterpret_cast<float2 *>(&steps[j0 + StepSums<LANES>::step(q) + j][ch]) = make_float2(rb[j], ra[j]);
         }
+        __builtin_amdgcn_sched_barrier(0);
         __syncthreads();
         if (on) {
             float ox[EPT], od[EPT], oz[EPT];
 #pragma unroll
             for (int i = 0; i < EPT; ++i) {
                 const float4 s = steps[el.j][el.c + i];
-                ox[i] = fmaf(d[i], s.x, skip[i] * gy[i]);
-                od[i] = fmaf(x[i], s.x, s.y) * slope[i];
+                ox[i] = fmaf(d[i], s.x, skip[i] * s.z);
+                od[i] = fmaf(xk[i], s.x, s.y) * slope[i];
                 if (i < have) gbias[i] += od[i];
-                if (zs) oz[i] = u[i] * fmaf(skip[i], x[i], s.w) * dsilu[i];
+                if (zs) {
+                    const float sg = sigmoid(zk[i]);
+                    oz[i] = uk[i] * fmaf(skip[i], xk[i], s.w) * (sg * fmaf(zk[i], 1.0f - sg, 1.0f));
+                }
             }
             store_row<EPT>(gx + (long)t * p.E, have, wide, ox);
             store_row<EPT>(gd + (long)t * p.E, have, wide, od);
             if (gz) store_row<EPT>(gz + (long)t * p.E, have, wide, oz);
         }
-        float *to = part_bc + (((long)w.n * gridDim.x + w.block) * tiles + tile) * (kSteps * 2 * SP);
-        for (int at = threadIdx.x; at < kSteps * 2 * SP; at += kThreads) {
+        float *to = part_bc + (((long)w.n * gridDim.x + w.block) * tiles + tile) * (STEPS * 2 * SP);
+        for (int at = threadIdx.x; at < STEPS * 2 * SP; at += kThreads) {
             float s = 0.0f;
 #pragma unroll
             for (int v = 0; v < WAVES; ++v) s += sums[v][at / (2 * SP)][at % (2 * SP)];
@@ -602,7 +631,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
         if (w.first + c >= w.end) continue;
         float s = 0.0f, b = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
+        for (int j = 0; j < STEPS; ++j) {
             s += steps[j][c].x;
             b += steps[j][c].y;
         }
@@ -616,11 +645,12 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
 template <typename IO, int LANES>
 __global__ __launch_bounds__(kThreads) void scan_grad_carry_kernel(warpctct_scan_t p, warpctct_scan_grad_t g,
                                                                    Chunks chunks, bool wide) {
-    constexpr int CH = kThreads / LANES, EPT = Elements<LANES>::EPT, SP = Shared<LANES>::SP, PER = Shared<LANES>::PER;
+    constexpr int CH = kThreads / LANES, SP = kStates * LANES, EPT = Elements<LANES, kSteps>::EPT;
+    constexpr int PER = Shared<LANES, kSteps>::PER;
     __shared__ float2 steps[kSteps][CH];           // d, gy
     __shared__ __align__(16) float bc[kSteps][2 * SP];
     const Place w = place_of<LANES>(p, chunks.tiles);
-    const Elements<LANES> el;
+    const Elements<LANES, kSteps> el;
     const int ch = threadIdx.x / LANES, q = threadIdx.x % LANES, e = w.first + ch;
     const bool live = e < w.end;
     float a[kStates], carry[kStates], total = 0.0f;
@@ -643,7 +673,7 @@ __global__ __launch_bounds__(kThreads) void scan_grad_carry_kernel(warpctct_scan
         load_row<EPT>(ds + (long)t * p.dt_t, n, wide, d);
         load_row<EPT>(us + (long)t * g.grad_t, n, wide, u);
         if (zs) load_row<EPT>(zs + (long)t * p.gate_t, n, wide, z);
-        load_bc<LANES, IO>(p, w, t0, side);
+        load_bc<LANES, kSteps, IO>(p, w, t0, side);
     };
     const int last = w.from + (w.to - w.from - 1) / kSteps * kSteps;
     if (w.from < w.to) request(last);
@@ -685,22 +715,22 @@ __global__ __launch_bounds__(kThreads) void scan_grad_carry_kernel(warpctct_scan
 }
 
 // gb, gc (N, L, G, S): the workgroups' partial sums of a group added up, zero
-// behind a sequence.  A thread has one value.
+// behind a sequence.  A thread has one value; `rows` steps a workgroup.
 template <typename IO>
 __global__ __launch_bounds__(kThreads) void scan_grad_bc_kernel(warpctct_scan_t p, warpctct_scan_grad_t g,
                                                                 const float *__restrict__ part_bc, int blocks,
-                                                                int SP) {
+                                                                int SP, int rows) {
     const int n = blockIdx.y, GS = p.G * p.S;
     const long i = (long)blockIdx.x * kThreads + threadIdx.x;
     if (i >= (long)p.L * 2 * GS) return;
     const int t = (int)(i / (2 * GS)), k = (int)(i - (long)t * 2 * GS), v = k % GS, grp = v / p.S, s = v % p.S;
-    const int tiles = (p.L + kSteps - 1) / kSteps;
     const int len = p.lengths ? min(max(p.lengths[n], 0), p.L) : p.L;
     float sum = 0.0f;
     if (t < len) {
-        const float *from = part_bc + (((long)n * blocks * p.G + (long)grp * blocks) * tiles * kSteps + t) * (2 * SP) +
-                            (k < GS ? 0 : SP) + s;
-        for (int b = 0; b < blocks; ++b) sum += from[(long)b * tiles * kSteps * 2 * SP];
+        const float *from =
+            part_bc + (((long)n * p.G + grp) * blocks * rows + t) * (2 * SP) + (k < GS ? 0 : SP) + s;
+#pragma unroll 4
+        for (int b = 0; b < blocks; ++b) sum += from[(long)b * rows * 2 * SP];
     }
     IO *to = static_cast<IO *>(k < GS ? g.grad_b : g.grad_c);
     to[((long)n * p.L + t) * GS + v] = from_float<IO>(sum);
@@ -755,6 +785,12 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(warpctct_scan_step_
         y *= z * sigmoid(z);
     }
     *out = from_float<IO>(y);
+}
+
+// steps, rounded up to whole tiles of the backward pass
+int back_rows(int L, int lanes) {
+    const int steps = back_steps(lanes);
+    return (L + steps - 1) / steps * steps;
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -859,7 +895,7 @@ hipError_t start(const warpctct_scan_t &p, const warpctct_scan_grad_t &g, const 
     auto join = scan_grad_bc_kernel<IO>;
     const long values = (long)p.L * 2 * p.G * p.S;
     TIMED_LAUNCH(join, dim3((unsigned)((values + kThreads - 1) / kThreads), p.N), dim3(kThreads), 0, stream, p, g,
-                 part_bc, blocks, Shared<LANES>::SP);
+                 part_bc, blocks, kStates * LANES, back_rows(p.L, LANES));
     return hipGetLastError();
 }
 
@@ -890,14 +926,15 @@ hipError_t by_type(int dtype, int S, const Args &...args) {
 }
 
 size_t part_bc_floats(const warpctct_scan_t &p) {
-    const size_t tiles = (p.L + kSteps - 1) / kSteps, SP = kStates * lanes_of(p.S);
-    return (size_t)p.N * p.G * blocks_of(p) * tiles * kSteps * 2 * SP;
+    const int lanes = lanes_of(p.S);
+    return (size_t)p.N * p.G * blocks_of(p) * back_rows(p.L, lanes) * 2 * kStates * lanes;
 }
 
 }  // namespace
 
 size_t scan_keep_floats(int N, int L, int E, int S) {
-    return (size_t)N * ((L + kSteps - 1) / kSteps) * E * (kStates * lanes_of(S));
+    const int lanes = lanes_of(S);
+    return (size_t)N * (back_rows(L, lanes) / back_steps(lanes)) * E * (kStates * lanes);
 }
 
 size_t scan_floats(const warpctct_scan_t &p) { return chunk_floats(p); }

@@ -130,8 +130,8 @@ def selective_scan(x: torch.Tensor,
 
     Returns out (N, T, E), or ``(out, state)``.  Differentiable with respect to
     everything but ``lengths``, through both results; every sum is added up in a
-    fixed order.  Where a gradient is tracked, the states in front of every 16
-    steps are kept for it: T/16 * N * E * S floats."""
+    fixed order.  Where a gradient is tracked, the states in front of every 8
+    steps are kept for it: T/8 * N * E * S floats for 16 states."""
     got = core.selective_scan(x, dt, a, b, c, skip, gate, dt_bias, bool(softplus), lengths, initial_state,
                               bool(return_state))
     return (got[0], got[1]) if return_state else got[0]
