@@ -52,25 +52,23 @@ constexpr int back_steps(int lanes) { return lanes == 1 ? 4 : lanes == 16 ? 16 :
 __device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
 
 // log(1 + e^v) and its derivative.  log1p(q), q = e^-|v| in [0, 1], is
-// 2 atanh(q / (2 + q)), whose argument is at most 1/3: eight terms of the
-// series leave a relative error of 3e-9, where log2(1 + q) on the transcendental
-// unit would lose q itself to the rounding of the sum.
+// 2 atanh(q / (2 + q)), whose argument r is at most 1/3.  atanh(r) / r as a
+// polynomial of degree 4 in r^2, its coefficients found by Remez exchange for the
+// least relative error over [0, 1/9], is off by 4e-9; log2(1 + q) on the
+// transcendental unit would lose q itself to the rounding of the sum.
 struct Softplus {
     float value, slope;
 };
 __device__ __forceinline__ Softplus softplus(float v) {
     const float q = exp2_hw(-kLog2e * fabsf(v));
     const float r = q * __builtin_amdgcn_rcpf(2.0f + q), r2 = r * r;
-    float s = 1.0f / 15.0f;
-    s = fmaf(s, r2, 1.0f / 13.0f);
-    s = fmaf(s, r2, 1.0f / 11.0f);
-    s = fmaf(s, r2, 1.0f / 9.0f);
-    s = fmaf(s, r2, 1.0f / 7.0f);
-    s = fmaf(s, r2, 1.0f / 5.0f);
-    s = fmaf(s, r2, 1.0f / 3.0f);
+    float s = 0.140891984f;
+    s = fmaf(s, r2, 0.139802948f);
+    s = fmaf(s, r2, 0.200124562f);
+    s = fmaf(s, r2, 0.333331585f);
     s = fmaf(s, r2, 1.0f);
     Softplus p;
-    p.value = fmaxf(v, 0.0f) + 2.0f * r * s;
+    p.value = fmaf(2.0f * r, s, fmaxf(v, 0.0f));
     if (v != v) p.value = v;
     const float inv = __builtin_amdgcn_rcpf(1.0f + q);
     p.slope = v >= 0.0f ? inv : q * inv;
@@ -167,27 +165,38 @@ __device__ __forceinline__ void store_row(IO *p, int have, bool wide, const floa
     }
 }
 
-// The tile's rows of b and c, STEPS x 2 SP values, by all threads.
-template <int LANES, int STEPS>
-struct Shared {
-    static constexpr int SP = kStates * LANES;
-    static constexpr int PER = (2 * STEPS * SP + kThreads - 1) / kThreads;
-};
-template <int LANES, int STEPS, typename IO>
-__device__ __forceinline__ void load_bc(const warpctct_scan_t &p, const Place &w, int t0,
-                                        float (&v)[Shared<LANES, STEPS>::PER]) {
-    constexpr int SP = Shared<LANES, STEPS>::SP;
-    const IO *b = static_cast<const IO *>(p.b) + (long)w.n * p.b_n + (long)w.g * p.b_g;
-    const IO *c = static_cast<const IO *>(p.c) + (long)w.n * p.c_n + (long)w.g * p.c_g;
-#pragma unroll
-    for (int i = 0; i < Shared<LANES, STEPS>::PER; ++i) {
-        const int at = i * kThreads + threadIdx.x, j = at / (2 * SP), k = at % (2 * SP);
-        const int s = k % SP, t = t0 + j;
-        v[i] = 0.0f;
-        if (j < STEPS && t < w.len && s < p.S)
-            v[i] = to_float(k < SP ? b[(long)t * p.b_t + s] : c[(long)t * p.c_t + s]);
+// The tile's rows of b and c, STEPS x 2 SP values, by all threads: a thread has
+// one column of b or of c, and of every kRows steps one.
+template <typename IO, int LANES, int STEPS>
+struct Sides {
+    static constexpr int SP = kStates * LANES, kRows = kThreads / (2 * SP);
+    static constexpr int PER = STEPS > kRows ? STEPS / kRows : 1;
+    const IO *at;
+    long stride;
+    int j, k;
+    bool in;
+    __device__ __forceinline__ Sides(const warpctct_scan_t &p, const Place &w, int t0) {
+        j = threadIdx.x / (2 * SP);
+        k = threadIdx.x % (2 * SP);
+        const int s = k % SP;
+        in = s < p.S && j < STEPS;
+        const IO *base = k < SP ? static_cast<const IO *>(p.b) + (long)w.n * p.b_n + (long)w.g * p.b_g
+                                : static_cast<const IO *>(p.c) + (long)w.n * p.c_n + (long)w.g * p.c_g;
+        stride = k < SP ? p.b_t : p.c_t;
+        at = base + (long)(t0 + j) * stride + s;
     }
-}
+    __device__ __forceinline__ void load(int t0, int len, float (&v)[PER]) const {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            v[i] = in && t0 + j + i * kRows < len ? to_float(at[i * kRows * stride]) : 0.0f;
+    }
+    __device__ __forceinline__ void put(float (*bc)[2 * SP], const float (&v)[PER]) const {
+        if (kRows > STEPS && j >= STEPS) return;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) bc[j + i * kRows][k] = v[i];
+    }
+    __device__ __forceinline__ void advance(int steps) { at += steps * stride; }
+};
 
 // Four steps of a tile as a lane takes them out of LDS.
 struct Four {
@@ -253,7 +262,6 @@ template <typename IO, int LANES, bool CARRY>
 __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float *__restrict__ keep, Chunks chunks,
                                                         const float *__restrict__ starts, bool wide) {
     constexpr int CH = kThreads / LANES, SP = kStates * LANES, EPT = Elements<LANES, kSteps>::EPT;
-    constexpr int PER = Shared<LANES, kSteps>::PER;
     __shared__ float2 steps[kSteps][CH];           // d, d x
     __shared__ __align__(16) float bc[kSteps][2 * SP];
     __shared__ float ys[kSteps][CARRY ? 1 : CH];
@@ -284,18 +292,27 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
         skip[i] = !CARRY && p.skip && i < have ? p.skip[e0 + i] : 0.0f;
         bias[i] = p.dt_bias && i < have ? p.dt_bias[e0 + i] : 0.0f;
     }
-    const IO *xs = static_cast<const IO *>(p.x) + (long)w.n * p.x_n + e0;
-    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + e0;
-    const IO *zs = !CARRY && p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + e0 : nullptr;
-    IO *out = static_cast<IO *>(p.out) + (long)w.n * p.L * p.E + e0;
+    // rows of the tile that is asked for next, and of the one that is written next
+    const int t1 = w.from + el.j;
+    const bool gated = !CARRY && p.gate;
+    const IO *xs = static_cast<const IO *>(p.x) + (long)w.n * p.x_n + t1 * p.x_t + e0;
+    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + t1 * p.dt_t + e0;
+    const IO *zs = gated ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + t1 * p.gate_t + e0 : nullptr;
+    IO *out = static_cast<IO *>(p.out) + ((long)w.n * p.L + t1) * p.E + e0;
+    typedef Sides<IO, LANES, kSteps> Side;
+    Side sides(p, w, w.from);
 
-    float x[EPT], d[EPT], z[EPT], side[PER];
+    float x[EPT], d[EPT], z[EPT], side[Side::PER];
     auto request = [&](int t0) {
-        const int t = t0 + el.j, n = t < w.to ? have : 0;
-        load_row<EPT>(xs + (long)t * p.x_t, n, wide, x);
-        load_row<EPT>(ds + (long)t * p.dt_t, n, wide, d);
-        if (zs) load_row<EPT>(zs + (long)t * p.gate_t, n, wide, z);
-        load_bc<LANES, kSteps, IO>(p, w, t0, side);
+        const int n = t0 + el.j < w.to ? have : 0;
+        load_row<EPT>(xs, n, wide, x);
+        load_row<EPT>(ds, n, wide, d);
+        if (gated) load_row<EPT>(zs, n, wide, z);
+        sides.load(t0, w.len, side);
+        xs += kSteps * p.x_t;
+        ds += kSteps * p.dt_t;
+        if (gated) zs += kSteps * p.gate_t;
+        sides.advance(kSteps);
     };
     if (w.from < w.to) request(w.from);
     for (int t0 = w.from; t0 < w.to; t0 += kSteps) {
@@ -310,11 +327,7 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
             xk[i] = x[i];
             zk[i] = z[i];
         }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int at = i * kThreads + threadIdx.x;
-            if (at < 2 * kSteps * SP) bc[at / (2 * SP)][at % (2 * SP)] = side[i];
-        }
+        sides.put(bc, side);
         __syncthreads();
         if (t0 + kSteps < w.to) request(t0 + kSteps);
         Four f[2];
@@ -354,10 +367,11 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
 #pragma unroll
             for (int i = 0; i < EPT; ++i) {
                 o[i] = fmaf(skip[i], xk[i], ys[el.j][el.c + i]);
-                if (zs) o[i] *= zk[i] * sigmoid(zk[i]);
+                if (gated) o[i] *= zk[i] * sigmoid(zk[i]);
             }
-            store_row<EPT>(out + (long)(t0 + el.j) * p.E, have, wide, o);
+            store_row<EPT>(out, have, wide, o);
         }
+        out += (long)kSteps * p.E;
     }
     if (CARRY) {
         if (live) {
@@ -370,6 +384,7 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
     if (blockIdx.z + 1 != gridDim.z) return;
     // the steps that do not count
     const float zero[EPT] = {};
+    out = static_cast<IO *>(p.out) + (long)w.n * p.L * p.E + e0;
     for (int t = w.len + el.j; t < p.L; t += kSteps) store_row<EPT>(out + (long)t * p.E, have, wide, zero);
     if (p.last && live) {
 #pragma unroll
@@ -426,7 +441,6 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
                                                                 const float *__restrict__ starts, bool wide) {
     constexpr int STEPS = back_steps(LANES);
     constexpr int CH = kThreads / LANES, SP = kStates * LANES, EPT = Elements<LANES, STEPS>::EPT;
-    constexpr int PER = Shared<LANES, STEPS>::PER;
     constexpr int WAVES = kThreads / 64;
     // d, d x, gy, and y without the skip; on the way back the first two give way
     // to sum gh b and sum a gh k h (a channel's lanes lie in one wavefront, which
@@ -461,10 +475,6 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
         bias[i] = p.dt_bias && i < have ? p.dt_bias[e0 + i] : 0.0f;
         gskip[i] = gbias[i] = 0.0f;
     }
-    const IO *xs = static_cast<const IO *>(p.x) + (long)w.n * p.x_n + e0;
-    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + e0;
-    const IO *zs = p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + e0 : nullptr;
-    const IO *us = static_cast<const IO *>(g.grad_out) + (long)w.n * g.grad_n + e0;
     const long rows = (long)w.n * p.L * p.E + e0;
     IO *gx = static_cast<IO *>(g.grad_x) + rows, *gd = static_cast<IO *>(g.grad_dt) + rows;
     IO *gz = p.gate ? static_cast<IO *>(g.grad_gate) + rows : nullptr;
@@ -477,23 +487,36 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     }
     // the rows of a tile and the states in front of it are asked for while the
     // tile behind it is worked on
-    float x[EPT], raw[EPT], z[EPT], u[EPT], side[PER];
+    const int top = (w.to + STEPS - 1) / STEPS - 1, bottom = w.from < w.to ? w.from / STEPS : top + 1;
+    const long t1 = (long)top * STEPS + el.j;
+    const IO *xs = static_cast<const IO *>(p.x) + (long)w.n * p.x_n + t1 * p.x_t + e0;
+    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + t1 * p.dt_t + e0;
+    const IO *zs = p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + t1 * p.gate_t + e0 : nullptr;
+    const IO *us = static_cast<const IO *>(g.grad_out) + (long)w.n * g.grad_n + t1 * g.grad_t + e0;
+    const float *fronts = keep + (((long)w.n * tiles + top) * p.E + e) * SP + q * kStates;
+    long row = t1 * p.E;         // of the tile that is written next
+    typedef Sides<IO, LANES, STEPS> Side;
+    Side sides(p, w, top * STEPS);
+    float x[EPT], raw[EPT], z[EPT], u[EPT], side[Side::PER];
     float4 front = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     auto request = [&](int tile) {
-        const int t = tile * STEPS + el.j, n = t < w.to ? have : 0;
-        load_row<EPT>(xs + (long)t * p.x_t, n, wide, x);
-        load_row<EPT>(ds + (long)t * p.dt_t, n, wide, raw);
-        load_row<EPT>(us + (long)t * g.grad_t, n, wide, u);
-        if (zs) load_row<EPT>(zs + (long)t * p.gate_t, n, wide, z);
-        load_bc<LANES, STEPS, IO>(p, w, tile * STEPS, side);
-        if (live)
-            front = *reinterpret_cast<const float4 *>(keep + (((long)w.n * tiles + tile) * p.E + e) * SP + q * kStates);
+        const int n = tile * STEPS + el.j < w.to ? have : 0;
+        load_row<EPT>(xs, n, wide, x);
+        load_row<EPT>(ds, n, wide, raw);
+        load_row<EPT>(us, n, wide, u);
+        if (zs) load_row<EPT>(zs, n, wide, z);
+        sides.load(tile * STEPS, w.len, side);
+        if (live) front = *reinterpret_cast<const float4 *>(fronts);
+        xs -= STEPS * p.x_t;
+        ds -= STEPS * p.dt_t;
+        us -= STEPS * g.grad_t;
+        if (zs) zs -= STEPS * p.gate_t;
+        fronts -= (long)p.E * SP;
+        sides.advance(-STEPS);
     };
-    const int top = (w.to + STEPS - 1) / STEPS - 1, bottom = w.from < w.to ? w.from / STEPS : top + 1;
     if (top >= bottom) request(top);
     for (int tile = top; tile >= bottom; --tile) {
-        const int t = tile * STEPS + el.j;
-        const bool on = t < w.to;
+        const bool on = tile * STEPS + el.j < w.to;
         float xk[EPT], d[EPT], slope[EPT], uk[EPT], zk[EPT];
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
@@ -514,11 +537,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
             uk[i] = u[i];
             zk[i] = z[i];
         }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int at = i * kThreads + threadIdx.x;
-            if (at < 2 * STEPS * SP) bc[at / (2 * SP)][at % (2 * SP)] = side[i];
-        }
+        sides.put(bc, side);
         const float h0[kStates] = {front.x, front.y, front.z, front.w};
         __syncthreads();
         if (tile > bottom) request(tile - 1);
@@ -599,10 +618,11 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
                     oz[i] = uk[i] * fmaf(skip[i], xk[i], s.w) * (sg * fmaf(zk[i], 1.0f - sg, 1.0f));
                 }
             }
-            store_row<EPT>(gx + (long)t * p.E, have, wide, ox);
-            store_row<EPT>(gd + (long)t * p.E, have, wide, od);
-            if (gz) store_row<EPT>(gz + (long)t * p.E, have, wide, oz);
+            store_row<EPT>(gx + row, have, wide, ox);
+            store_row<EPT>(gd + row, have, wide, od);
+            if (gz) store_row<EPT>(gz + row, have, wide, oz);
         }
+        row -= (long)STEPS * p.E;
         float *to = part_bc + (((long)w.n * gridDim.x + w.block) * tiles + tile) * (STEPS * 2 * SP);
         for (int at = threadIdx.x; at < STEPS * 2 * SP; at += kThreads) {
             float s = 0.0f;
@@ -646,7 +666,6 @@ template <typename IO, int LANES>
 __global__ __launch_bounds__(kThreads) void scan_grad_carry_kernel(warpctct_scan_t p, warpctct_scan_grad_t g,
                                                                    Chunks chunks, bool wide) {
     constexpr int CH = kThreads / LANES, SP = kStates * LANES, EPT = Elements<LANES, kSteps>::EPT;
-    constexpr int PER = Shared<LANES, kSteps>::PER;
     __shared__ float2 steps[kSteps][CH];           // d, gy
     __shared__ __align__(16) float bc[kSteps][2 * SP];
     const Place w = place_of<LANES>(p, chunks.tiles);
@@ -664,18 +683,25 @@ __global__ __launch_bounds__(kThreads) void scan_grad_carry_kernel(warpctct_scan
     float bias[EPT];
 #pragma unroll
     for (int i = 0; i < EPT; ++i) bias[i] = p.dt_bias && i < have ? p.dt_bias[e0 + i] : 0.0f;
-    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + e0;
-    const IO *zs = p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + e0 : nullptr;
-    const IO *us = static_cast<const IO *>(g.grad_out) + (long)w.n * g.grad_n + e0;
-    float d[EPT], u[EPT], z[EPT], side[PER];
-    auto request = [&](int t0) {
-        const int t = t0 + el.j, n = t < w.to ? have : 0;
-        load_row<EPT>(ds + (long)t * p.dt_t, n, wide, d);
-        load_row<EPT>(us + (long)t * g.grad_t, n, wide, u);
-        if (zs) load_row<EPT>(zs + (long)t * p.gate_t, n, wide, z);
-        load_bc<LANES, kSteps, IO>(p, w, t0, side);
-    };
     const int last = w.from + (w.to - w.from - 1) / kSteps * kSteps;
+    const long t1 = last + el.j;
+    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + t1 * p.dt_t + e0;
+    const IO *zs = p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + t1 * p.gate_t + e0 : nullptr;
+    const IO *us = static_cast<const IO *>(g.grad_out) + (long)w.n * g.grad_n + t1 * g.grad_t + e0;
+    typedef Sides<IO, LANES, kSteps> Side;
+    Side sides(p, w, last);
+    float d[EPT], u[EPT], z[EPT], side[Side::PER];
+    auto request = [&](int t0) {
+        const int n = t0 + el.j < w.to ? have : 0;
+        load_row<EPT>(ds, n, wide, d);
+        load_row<EPT>(us, n, wide, u);
+        if (zs) load_row<EPT>(zs, n, wide, z);
+        sides.load(t0, w.len, side);
+        ds -= kSteps * p.dt_t;
+        us -= kSteps * g.grad_t;
+        if (zs) zs -= kSteps * p.gate_t;
+        sides.advance(-kSteps);
+    };
     if (w.from < w.to) request(last);
     for (int t0 = w.from < w.to ? last : -1; t0 >= w.from; t0 -= kSteps) {
         const bool on = t0 + el.j < w.to;
@@ -689,11 +715,7 @@ __global__ __launch_bounds__(kThreads) void scan_grad_carry_kernel(warpctct_scan
             if (!(on && i < have)) y = 0.0f;
             steps[el.j][el.c + i] = make_float2(v, y);
         }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int at = i * kThreads + threadIdx.x;
-            if (at < 2 * kSteps * SP) bc[at / (2 * SP)][at % (2 * SP)] = side[i];
-        }
+        sides.put(bc, side);
         __syncthreads();
         if (t0 - kSteps >= w.from) request(t0 - kSteps);
 #pragma unroll
