@@ -100,6 +100,33 @@ __device__ __forceinline__ void store_n(IO *p, const float *x) {
     }
 }
 
+// N elements next to each other as they are loaded, not yet converted: a
+// conversion waits for its load, so loads that are to be in flight together, or
+// while something else is worked on, are kept in this form.  `wide`: the start is
+// aligned for pieces of up to 16 bytes; otherwise element i is p[min(i, most)].
+template <typename IO, int N>
+struct Raw {
+    static constexpr int kPiece = N * (int)sizeof(IO) > 16 ? kVec<IO> : N;
+    typedef IO piece __attribute__((ext_vector_type(kPiece)));
+    piece v[N / kPiece];
+    __device__ __forceinline__ void load(const IO *p, bool wide, int most) {
+        if (wide) {
+#pragma unroll
+            for (int k = 0; k < N / kPiece; ++k) v[k] = *reinterpret_cast<const piece *>(p + k * kPiece);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i / kPiece][i % kPiece] = p[min(i, most)];
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const { return (float)v[i / kPiece][i % kPiece]; }
+};
+template <typename IO>
+struct Raw<IO, 1> {
+    IO v;
+    __device__ __forceinline__ void load(const IO *p, bool, int) { v = *p; }
+    __device__ __forceinline__ float operator[](int) const { return (float)v; }
+};
+
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
     return __uint_as_float(

@@ -140,18 +140,7 @@ struct Elements {
 };
 
 // N elements of a row, in the widest pieces where `wide`; those at or past `have`
-// read as zero and are not written.
-template <int N, typename IO>
-__device__ __forceinline__ void load_row(const IO *p, int have, bool wide, float (&v)[N]) {
-    constexpr int piece = N < 4 ? 1 : (N < kVec<IO> ? 4 : kVec<IO>);
-    if (wide && have >= N) {
-#pragma unroll
-        for (int i = 0; i < N; i += piece) load_n<piece>(p + i, v + i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = i < have ? to_float(p[i]) : 0.0f;
-    }
-}
+// are not written.
 template <int N, typename IO>
 __device__ __forceinline__ void store_row(IO *p, int have, bool wide, const float (&v)[N]) {
     constexpr int piece = N < 4 ? 1 : (N < kVec<IO> ? 4 : kVec<IO>);
@@ -166,36 +155,61 @@ __device__ __forceinline__ void store_row(IO *p, int have, bool wide, const floa
 }
 
 // The tile's rows of b and c, STEPS x 2 SP values, by all threads: a thread has
-// one column of b or of c, and of every kRows steps one.
+// one column of b or of c, and of every kRows steps one.  Where there is nothing
+// to read (behind the sequence, past the states) it reads row `safe` of its
+// column, or the last state, and puts zero.
 template <typename IO, int LANES, int STEPS>
 struct Sides {
     static constexpr int SP = kStates * LANES, kRows = kThreads / (2 * SP);
     static constexpr int PER = STEPS > kRows ? STEPS / kRows : 1;
-    const IO *at;
+    const IO *at, *safe;
     long stride;
     int j, k;
     bool in;
-    __device__ __forceinline__ Sides(const warpctct_scan_t &p, const Place &w, int t0) {
+    IO v[PER];
+    __device__ __forceinline__ Sides(const warpctct_scan_t &p, const Place &w, int t0, int safe_row) {
         j = threadIdx.x / (2 * SP);
         k = threadIdx.x % (2 * SP);
-        const int s = k % SP;
-        in = s < p.S && j < STEPS;
-        const IO *base = k < SP ? static_cast<const IO *>(p.b) + (long)w.n * p.b_n + (long)w.g * p.b_g
-                                : static_cast<const IO *>(p.c) + (long)w.n * p.c_n + (long)w.g * p.c_g;
+        const int s = min(k % SP, p.S - 1);
+        in = k % SP < p.S && j < STEPS;
+        const IO *base = (k < SP ? static_cast<const IO *>(p.b) + (long)w.n * p.b_n + (long)w.g * p.b_g
+                                 : static_cast<const IO *>(p.c) + (long)w.n * p.c_n + (long)w.g * p.c_g) + s;
         stride = k < SP ? p.b_t : p.c_t;
-        at = base + (long)(t0 + j) * stride + s;
+        at = base + (long)(t0 + j) * stride;
+        safe = base + safe_row * stride;
     }
-    __device__ __forceinline__ void load(int t0, int len, float (&v)[PER]) const {
+    __device__ __forceinline__ void load(int t0, int len) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-            v[i] = in && t0 + j + i * kRows < len ? to_float(at[i * kRows * stride]) : 0.0f;
+        for (int i = 0; i < PER; ++i) v[i] = *(t0 + j + i * kRows < len ? at + i * kRows * stride : safe);
     }
-    __device__ __forceinline__ void put(float (*bc)[2 * SP], const float (&v)[PER]) const {
+    // of the tile at t0, which load() was asked for
+    __device__ __forceinline__ void put(float (*bc)[2 * SP], int t0, int len) const {
         if (kRows > STEPS && j >= STEPS) return;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) bc[j + i * kRows][k] = v[i];
+        for (int i = 0; i < PER; ++i)
+            bc[j + i * kRows][k] = in && t0 + j + i * kRows < len ? to_float(v[i]) : 0.0f;
     }
     __device__ __forceinline__ void advance(int steps) { at += steps * stride; }
+};
+
+// A thread's elements of x, dt, gate or grad_out, tile after tile.  Where it has
+// none it reads row `safe`, or the workgroup's first channels, and masks what it
+// makes of them.
+template <typename IO, int EPT>
+struct Column {
+    const IO *at, *safe;
+    long stride;
+    __device__ __forceinline__ Column(const void *base, long start, long t_stride, long row, int safe_row) {
+        const IO *p = static_cast<const IO *>(base) + start;
+        stride = t_stride;
+        at = p + row * stride;
+        safe = p + safe_row * stride;
+    }
+    // the present row, and on by `steps`
+    __device__ __forceinline__ void next(Raw<IO, EPT> &v, bool on, bool wide, int most, int steps) {
+        v.load(on ? at : safe, wide, most);
+        at += steps * stride;
+    }
 };
 
 // Four steps of a tile as a lane takes them out of LDS.
@@ -292,42 +306,37 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
         skip[i] = !CARRY && p.skip && i < have ? p.skip[e0 + i] : 0.0f;
         bias[i] = p.dt_bias && i < have ? p.dt_bias[e0 + i] : 0.0f;
     }
-    // rows of the tile that is asked for next, and of the one that is written next
-    const int t1 = w.from + el.j;
+    const int el0 = have > 0 ? e0 : w.first, most = max(have - 1, 0), t1 = w.from + el.j;
     const bool gated = !CARRY && p.gate;
-    const IO *xs = static_cast<const IO *>(p.x) + (long)w.n * p.x_n + t1 * p.x_t + e0;
-    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + t1 * p.dt_t + e0;
-    const IO *zs = gated ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + t1 * p.gate_t + e0 : nullptr;
+    typedef Raw<IO, EPT> Row;
+    Column<IO, EPT> xs(p.x, (long)w.n * p.x_n + el0, p.x_t, t1, w.from);
+    Column<IO, EPT> ds(p.dt, (long)w.n * p.dt_n + el0, p.dt_t, t1, w.from);
+    Column<IO, EPT> zs(p.gate, (long)w.n * p.gate_n + el0, p.gate_t, t1, w.from);
     IO *out = static_cast<IO *>(p.out) + ((long)w.n * p.L + t1) * p.E + e0;
     typedef Sides<IO, LANES, kSteps> Side;
-    Side sides(p, w, w.from);
-
-    float x[EPT], d[EPT], z[EPT], side[Side::PER];
+    Side sides(p, w, w.from, w.from);
+    Row x, d, z;
     auto request = [&](int t0) {
-        const int n = t0 + el.j < w.to ? have : 0;
-        load_row<EPT>(xs, n, wide, x);
-        load_row<EPT>(ds, n, wide, d);
-        if (gated) load_row<EPT>(zs, n, wide, z);
-        sides.load(t0, w.len, side);
-        xs += kSteps * p.x_t;
-        ds += kSteps * p.dt_t;
-        if (gated) zs += kSteps * p.gate_t;
+        const bool on = t0 + el.j < w.to;
+        xs.next(x, on, wide, most, kSteps);
+        ds.next(d, on, wide, most, kSteps);
+        if (gated) zs.next(z, on, wide, most, kSteps);
+        sides.load(t0, w.len);
         sides.advance(kSteps);
     };
     if (w.from < w.to) request(w.from);
     for (int t0 = w.from; t0 < w.to; t0 += kSteps) {
         const bool on = t0 + el.j < w.to;
-        float xk[EPT], zk[EPT];
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
             float v = d[i] + bias[i];
             if (p.softplus) v = softplus(v).value;
-            if (!(on && i < have)) v = 0.0f;       // a step that leaves the state as it is
-            steps[el.j][el.c + i] = make_float2(v, v * x[i]);
-            xk[i] = x[i];
-            zk[i] = z[i];
+            const bool in = on && i < have;         // otherwise a step that leaves the state as it is
+            v = in ? v : 0.0f;
+            steps[el.j][el.c + i] = make_float2(v, in ? v * x[i] : 0.0f);
         }
-        sides.put(bc, side);
+        const Row xk = x, zk = z;
+        sides.put(bc, t0, w.len);
         __syncthreads();
         if (t0 + kSteps < w.to) request(t0 + kSteps);
         Four f[2];
@@ -489,35 +498,34 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     // tile behind it is worked on
     const int top = (w.to + STEPS - 1) / STEPS - 1, bottom = w.from < w.to ? w.from / STEPS : top + 1;
     const long t1 = (long)top * STEPS + el.j;
-    const IO *xs = static_cast<const IO *>(p.x) + (long)w.n * p.x_n + t1 * p.x_t + e0;
-    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + t1 * p.dt_t + e0;
-    const IO *zs = p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + t1 * p.gate_t + e0 : nullptr;
-    const IO *us = static_cast<const IO *>(g.grad_out) + (long)w.n * g.grad_n + t1 * g.grad_t + e0;
-    const float *fronts = keep + (((long)w.n * tiles + top) * p.E + e) * SP + q * kStates;
+    const int el0 = have > 0 ? e0 : w.first, most = max(have - 1, 0);
+    const bool gated = p.gate;
+    typedef Raw<IO, EPT> Row;
+    Column<IO, EPT> xs(p.x, (long)w.n * p.x_n + el0, p.x_t, t1, w.from);
+    Column<IO, EPT> ds(p.dt, (long)w.n * p.dt_n + el0, p.dt_t, t1, w.from);
+    Column<IO, EPT> zs(p.gate, (long)w.n * p.gate_n + el0, p.gate_t, t1, w.from);
+    Column<IO, EPT> us(g.grad_out, (long)w.n * g.grad_n + el0, g.grad_t, t1, w.from);
+    const float *fronts = keep + (((long)w.n * tiles + top) * p.E + (live ? e : w.first)) * SP + q * kStates;
     long row = t1 * p.E;         // of the tile that is written next
     typedef Sides<IO, LANES, STEPS> Side;
-    Side sides(p, w, top * STEPS);
-    float x[EPT], raw[EPT], z[EPT], u[EPT], side[Side::PER];
-    float4 front = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    Side sides(p, w, top * STEPS, w.from);
+    Row x, raw, z, u;
+    float4 front;
     auto request = [&](int tile) {
-        const int n = tile * STEPS + el.j < w.to ? have : 0;
-        load_row<EPT>(xs, n, wide, x);
-        load_row<EPT>(ds, n, wide, raw);
-        load_row<EPT>(us, n, wide, u);
-        if (zs) load_row<EPT>(zs, n, wide, z);
-        sides.load(tile * STEPS, w.len, side);
-        if (live) front = *reinterpret_cast<const float4 *>(fronts);
-        xs -= STEPS * p.x_t;
-        ds -= STEPS * p.dt_t;
-        us -= STEPS * g.grad_t;
-        if (zs) zs -= STEPS * p.gate_t;
+        const bool on = tile * STEPS + el.j < w.to;
+        xs.next(x, on, wide, most, -STEPS);
+        ds.next(raw, on, wide, most, -STEPS);
+        us.next(u, on, wide, most, -STEPS);
+        if (gated) zs.next(z, on, wide, most, -STEPS);
+        sides.load(tile * STEPS, w.len);
+        front = *reinterpret_cast<const float4 *>(fronts);
         fronts -= (long)p.E * SP;
         sides.advance(-STEPS);
     };
     if (top >= bottom) request(top);
     for (int tile = top; tile >= bottom; --tile) {
         const bool on = tile * STEPS + el.j < w.to;
-        float xk[EPT], d[EPT], slope[EPT], uk[EPT], zk[EPT];
+        float d[EPT], slope[EPT];
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
             const float v = raw[i] + bias[i];
@@ -528,17 +536,16 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
                 d[i] = s.value;
                 slope[i] = s.slope;
             }
-            float gy = u[i];
-            if (zs) gy *= z[i] * sigmoid(z[i]);
-            if (!(on && i < have)) d[i] = gy = 0.0f;
-            steps[el.j][el.c + i] = make_float4(d[i], d[i] * x[i], gy, 0.0f);
-            gskip[i] = fmaf(gy, x[i], gskip[i]);
-            xk[i] = x[i];
-            uk[i] = u[i];
-            zk[i] = z[i];
+            float gy = u[i], xi = x[i];
+            if (gated) gy *= z[i] * sigmoid(z[i]);
+            if (!(on && i < have)) d[i] = gy = xi = 0.0f;
+            steps[el.j][el.c + i] = make_float4(d[i], d[i] * xi, gy, 0.0f);
+            gskip[i] = fmaf(gy, xi, gskip[i]);
         }
-        sides.put(bc, side);
-        const float h0[kStates] = {front.x, front.y, front.z, front.w};
+        const Row xk = x, uk = u, zk = z;
+        sides.put(bc, tile * STEPS, w.len);
+        const float h0[kStates] = {live ? front.x : 0.0f, live ? front.y : 0.0f, live ? front.z : 0.0f,
+                                   live ? front.w : 0.0f};
         __syncthreads();
         if (tile > bottom) request(tile - 1);
         float k[STEPS][kStates], h[STEPS][kStates];
@@ -559,7 +566,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
                 const float4 c4 = *reinterpret_cast<const float4 *>(&bc[j][SP + q * kStates]);
                 y[j - j0] = fmaf(c4.w, h[j][3], fmaf(c4.z, h[j][2], fmaf(c4.y, h[j][1], c4.x * h[j][0])));
             }
-            if (zs) {
+            if (gated) {
                 float r[StepSums<LANES>::kept];
                 StepSums<LANES>::add(y, q, r);
 #pragma unroll
@@ -613,7 +620,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
                 ox[i] = fmaf(d[i], s.x, skip[i] * s.z);
                 od[i] = fmaf(xk[i], s.x, s.y) * slope[i];
                 if (i < have) gbias[i] += od[i];
-                if (zs) {
+                if (gated) {
                     const float sg = sigmoid(zk[i]);
                     oz[i] = uk[i] * fmaf(skip[i], xk[i], s.w) * (sg * fmaf(zk[i], 1.0f - sg, 1.0f));
                 }
@@ -685,21 +692,20 @@ __global__ __launch_bounds__(kThreads) void scan_grad_carry_kernel(warpctct_scan
     for (int i = 0; i < EPT; ++i) bias[i] = p.dt_bias && i < have ? p.dt_bias[e0 + i] : 0.0f;
     const int last = w.from + (w.to - w.from - 1) / kSteps * kSteps;
     const long t1 = last + el.j;
-    const IO *ds = static_cast<const IO *>(p.dt) + (long)w.n * p.dt_n + t1 * p.dt_t + e0;
-    const IO *zs = p.gate ? static_cast<const IO *>(p.gate) + (long)w.n * p.gate_n + t1 * p.gate_t + e0 : nullptr;
-    const IO *us = static_cast<const IO *>(g.grad_out) + (long)w.n * g.grad_n + t1 * g.grad_t + e0;
+    const int el0 = have > 0 ? e0 : w.first, most = max(have - 1, 0);
+    const bool gated = p.gate;
+    Column<IO, EPT> ds(p.dt, (long)w.n * p.dt_n + el0, p.dt_t, t1, w.from);
+    Column<IO, EPT> zs(p.gate, (long)w.n * p.gate_n + el0, p.gate_t, t1, w.from);
+    Column<IO, EPT> us(g.grad_out, (long)w.n * g.grad_n + el0, g.grad_t, t1, w.from);
     typedef Sides<IO, LANES, kSteps> Side;
-    Side sides(p, w, last);
-    float d[EPT], u[EPT], z[EPT], side[Side::PER];
+    Side sides(p, w, last, w.from);
+    Raw<IO, EPT> d, u, z;
     auto request = [&](int t0) {
-        const int n = t0 + el.j < w.to ? have : 0;
-        load_row<EPT>(ds, n, wide, d);
-        load_row<EPT>(us, n, wide, u);
-        if (zs) load_row<EPT>(zs, n, wide, z);
-        sides.load(t0, w.len, side);
-        ds -= kSteps * p.dt_t;
-        us -= kSteps * g.grad_t;
-        if (zs) zs -= kSteps * p.gate_t;
+        const bool on = t0 + el.j < w.to;
+        ds.next(d, on, wide, most, -kSteps);
+        us.next(u, on, wide, most, -kSteps);
+        if (gated) zs.next(z, on, wide, most, -kSteps);
+        sides.load(t0, w.len);
         sides.advance(-kSteps);
     };
     if (w.from < w.to) request(last);
@@ -709,13 +715,12 @@ __global__ __launch_bounds__(kThreads) void scan_grad_carry_kernel(warpctct_scan
         for (int i = 0; i < EPT; ++i) {
             float v = d[i] + bias[i];
             if (p.softplus) v = softplus(v).value;
-            if (!(on && i < have)) v = 0.0f;
             float y = u[i];
-            if (zs) y *= z[i] * sigmoid(z[i]);
-            if (!(on && i < have)) y = 0.0f;
+            if (gated) y *= z[i] * sigmoid(z[i]);
+            if (!(on && i < have)) v = y = 0.0f;
             steps[el.j][el.c + i] = make_float2(v, y);
         }
-        sides.put(bc, side);
+        sides.put(bc, t0, w.len);
         __syncthreads();
         if (t0 - kSteps >= w.from) request(t0 - kSteps);
 #pragma unroll
@@ -828,11 +833,12 @@ int blocks_of(const warpctct_scan_t &p) {      // of a group
 }
 
 // Rows may be read and written in 16-byte pieces: so are they spaced and aligned,
-// and every group starts at a multiple of 16 bytes.
+// every group starts at a multiple of 16 bytes, and a thread has all of its `ept`
+// channels or none.
 template <typename IO>
-bool rows_wide(const warpctct_scan_t &p) {
+bool rows_wide(const warpctct_scan_t &p, int ept) {
     constexpr int V = kVec<IO>;
-    return p.E % V == 0 && (p.E / p.G) % V == 0 && p.x_n % V == 0 && p.x_t % V == 0 && p.dt_n % V == 0 &&
+    return p.E % V == 0 && (p.E / p.G) % V == 0 && (p.E / p.G) % ept == 0 && p.x_n % V == 0 && p.x_t % V == 0 && p.dt_n % V == 0 &&
            p.dt_t % V == 0 && p.gate_n % V == 0 && p.gate_t % V == 0 && aligned16(p.x) && aligned16(p.dt) &&
            aligned16(p.gate) && aligned16(p.out);
 }
@@ -879,7 +885,7 @@ hipError_t start(const warpctct_scan_t &p, float *keep, float *workspace, hipStr
     const Cut cut = cut_of(p);
     const Chunks chunks = chunks_of(p, workspace);
     const dim3 grid(p.G * blocks_of(p), p.N, cut.count);
-    const bool wide = rows_wide<IO>(p);
+    const bool wide = rows_wide<IO>(p, Elements<LANES, kSteps>::EPT);
     if (cut.count > 1) {
         auto carry = scan_kernel<IO, LANES, true>;
         TIMED_LAUNCH(carry, grid, dim3(kThreads), 0, stream, p, nullptr, chunks, nullptr, wide);
@@ -895,7 +901,7 @@ template <typename IO, int LANES>
 hipError_t start(const warpctct_scan_t &p, const warpctct_scan_grad_t &g, const float *keep, float *part_bc,
                  float *part_sums, float *workspace, hipStream_t stream) {
     constexpr int V = kVec<IO>;
-    const bool wide = rows_wide<IO>(p) && g.grad_n % V == 0 && g.grad_t % V == 0 && aligned16(g.grad_out) &&
+    const bool wide = rows_wide<IO>(p, Elements<LANES, kSteps>::EPT) && g.grad_n % V == 0 && g.grad_t % V == 0 && aligned16(g.grad_out) &&
                       aligned16(g.grad_x) && aligned16(g.grad_dt) && aligned16(g.grad_gate);
     const int blocks = blocks_of(p);
     if (p.N == 0) return hipSuccess;
