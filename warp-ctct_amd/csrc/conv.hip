@@ -84,13 +84,23 @@ __global__ __launch_bounds__(kThreads) void conv_kernel(warpctct_conv_t p, int t
     const int end = min(a.t0 + steps, p.L), live = min(end, len);
     int t = a.t0;
     if (t < live) {
+        // the rows asked for, and those being worked on
+        Raw<IO, EV> next[kAhead];
+        auto request = [&](int from) {
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) next[j].load(x + (long)min(from + j, live - 1) * p.x_t, true, 0);
+        };
+        request(t);
         float w[K][EV], b[EV], v[K - 1 + kAhead][EV];
         load_taps<EV, K>(p.weight, p.bias, a.e, w, b);
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) load_row<EV, K>(x, p.x_t, initial, p.E, t - (K - 1) + k, v[k]);
         for (; t < live; t += kAhead) {
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) load_n<EV>(x + (long)min(t + j, live - 1) * p.x_t, v[K - 1 + j]);
+            for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+                for (int i = 0; i < EV; ++i) v[K - 1 + j][i] = next[j][i];
+            if (t + kAhead < live) request(t + kAhead);
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 if (t + j >= live) break;
@@ -133,69 +143,86 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(warpctct_conv_t p, 
     IO *ginitial = g.grad_initial ? static_cast<IO *>(g.grad_initial) + before : nullptr;
     IO *gx = static_cast<IO *>(g.grad_x) + (long)a.n * p.L * p.E + a.e;
     const int end = min(a.t0 + steps, p.L);
-    float w[K][EV], b[EV], v[K][EV], gp[K][EV], gw[K][EV], gb[EV];
+    // windows of x and gp: K-1 rows behind, kAhead being worked on
+    float w[K][EV], b[EV], v[K - 1 + kAhead][EV], gp[K - 1 + kAhead][EV], gw[K][EV], gb[EV];
+    Raw<IO, EV> next_x[kAhead], next_g[kAhead];
+    auto request = [&](int from) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const long t = min(from + j, len - 1);
+            next_x[j].load(x + t * p.x_t, true, 0);
+            next_g[j].load(up + t * g.grad_t, true, 0);
+        }
+    };
+    if (a.t0 < len) request(a.t0);
     load_taps<EV, K>(p.weight, p.bias, a.e, w, b);
 #pragma unroll
     for (int i = 0; i < EV; ++i) {
         gb[i] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) gw[k][i] = gp[k][i] = v[k][i] = 0.0f;
+        for (int k = 0; k < K; ++k) gw[k][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) gp[k][i] = v[k][i] = 0.0f;
     }
     if (a.t0 < len) {
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) load_row<EV, K>(x, p.x_t, initial, p.E, a.t0 - (K - 1) + k, v[k + 1]);
+        for (int k = 0; k < K - 1; ++k) load_row<EV, K>(x, p.x_t, initial, p.E, a.t0 - (K - 1) + k, v[k]);
     }
-    for (int t = a.t0; t < end + K - 1; ++t) {
-        // the window moves on
+    for (int t0 = a.t0; t0 < end + K - 1; t0 += kAhead) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const bool in = t0 + j < len;
+#pragma unroll
+            for (int i = 0; i < EV; ++i) {
+                v[K - 1 + j][i] = in ? next_x[j][i] : 0.0f;
+                gp[K - 1 + j][i] = in ? next_g[j][i] : 0.0f;
+            }
+        }
+        if (t0 + kAhead < min(len, end + K - 1)) request(t0 + kAhead);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int t = t0 + j;
+#pragma unroll
+            for (int i = 0; i < EV; ++i) {
+                float &e = gp[K - 1 + j][i];
+                if (p.silu) {
+                    float y = b[i];
+#pragma unroll
+                    for (int k = 0; k < K; ++k) y = fmaf(w[k][i], v[j + k][i], y);
+                    const float s = sigmoid(y);
+                    e *= s * fmaf(y, 1.0f - s, 1.0f);
+                    if (t >= len) e = 0.0f;
+                }
+                const float own = t < end ? e : 0.0f;
+                gb[i] += own;
+#pragma unroll
+                for (int k = 0; k < K; ++k) gw[k][i] = fmaf(own, v[j + k][i], gw[k][i]);
+            }
+            const int s = t - (K - 1);      // gx[s] is complete
+            if (s >= end || (s < a.t0 && a.t0 > 0) || (s < 0 && !ginitial)) continue;
+            float d[EV];
+#pragma unroll
+            for (int i = 0; i < EV; ++i) {
+                d[i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < K; ++k) d[i] = fmaf(w[K - 1 - k][i], gp[j + k][i], d[i]);
+            }
+            const int r = s - len + K - 1;   // row s is row r of the state that was handed on
+            if (glast && r >= 0 && r < K - 1) {
+                float last[EV];
+                load_n<EV>(glast + (long)r * p.E, last);
+#pragma unroll
+                for (int i = 0; i < EV; ++i) d[i] += last[i];
+            }
+            store_n<EV>(s >= 0 ? gx + (long)s * p.E : ginitial + (long)(s + K - 1) * p.E, d);
+        }
 #pragma unroll
         for (int k = 0; k < K - 1; ++k)
 #pragma unroll
             for (int i = 0; i < EV; ++i) {
-                v[k][i] = v[k + 1][i];
-                gp[k][i] = gp[k + 1][i];
+                v[k][i] = v[k + kAhead][i];
+                gp[k][i] = gp[k + kAhead][i];
             }
-        if (t < len) {
-            load_n<EV>(x + (long)t * p.x_t, v[K - 1]);
-            float e[EV];
-            load_n<EV>(up + (long)t * g.grad_t, e);
-#pragma unroll
-            for (int i = 0; i < EV; ++i) {
-                if (p.silu) {
-                    float y = b[i];
-#pragma unroll
-                    for (int k = 0; k < K; ++k) y = fmaf(w[k][i], v[k][i], y);
-                    const float s = sigmoid(y);
-                    e[i] *= s * fmaf(y, 1.0f - s, 1.0f);
-                }
-                gp[K - 1][i] = e[i];
-                if (t < end) {
-                    gb[i] += e[i];
-#pragma unroll
-                    for (int k = 0; k < K; ++k) gw[k][i] = fmaf(e[i], v[k][i], gw[k][i]);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < EV; ++i) gp[K - 1][i] = v[K - 1][i] = 0.0f;
-        }
-        const int s = t - (K - 1);      // gx[s] is complete
-        if (s >= end || (s < a.t0 && a.t0 > 0)) continue;
-        if (s < 0 && !ginitial) continue;
-        float d[EV];
-#pragma unroll
-        for (int i = 0; i < EV; ++i) {
-            d[i] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < K; ++k) d[i] = fmaf(w[K - 1 - k][i], gp[k][i], d[i]);
-        }
-        const int r = s - len + K - 1;   // row s is row r of the state that was handed on
-        if (glast && r >= 0 && r < K - 1) {
-            float last[EV];
-            load_n<EV>(glast + (long)r * p.E, last);
-#pragma unroll
-            for (int i = 0; i < EV; ++i) d[i] += last[i];
-        }
-        store_n<EV>(s >= 0 ? gx + (long)s * p.E : ginitial + (long)(s + K - 1) * p.E, d);
     }
     if (!partial) return;
     float *mine = partial + ((size_t)a.n * tiles + a.t0 / steps) * (size_t)p.E * (K + 1);

@@ -21,7 +21,8 @@ namespace {
 constexpr int kThreads = 256;        // of a workgroup whose wavefronts take a row each
 constexpr int kWide = 1024;          // the largest number of threads on one row
 constexpr int kMostInRegisters = 16 * kWide;
-constexpr int kGradGroups = 512;     // workgroups of the backward pass, at most
+constexpr unsigned kGroups = 1024;   // workgroups of the forward pass, at most
+constexpr int kGradGroups = 512;     // and of the backward pass, two on a compute unit
 
 // Sums of two values over the threads of a row: a wavefront (threads == 64) or
 // the whole workgroup.  `shared` holds 2 floats per wavefront and is free again
@@ -72,20 +73,21 @@ struct Slots {
     static __device__ __forceinline__ int first(int j, int t, int threads) {
         return (j * threads + t) * EV;
     }
-    // elements past the row read as `fill`
-    static __device__ __forceinline__ void load(const IO *row, int width, int t, int threads, float (&x)[CAP]) {
+    // A row as it was loaded.  All loads are issued together, those past the row
+    // at its last elements; unpack() masks them.
+    struct Row {
+        Raw<IO, EV> v[NV];
+    };
+    static __device__ __forceinline__ void load(Row &r, const IO *row, int width, int t, int threads) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) r.v[j].load(row + min(first(j, t, threads), width - EV), true, 0);
+    }
+    static __device__ __forceinline__ void unpack(const Row &r, int width, int t, int threads, float (&x)[CAP]) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int at = first(j, t, threads);
-            if (at < width) {
-                if (VEC)
-                    load_vec(row + at, x + j * EV);
-                else
-                    x[j] = to_float(row[at]);
-            } else {
+            const bool in = first(j, t, threads) < width;
 #pragma unroll
-                for (int i = 0; i < EV; ++i) x[j * EV + i] = 0.0f;
-            }
+            for (int i = 0; i < EV; ++i) x[j * EV + i] = in ? r.v[j][i] : 0.0f;
         }
     }
     static __device__ __forceinline__ void store(IO *row, int width, int t, int threads, const float (&x)[CAP]) {
@@ -100,16 +102,19 @@ struct Slots {
             }
         }
     }
-    // a parameter of the columns, `other` where there is none; not through
-    // vectors: its start need not be aligned, and it comes from the caches
+    // a parameter of the columns, `other` where there is none (its start need not
+    // be aligned)
     template <typename W>
     static __device__ __forceinline__ void load_param(const W *p, float other, int width, int t, int threads,
                                                       float (&x)[CAP]) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int at = first(j, t, threads);
+        for (int i = 0; i < CAP; ++i) x[i] = other;
+        if (!p) return;
 #pragma unroll
-            for (int i = 0; i < EV; ++i) x[j * EV + i] = (p && at < width) ? to_float(p[at + i]) : other;
+        for (int j = 0; j < NV; ++j) {
+            const int at = min(first(j, t, threads), width - EV);
+#pragma unroll
+            for (int i = 0; i < EV; ++i) x[j * EV + i] = to_float(p[at + i]);
         }
     }
 };
@@ -122,43 +127,47 @@ __global__ __launch_bounds__(BLOCK) void norm_kernel(const IO *__restrict__ x, R
     typedef Slots<IO, VEC, CAP> S;
     __shared__ float shared[2 * kWide / 64];
     const int t = threads == 64 ? threadIdx.x & 63 : threadIdx.x;
-    const unsigned row = threads == 64 ? blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6) : blockIdx.x;
-    if (row >= rows) return;      // whole wavefronts; a row of the whole workgroup always exists
-    float v[CAP];
-    S::load(x + at.at(row), width, t, threads, v);
+    const unsigned per = threads == 64 ? blockDim.x >> 6 : 1u;
+    const unsigned stride = gridDim.x * per;
+    unsigned row = blockIdx.x * per + (threads == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+    if (row >= rows) return;      // whole wavefronts; a workgroup on one row always has one
     const float inv = 1.0f / (float)width;
-    float sum = 0.0f, none = 0.0f;
-#pragma unroll
-    for (int i = 0; i < CAP; ++i) sum += v[i];
-    row_sums(sum, none, threads, shared);
-    const float m = sum * inv;
-    float off = 0.0f, sq = 0.0f;
-#pragma unroll
-    for (int j = 0; j < S::NV; ++j) {
-        const bool in = S::first(j, t, threads) < width;
-#pragma unroll
-        for (int i = 0; i < S::EV; ++i) {
-            float &e = v[j * S::EV + i];
-            e = in ? e - m : 0.0f;
-            off += e;
-            sq = fmaf(e, e, sq);
-        }
-    }
-    row_sums(off, sq, threads, shared);
-    const float c = off * inv;                       // what the first mean was off by
-    const float var = fmaxf(sq * inv - c * c, 0.0f);
-    const float r = 1.0f / sqrtf(var + eps);
-    if (stats && t == 0) keep_stats(stats, row, m, c, r);
-    float w[CAP];
+    typename S::Row raw;
+    S::load(raw, x + at.at(row), width, t, threads);
+    float w[CAP], b[CAP];
     S::load_param(weight, 1.0f, width, t, threads, w);
+    S::load_param(bias, 0.0f, width, t, threads, b);
+    for (; row < rows; row += stride) {
+        float v[CAP];
+        S::unpack(raw, width, t, threads, v);
+        // the next row, while this one is worked on
+        if (rows - row > stride) S::load(raw, x + at.at(row + stride), width, t, threads);
+        float sum = 0.0f, none = 0.0f;
 #pragma unroll
-    for (int i = 0; i < CAP; ++i) v[i] = (v[i] - c) * r * w[i];
-    if (bias) {
-        S::load_param(bias, 0.0f, width, t, threads, w);
+        for (int i = 0; i < CAP; ++i) sum += v[i];
+        row_sums(sum, none, threads, shared);
+        const float m = sum * inv;
+        float off = 0.0f, sq = 0.0f;
 #pragma unroll
-        for (int i = 0; i < CAP; ++i) v[i] += w[i];
+        for (int j = 0; j < S::NV; ++j) {
+            const bool in = S::first(j, t, threads) < width;
+#pragma unroll
+            for (int i = 0; i < S::EV; ++i) {
+                float &e = v[j * S::EV + i];
+                e = in ? e - m : 0.0f;
+                off += e;
+                sq = fmaf(e, e, sq);
+            }
+        }
+        row_sums(off, sq, threads, shared);
+        const float c = off * inv;                       // what the first mean was off by
+        const float var = fmaxf(sq * inv - c * c, 0.0f);
+        const float r = 1.0f / sqrtf(var + eps);
+        if (stats && t == 0) keep_stats(stats, row, m, c, r);
+#pragma unroll
+        for (int i = 0; i < CAP; ++i) v[i] = fmaf((v[i] - c) * r, w[i], b[i]);
+        S::store(out + (long)row * width, width, t, threads, v);
     }
-    S::store(out + (long)row * width, width, t, threads, v);
 }
 
 // Rows too wide for the registers of one workgroup: three passes over the row.
@@ -213,10 +222,21 @@ __global__ __launch_bounds__(BLOCK) void norm_grad_kernel(
     S::load_param(weight, 1.0f, width, t, threads, w);
 #pragma unroll
     for (int i = 0; i < CAP; ++i) gw[i] = gb[i] = 0.0f;
-    for (unsigned row = blockIdx.x * per + wave; row < rows; row += gridDim.x * per) {
+    const unsigned stride = gridDim.x * per;
+    unsigned row = blockIdx.x * per + wave;
+    typename S::Row xr, gr;
+    if (row < rows) {
+        S::load(xr, x + x_at.at(row), width, t, threads);
+        S::load(gr, g + g_at.at(row), width, t, threads);
+    }
+    for (; row < rows; row += stride) {
         float h[CAP], e[CAP];
-        S::load(x + x_at.at(row), width, t, threads, h);
-        S::load(g + g_at.at(row), width, t, threads, e);
+        S::unpack(xr, width, t, threads, h);
+        S::unpack(gr, width, t, threads, e);
+        if (rows - row > stride) {      // the next row, while this one is worked on
+            S::load(xr, x + x_at.at(row + stride), width, t, threads);
+            S::load(gr, g + g_at.at(row + stride), width, t, threads);
+        }
         const RowStats s = row_stats(stats, row);
         float su = 0.0f, suh = 0.0f;
 #pragma unroll
@@ -322,12 +342,13 @@ bool rows_aligned(const void *p, const RowAddress &a, size_t size) {
 // Threads on a row: a wavefront up to 2048 elements (32 registers a lane),
 // then a workgroup of 256, or of 1024 above
 // 8192 elements (16 registers a lane there: a lane of so large a workgroup has 128).
-int threads_for(int width) { return width <= 32 * 64 ? 64 : width <= 32 * kThreads ? kThreads : kWide; }
+int threads_for(int width) { return width <= 16 * 64 ? 64 : width <= 32 * kThreads ? kThreads : kWide; }
 
 template <typename IO, typename W, bool VEC, int CAP, int BLOCK>
 hipError_t start(const warpctct_norm_t &p, const RowAddress &at, int threads, hipStream_t stream) {
     const unsigned rows = (unsigned)p.rows;
-    const dim3 grid(threads == 64 ? (rows + 3) / 4 : rows), block(BLOCK);
+    const unsigned groups = threads == 64 ? (rows + 3) / 4 : rows;
+    const dim3 grid(groups < kGroups ? groups : kGroups), block(BLOCK);
     auto kernel = norm_kernel<IO, W, VEC, CAP, BLOCK>;
     TIMED_LAUNCH(kernel, grid, block, 0, stream, static_cast<const IO *>(p.x), at, static_cast<const W *>(p.weight),
                  static_cast<const W *>(p.bias), p.eps, static_cast<IO *>(p.out), p.stats, rows, p.width,
@@ -413,7 +434,7 @@ hipError_t start_grad(const warpctct_norm_t &p, const warpctct_norm_grad_t &g, f
 }  // namespace
 
 int norm_grad_groups(long rows, int width) {
-    const long per = width <= 32 * 64 ? 4 : 1;      // rows of a workgroup at a time
+    const long per = width <= 16 * 64 ? 4 : 1;      // rows of a workgroup at a time
     const long groups = (rows + per - 1) / per;
     return (int)(groups < kGradGroups ? groups : kGradGroups);
 }
