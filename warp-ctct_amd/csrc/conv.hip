@@ -316,7 +316,7 @@ bool fits(const warpctct_conv_t &p, int ev) {
 
 template <typename IO, int K>
 hipError_t run(const warpctct_conv_t &p, hipStream_t stream) {
-    return fits<IO>(p, kVec<IO>) ? start<IO, K, kVec<IO>>(p, stream) : start<IO, K, 1>(p, stream);
+    return fits<IO>(p, 4) ? start<IO, K, 4>(p, stream) : start<IO, K, 1>(p, stream);
 }
 template <typename IO, int K>
 hipError_t run(const warpctct_conv_t &p, const warpctct_conv_grad_t &g, float *partial, hipStream_t stream) {
