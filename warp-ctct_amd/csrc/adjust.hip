@@ -5,8 +5,12 @@
 //               l = l - presence - frequency * count
 //   l = l + bias[v];  not allowed: l = -infinity
 // Bound by HBM, or by the launch where the logits are few.  A workgroup takes
-// `segment` columns of a row: it counts those of the row's tokens that fall into
-// them in LDS (integers: the order does not matter), then streams its columns.
+// kVectors 16-byte vectors a thread (4096 columns of 2-byte elements) of a row,
+// asks for them first, counts meanwhile those of the row's tokens that fall into
+// its columns in LDS (integers: the order does not matter), and applies the rules.
+// More columns a workgroup would read the history less often, but 16384 of them
+// take 64 KB of LDS for the counts, which leaves 8 wavefronts on a compute unit:
+// 20.3 us instead of 11.5 for 128 rows of 65536 bfloat16 logits with 300 tokens each.
 #include "network.h"
 #include "rows.h"
 
@@ -15,87 +19,104 @@ namespace wctct {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kVectors = 2;      // 16-byte vectors of a thread
 
-template <typename B>
-__device__ __forceinline__ float bias_at(const void *bias, long at) {
-    return to_float(static_cast<const B *>(bias)[at]);
-}
-__device__ __forceinline__ float bias_of(const void *bias, int type, long at) {
-    return type == kIoF32 ? bias_at<float>(bias, at)
-                          : type == kIoF16 ? bias_at<f16>(bias, at) : bias_at<bf16>(bias, at);
+// EV columns of a bias of any of the three types, all of them asked for at once
+template <typename B, int EV>
+__device__ __forceinline__ void load_bias(const void *bias, long at, float (&b)[EV]) {
+    B v[EV];
+#pragma unroll
+    for (int i = 0; i < EV; ++i) v[i] = static_cast<const B *>(bias)[at + i];
+#pragma unroll
+    for (int i = 0; i < EV; ++i) b[i] = to_float(v[i]);
 }
 
 template <typename IO, bool VEC>
-__global__ __launch_bounds__(kThreads) void adjust_kernel(warpctct_adjust_t p, int segment) {
-    constexpr int EV = VEC ? kVec<IO> : 1;
-    extern __shared__ unsigned counts[];
-    const int n = blockIdx.y, from = blockIdx.x * segment, to = min(from + segment, p.V);
+__global__ __launch_bounds__(kThreads) void adjust_kernel(warpctct_adjust_t p) {
+    constexpr int EV = VEC ? kVec<IO> : 1, U = VEC ? kVectors : kVectors * kVec<IO>, SEGMENT = kThreads * EV * U;
+    __shared__ unsigned counts[SEGMENT];
+    const int n = blockIdx.y, from = blockIdx.x * SEGMENT, t = threadIdx.x;
     const bool history = p.tokens && p.H > 0;
+    const IO *in = static_cast<const IO *>(p.logits) + (long)n * p.logits_n;
+    Raw<IO, EV> raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) raw[u].load(in + min(from + (u * kThreads + t) * EV, p.V - EV), true, 0);
+    // the bias, and a bit for every column that is allowed
+    float bias[U][EV];
+    unsigned bits[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int at = min(from + (u * kThreads + t) * EV, p.V - EV);
+        const long b = (long)n * p.bias_n + at, m = (long)n * p.allowed_n;
+        if (p.bias && p.bias_dtype == kIoF32) load_bias<float>(p.bias, b, bias[u]);
+        if (p.bias && p.bias_dtype == kIoF16) load_bias<f16>(p.bias, b, bias[u]);
+        if (p.bias && p.bias_dtype == kIoBF16) load_bias<bf16>(p.bias, b, bias[u]);
+        bits[u] = ~0u;
+        if (p.allowed && p.allowed_packed) {
+            // (at is a multiple of EV, which divides 32: the bits lie in one word)
+            bits[u] = static_cast<const unsigned *>(p.allowed)[m + (at >> 5)] >> (at & 31);
+        } else if (p.allowed) {
+            unsigned char flag[EV];
+#pragma unroll
+            for (int i = 0; i < EV; ++i) flag[i] = static_cast<const unsigned char *>(p.allowed)[m + at + i];
+            bits[u] = 0u;
+#pragma unroll
+            for (int i = 0; i < EV; ++i) bits[u] |= (flag[i] ? 1u : 0u) << i;
+        }
+    }
     float repetition = p.repetition, presence = p.presence, frequency = p.frequency;
     if (history) {
-        for (int k = threadIdx.x; k < to - from; k += kThreads) counts[k] = 0u;
-        __syncthreads();
+        const int to = min(from + SEGMENT, p.V);
+        for (int k = t; k < to - from; k += kThreads) counts[k] = 0u;
         const int h = p.tokens_lengths ? min(max(p.tokens_lengths[n], 0), p.H) : p.H;
         const long row = (long)n * p.tokens_n;
-        for (int i = threadIdx.x; i < h; i += kThreads) {
+        __syncthreads();
+        for (int i = t; i < h; i += kThreads) {
             const long v = p.tokens_64 ? (long)static_cast<const long long *>(p.tokens)[row + i]
                                        : (long)static_cast<const int *>(p.tokens)[row + i];
             if (v >= from && v < to) atomicAdd(&counts[v - from], 1u);
         }
-        __syncthreads();
         if (p.repetitions) repetition = p.repetitions[n];
         if (p.presences) presence = p.presences[n];
         if (p.frequencies) frequency = p.frequencies[n];
+        __syncthreads();
     }
-    const IO *in = static_cast<const IO *>(p.logits) + (long)n * p.logits_n;
     IO *out = static_cast<IO *>(p.out) + (long)n * p.V;
-    const unsigned char *flags =
-        p.allowed && !p.allowed_packed ? static_cast<const unsigned char *>(p.allowed) + (long)n * p.allowed_n : nullptr;
-    const unsigned *words =
-        p.allowed && p.allowed_packed ? static_cast<const unsigned *>(p.allowed) + (long)n * p.allowed_n : nullptr;
-    for (int at = from + threadIdx.x * EV; at < to; at += kThreads * EV) {
-        float l[EV];
-        load_n<EV>(in + at, l);
-        // (from is a multiple of 32 and EV divides 32: the bits lie in one word)
-        const unsigned bits = words ? words[at >> 5] >> (at & 31) : 0u;
 #pragma unroll
-        for (int i = 0; i < EV; ++i) {
-            const int v = at + i;
-            if (history) {
-                const unsigned count = counts[v - from];
-                if (count) {
-                    l[i] = l[i] > 0.0f ? l[i] / repetition : l[i] * repetition;
-                    l[i] = l[i] - presence - frequency * (float)count;
+    for (int u = 0; u < U; ++u) {
+        const int at = from + (u * kThreads + t) * EV;
+        if (at >= p.V) break;
+        float l[EV];
+#pragma unroll
+        for (int i = 0; i < EV; ++i) l[i] = raw[u][i];
+        if (history) {
+            // (of a vector's columns together: most of them have no count)
+            unsigned count[EV], any = 0u;
+#pragma unroll
+            for (int i = 0; i < EV; ++i) any |= count[i] = counts[at - from + i];
+            if (any) {
+#pragma unroll
+                for (int i = 0; i < EV; ++i) {
+                    const float scaled = l[i] > 0.0f ? l[i] / repetition : l[i] * repetition;
+                    const float less = scaled - presence - frequency * (float)count[i];
+                    l[i] = count[i] ? less : l[i];
                 }
             }
-            if (p.bias) l[i] += bias_of(p.bias, p.bias_dtype, (long)n * p.bias_n + v);
-            if (words && !((bits >> i) & 1u)) l[i] = -__builtin_huge_valf();
-            if (flags && !flags[v]) l[i] = -__builtin_huge_valf();
+        }
+#pragma unroll
+        for (int i = 0; i < EV; ++i) {
+            if (p.bias) l[i] += bias[u][i];
+            l[i] = (bits[u] >> i) & 1u ? l[i] : -__builtin_huge_valf();
         }
         store_n<EV>(out + at, l);
     }
 }
 
-// Columns of a workgroup, a multiple of 2048.  Every workgroup of a row reads
-// the row's whole history, which should stay the smaller part of its traffic; but
-// there should be two workgroups for every compute unit first, and the counts of
-// 16384 columns take all the LDS that two workgroups on a compute unit can have.
-int segment_of(long N, int V, int H, bool history) {
-    long segment = 2048;
-    while (segment < V && segment < 16384 && N * ((V + 2 * segment - 1) / (2 * segment)) >= 512 &&
-           (!history || 2L * H > segment || segment < 4096))
-        segment *= 2;
-    return (int)segment;
-}
-
 template <typename IO, bool VEC>
 hipError_t start(const warpctct_adjust_t &p, hipStream_t stream) {
-    const bool history = p.tokens && p.H > 0;
-    const int segment = segment_of(p.N, p.V, p.H, history);
-    const dim3 grid((p.V + segment - 1) / segment, p.N);
-    const size_t shared = history ? sizeof(unsigned) * (size_t)(p.V < segment ? p.V : segment) : 0;
+    const int segment = kThreads * kVec<IO> * kVectors;
     auto kernel = adjust_kernel<IO, VEC>;
-    TIMED_LAUNCH(kernel, grid, dim3(kThreads), shared, stream, p, segment);
+    TIMED_LAUNCH(kernel, dim3((p.V + segment - 1) / segment, p.N), dim3(kThreads), 0, stream, p);
     return hipGetLastError();
 }
 

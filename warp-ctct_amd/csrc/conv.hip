@@ -168,7 +168,9 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(warpctct_conv_t p, 
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) load_row<EV, K>(x, p.x_t, initial, p.E, a.t0 - (K - 1) + k, v[k]);
     }
-    for (int t0 = a.t0; t0 < end + K - 1; t0 += kAhead) {
+    // behind the sequence there is nothing but zeros to write
+    const int work = a.t0 < len || a.t0 == 0 ? min(end, len) + K - 1 : a.t0;
+    for (int t0 = a.t0; t0 < work; t0 += kAhead) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const bool in = t0 + j < len;
@@ -178,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(warpctct_conv_t p, 
                 gp[K - 1 + j][i] = in ? next_g[j][i] : 0.0f;
             }
         }
-        if (t0 + kAhead < min(len, end + K - 1)) request(t0 + kAhead);
+        if (t0 + kAhead < min(len, work)) request(t0 + kAhead);
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int t = t0 + j;
@@ -199,7 +201,7 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(warpctct_conv_t p, 
                 for (int k = 0; k < K; ++k) gw[k][i] = fmaf(own, v[j + k][i], gw[k][i]);
             }
             const int s = t - (K - 1);      // gx[s] is complete
-            if (s >= end || (s < a.t0 && a.t0 > 0) || (s < 0 && !ginitial)) continue;
+            if (s >= min(end, len) || (s < a.t0 && a.t0 > 0) || (s < 0 && !ginitial)) continue;
             float d[EV];
 #pragma unroll
             for (int i = 0; i < EV; ++i) {
@@ -224,6 +226,8 @@ __global__ __launch_bounds__(kThreads) void conv_grad_kernel(warpctct_conv_t p, 
                 gp[k][i] = gp[k + kAhead][i];
             }
     }
+    const float zero[EV] = {};
+    for (int s = max(a.t0, len); s < end; ++s) store_n<EV>(gx + (long)s * p.E, zero);
     if (!partial) return;
     float *mine = partial + ((size_t)a.n * tiles + a.t0 / steps) * (size_t)p.E * (K + 1);
 #pragma unroll
