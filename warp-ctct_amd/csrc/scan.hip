@@ -843,53 +843,57 @@ bool rows_wide(const warpctct_scan_t &p, int ept) {
            aligned16(p.gate) && aligned16(p.out);
 }
 
-// Chunks that a sequence is cut into: one while its workgroups alone put a
-// wavefront on every second SIMD or more, since two passes cost twice the
-// arithmetic; otherwise as many as put two wavefronts on each, of two tiles at
-// least.
+// Chunks that a sequence is cut into.  Two passes cost twice the arithmetic
+// forwards and a quarter more backwards, but a wavefront alone on its SIMD waits
+// most of the time: cutting pays up to 768 wavefronts of uncut sequences (1024
+// SIMDs) forwards and 1024 backwards, into as many chunks as put eight wavefronts
+// on each, of two tiles at least.  Measured with 1024 channels, 16 states, 1500
+// steps (us, uncut / cut): forwards 512 wavefronts 186 / 102, 768 186 / 139, 1024
+// 188 / 178, 1536 245 / 272; backwards 1024 595 / 454, 1536 746 / 711, 2048
+// 751 / 885; with 300 steps forwards 768 41 / 45, backwards 1024 130 / 111, 1536
+// 157 / 162.  Fewer than 8 tiles are not worth the two launches more.
 struct Cut {
     int count, tiles;
 };
-Cut cut_of(const warpctct_scan_t &p) {
+Cut cut_of(const warpctct_scan_t &p, bool backward) {
     const long waves = (long)p.N * p.G * blocks_of(p) * (kThreads / 64), tiles = ((long)p.L + kSteps - 1) / kSteps;
     Cut c = {1, (int)tiles};
-    if (waves <= 0 || waves > 512 || tiles < 4) return c;
-    const long count = std::min(2048 / waves, tiles / 2);
+    if (waves <= 0 || waves > (backward ? 1024 : 768) || tiles < 8) return c;
+    const long count = std::min(8192 / waves, tiles / 2);
     c.tiles = (int)((tiles + count - 1) / count);
     c.count = (int)((tiles + c.tiles - 1) / c.tiles);
     return c;
 }
-size_t chunk_floats(const warpctct_scan_t &p) {
-    const Cut c = cut_of(p);
+size_t chunk_floats(const warpctct_scan_t &p, bool backward) {
+    const Cut c = cut_of(p, backward);
     return c.count > 1 ? (size_t)p.N * c.count * p.E * (kStates * lanes_of(p.S) + 1) : 0;
 }
-Chunks chunks_of(const warpctct_scan_t &p, float *workspace) {
-    const Cut c = cut_of(p);
+Chunks chunks_of(const warpctct_scan_t &p, const Cut &c, float *workspace) {
     Chunks k;
     k.local = workspace;
     k.total = workspace + (c.count > 1 ? (size_t)p.N * c.count * p.E * (kStates * lanes_of(p.S)) : 0);
     k.tiles = c.tiles;
     return k;
 }
-hipError_t join_chunks(const warpctct_scan_t &p, const float *first, const Chunks &chunks, bool backwards, float *end,
-                       hipStream_t stream) {
+hipError_t join_chunks(const warpctct_scan_t &p, const float *first, const Chunks &chunks, int count, bool backwards,
+                       float *end, hipStream_t stream) {
     const int SP = kStates * lanes_of(p.S);
     const long threads = (long)p.E * SP;
     TIMED_LAUNCH(scan_join_kernel, dim3((unsigned)((threads + kThreads - 1) / kThreads), p.N), dim3(kThreads), 0,
-                 stream, p.a, first, chunks, cut_of(p).count, p.E, p.S, SP, backwards, end);
+                 stream, p.a, first, chunks, count, p.E, p.S, SP, backwards, end);
     return hipGetLastError();
 }
 
 template <typename IO, int LANES>
 hipError_t start(const warpctct_scan_t &p, float *keep, float *workspace, hipStream_t stream) {
-    const Cut cut = cut_of(p);
-    const Chunks chunks = chunks_of(p, workspace);
+    const Cut cut = cut_of(p, false);
+    const Chunks chunks = chunks_of(p, cut, workspace);
     const dim3 grid(p.G * blocks_of(p), p.N, cut.count);
     const bool wide = rows_wide<IO>(p, Elements<LANES, kSteps>::EPT);
     if (cut.count > 1) {
         auto carry = scan_kernel<IO, LANES, true>;
         TIMED_LAUNCH(carry, grid, dim3(kThreads), 0, stream, p, nullptr, chunks, nullptr, wide);
-        const hipError_t e = join_chunks(p, p.initial, chunks, false, nullptr, stream);
+        const hipError_t e = join_chunks(p, p.initial, chunks, cut.count, false, nullptr, stream);
         if (e != hipSuccess) return e;
     }
     auto kernel = scan_kernel<IO, LANES, false>;
@@ -905,14 +909,14 @@ hipError_t start(const warpctct_scan_t &p, const warpctct_scan_grad_t &g, const 
                       aligned16(g.grad_x) && aligned16(g.grad_dt) && aligned16(g.grad_gate);
     const int blocks = blocks_of(p);
     if (p.N == 0) return hipSuccess;
-    const Cut cut = cut_of(p);
-    const Chunks chunks = chunks_of(p, workspace);
+    const Cut cut = cut_of(p, true);
+    const Chunks chunks = chunks_of(p, cut, workspace);
     const dim3 grid(p.G * blocks, p.N, cut.count);
     hipError_t e;
     if (cut.count > 1) {
         auto carry = scan_grad_carry_kernel<IO, LANES>;
         TIMED_LAUNCH(carry, grid, dim3(kThreads), 0, stream, p, g, chunks, wide);
-        e = join_chunks(p, g.grad_last, chunks, true, g.grad_initial, stream);
+        e = join_chunks(p, g.grad_last, chunks, cut.count, true, g.grad_initial, stream);
         if (e != hipSuccess) return e;
     }
     auto kernel = scan_grad_kernel<IO, LANES>;
@@ -965,10 +969,11 @@ size_t scan_keep_floats(int N, int L, int E, int S) {
     return (size_t)N * (back_rows(L, lanes) / back_steps(lanes)) * E * (kStates * lanes);
 }
 
-size_t scan_floats(const warpctct_scan_t &p) { return chunk_floats(p); }
+size_t scan_floats(const warpctct_scan_t &p) { return chunk_floats(p, false); }
 
 size_t scan_grad_floats(const warpctct_scan_t &p) {
-    return part_bc_floats(p) + chunk_floats(p) + column_sums_floats((long)p.N * cut_of(p).count, (long)p.E * (p.S + 2));
+    return part_bc_floats(p) + chunk_floats(p, true) +
+           column_sums_floats((long)p.N * cut_of(p, true).count, (long)p.E * (p.S + 2));
 }
 
 hipError_t launch_scan(const warpctct_scan_t &p, float *keep, float *workspace, hipStream_t stream) {
@@ -977,11 +982,11 @@ hipError_t launch_scan(const warpctct_scan_t &p, float *keep, float *workspace, 
 
 hipError_t launch_scan_grad(const warpctct_scan_t &p, const warpctct_scan_grad_t &g, const float *keep,
                             float *workspace, hipStream_t stream) {
-    float *part_bc = workspace, *local = part_bc + part_bc_floats(p), *part_sums = local + chunk_floats(p);
+    float *part_bc = workspace, *local = part_bc + part_bc_floats(p), *part_sums = local + chunk_floats(p, true);
     const hipError_t e = by_type(p.dtype, p.S, p, g, keep, part_bc, part_sums, local, stream);
     if (e != hipSuccess) return e;
     // (the skip's and the bias's gradients lie next to each other)
-    return launch_column_sums(part_sums, (long)p.N * cut_of(p).count, p.E * (p.S + 2), p.E * p.S, g.grad_a, kIoF32,
+    return launch_column_sums(part_sums, (long)p.N * cut_of(p, true).count, p.E * (p.S + 2), p.E * p.S, g.grad_a, kIoF32,
                               g.grad_skip_bias, kIoF32, stream);
 }
 
