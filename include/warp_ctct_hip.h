@@ -636,8 +636,8 @@ int warpctct_selective_scan(const warpctct_scan_t *p, void *keep, size_t keep_by
 /* Gradients for grad_out (addressed like x by grad_n, grad_t) and, if not NULL,
  * grad_last (N, E, S): in the type of x and dense grad_x, grad_dt, grad_gate
  * (N, L, E; the last NULL without a gate), grad_b, grad_c (N, L, G, S); in float
- * grad_a (E, S), grad_skip_bias (2, E: those of skip and of dt_bias, formed
- * whether or not there is one) and grad_initial (N, E, S; may be NULL).  keep as
+ * grad_a (E, S), grad_skip, grad_dt_bias (E) and grad_initial (N, E, S), the
+ * last three of which may be NULL.  keep as
  * the forward call left it; `out` and `last` of p are not used.  Sums over
  * channels, steps and sequences are added up in a fixed order through
  * `workspace` (warpctct_selective_scan_workspace_bytes(..., 1), 16-byte aligned). */
@@ -646,7 +646,7 @@ typedef struct {
     const void *grad_out;
     const float *grad_last;
     void *grad_x, *grad_dt, *grad_gate, *grad_b, *grad_c;
-    float *grad_a, *grad_skip_bias, *grad_initial;
+    float *grad_a, *grad_skip, *grad_dt_bias, *grad_initial;
 } warpctct_scan_grad_t;
 int warpctct_selective_scan_grad(const warpctct_scan_t *p, const warpctct_scan_grad_t *g, const void *keep,
                                  size_t keep_bytes, void *workspace, size_t workspace_bytes, void *stream);

@@ -161,7 +161,7 @@ class Scan(ctypes.Structure):
 class ScanGrad(ctypes.Structure):
     _fields_ = [("grad_n", ctypes.c_long), ("grad_t", ctypes.c_long)] + [
         (k, P) for k in ("grad_out", "grad_last", "grad_x", "grad_dt", "grad_gate", "grad_b", "grad_c", "grad_a",
-                         "grad_skip_bias", "grad_initial")]
+                         "grad_skip", "grad_dt_bias", "grad_initial")]
 
 
 class ScanStep(ctypes.Structure):
@@ -216,18 +216,17 @@ def test_selective_scan_gradient_and_step_arguments():
     size = lib.warpctct_selective_scan_workspace_bytes
     size.restype = ctypes.c_size_t
     need = size(2, 20, 8, 16, 2, 1)
-    assert need >= 4 * (2 * 2 * 2 * 16 * 32 + 2 * 8 * 18) and size(2, 20, 9, 16, 2, 1) == 0
+    assert need == 4 * (2 * 2 * 24 * 32 + 2 * 8 * 18) and size(2, 20, 9, 16, 2, 1) == 0
 
     def call(p=None, keep=ALIGNED, kept=1 << 20, workspace=ALIGNED, have=1 << 20, **over):
-        fields = dict(grad_out=SOME, grad_x=SOME, grad_dt=SOME, grad_b=SOME, grad_c=SOME, grad_a=SOME,
-                      grad_skip_bias=SOME)
+        fields = dict(grad_out=SOME, grad_x=SOME, grad_dt=SOME, grad_b=SOME, grad_c=SOME, grad_a=SOME)
         fields.update(over)
         return lib.warpctct_selective_scan_grad(ctypes.byref(p or scan()), ctypes.byref(ScanGrad(**fields)), P(keep),
                                                 ctypes.c_size_t(kept), P(workspace), ctypes.c_size_t(have), P(0))
 
     for bad in BAD_SCANS:
         assert call(scan(**bad)) == EINVAL, bad
-    for bad in ("grad_out", "grad_x", "grad_dt", "grad_b", "grad_c", "grad_a", "grad_skip_bias"):
+    for bad in ("grad_out", "grad_x", "grad_dt", "grad_b", "grad_c", "grad_a"):
         assert call(**{bad: None}) == EINVAL, bad
     assert call(scan(gate=SOME)) == EINVAL
     assert call(keep=0) == EINVAL and call(workspace=0) == EINVAL and call(workspace=ALIGNED + 4) == EINVAL

@@ -47,9 +47,19 @@ void refuse_second_derivative(const char *name) {
 const void *ptr(const torch::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 float *floats(const torch::Tensor &t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 
-torch::Tensor bytes_like(const torch::Tensor &like, size_t bytes) {
-    return torch::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::ScalarType::Byte));
+// An uninitialised tensor on the device of `like`.  (Below autograd in the
+// dispatcher: these calls are a good part of what a step costs the host.)
+torch::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const torch::Tensor &like) {
+    const at::AutoDispatchBelowAutograd below;
+    return at::empty(sizes, like.options().dtype(type));
 }
+torch::Tensor fresh(at::IntArrayRef sizes, const torch::Tensor &like) {
+    return fresh(sizes, like.scalar_type(), like);
+}
+torch::Tensor fresh_bytes(size_t bytes, const torch::Tensor &like) {
+    return fresh({static_cast<int64_t>(bytes)}, at::ScalarType::Byte, like);
+}
+constexpr at::ScalarType kFloat = at::ScalarType::Float;
 
 // ---- layer norm --------------------------------------------------------------
 
@@ -116,10 +126,10 @@ struct NormCall {
 // out, and with `keep` what the backward pass needs of every row
 std::tuple<torch::Tensor, torch::Tensor> norm_forward(NormCall &call, bool keep) {
     const DeviceGuard guard(device_of(call.x.t));
-    auto out = torch::empty(call.x.t.sizes(), call.x.t.options());
+    auto out = fresh(call.x.t.sizes(), call.x.t);
     torch::Tensor stats;
     if (keep) {
-        stats = torch::empty({call.p.rows, 3}, call.x.t.options().dtype(at::ScalarType::Float));
+        stats = fresh({call.p.rows, 3}, kFloat, call.x.t);
         call.p.stats = stats.data_ptr<float>();
     }
     call.p.out = out.data_ptr();
@@ -159,16 +169,15 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
         grads.inner_stride = g.inner_stride;
         grads.grad_out = g.t.data_ptr();
         torch::Tensor gx, gw, gb, workspace;
-        if (track[0]) gx = torch::empty(x.sizes(), x.options());
-        const auto params = x.options().dtype(call.p.weight_dtype == call.p.dtype ? x.scalar_type()
-                                                                                  : at::ScalarType::Float);
-        if (track[1]) gw = torch::empty({call.p.width}, params);
-        if (track[2]) gb = torch::empty({call.p.width}, params);
+        if (track[0]) gx = fresh(x.sizes(), x);
+        const auto params = call.p.weight_dtype == call.p.dtype ? x.scalar_type() : kFloat;
+        if (track[1]) gw = fresh({call.p.width}, params, x);
+        if (track[2]) gb = fresh({call.p.width}, params, x);
         grads.grad_x = gx.defined() ? gx.data_ptr() : nullptr;
         grads.grad_weight = gw.defined() ? gw.data_ptr() : nullptr;
         grads.grad_bias = gb.defined() ? gb.data_ptr() : nullptr;
         if (track[1] || track[2])
-            workspace = bytes_like(x, warpctct_layer_norm_workspace_bytes(call.p.rows, call.p.width));
+            workspace = fresh_bytes(warpctct_layer_norm_workspace_bytes(call.p.rows, call.p.width), x);
         check_rc(warpctct_layer_norm_grad(&call.p, &grads, workspace.defined() ? workspace.data_ptr() : nullptr,
                                           workspace.defined() ? workspace.numel() : 0, current_stream()),
                  "layer_norm");
@@ -193,7 +202,8 @@ torch::Tensor layer_norm(const torch::Tensor &input, Maybe weight, Maybe bias, c
         same = same && (*p)->scalar_type() == x.scalar_type();
     }
     for (Maybe *p : {&weight, &bias})
-        if (given(*p)) *p = (same ? **p : (*p)->to(at::ScalarType::Float)).contiguous();
+        if (given(*p) && !((same || (*p)->scalar_type() == kFloat) && (*p)->is_contiguous()))
+            *p = (same ? **p : (*p)->to(kFloat)).contiguous();
     const bool tx = tracked(x), tw = tracked(weight), tb = tracked(bias);
     if (tx || tw || tb) return LayerNorm::apply(x, weight, bias, eps, tx, tw, tb);
     NormCall call(x, given(weight) ? *weight : torch::Tensor(), given(bias) ? *bias : torch::Tensor(), eps);
@@ -261,8 +271,8 @@ tensor_list conv_forward(const ConvInputs &in, bool silu, bool want_state) {
     const DeviceGuard guard(device_of(in.x));
     auto p = in.call();
     p.silu = silu ? 1 : 0;
-    tensor_list outs = {torch::empty(in.x.sizes(), in.x.options())};
-    if (want_state) outs.push_back(torch::empty({p.N, p.K - 1, p.E}, in.x.options()));
+    tensor_list outs = {fresh(in.x.sizes(), in.x)};
+    if (want_state) outs.push_back(fresh({p.N, p.K - 1, p.E}, in.x));
     p.out = outs[0].data_ptr();
     p.last = want_state ? outs[1].data_ptr() : nullptr;
     check_rc(warpctct_causal_conv(&p, current_stream()), "causal_conv");
@@ -296,13 +306,12 @@ class CausalConv : public torch::autograd::Function<CausalConv> {
                                                            : torch::zeros(in.x.sizes(), in.x.options());
         torch::Tensor glast;
         if (grad_outputs.size() > 1 && grad_outputs[1].defined()) glast = grad_outputs[1].contiguous();
-        const auto f32 = in.x.options().dtype(at::ScalarType::Float);
-        torch::Tensor gx = torch::empty(in.x.sizes(), in.x.options()), gw, gb, ginitial, workspace;
-        if (track[0]) gw = torch::empty({p.E, p.K}, f32);
-        if (track[1]) gb = torch::empty({p.E}, f32);
-        if (track[2]) ginitial = torch::empty(in.initial.sizes(), in.x.options());
+        torch::Tensor gx = fresh(in.x.sizes(), in.x), gw, gb, ginitial, workspace;
+        if (track[0]) gw = fresh({p.E, p.K}, kFloat, in.x);
+        if (track[1]) gb = fresh({p.E}, kFloat, in.x);
+        if (track[2]) ginitial = fresh(in.initial.sizes(), in.x);
         if (track[0] || track[1])
-            workspace = bytes_like(in.x, warpctct_causal_conv_workspace_bytes(p.N, p.L, p.E, p.K));
+            workspace = fresh_bytes(warpctct_causal_conv_workspace_bytes(p.N, p.L, p.E, p.K), in.x);
         warpctct_conv_grad_t g = {};
         g.grad_n = up.stride(0);
         g.grad_t = up.stride(1);
@@ -331,7 +340,9 @@ void check_taps(const torch::Tensor &weight, const Maybe &bias, const torch::Ten
     TORCH_CHECK(bias->dim() == 1 && bias->size(0) == x.size(-1), what, ": bias must have one element a channel");
     check_on(*bias, x, "bias");
 }
-torch::Tensor as_float(const torch::Tensor &t) { return t.to(at::ScalarType::Float).contiguous(); }
+torch::Tensor as_float(const torch::Tensor &t) {
+    return t.scalar_type() == kFloat && t.is_contiguous() ? t : t.to(kFloat).contiguous();
+}
 
 tensor_list causal_conv(const torch::Tensor &input, const torch::Tensor &weight, const Maybe &bias,
                         const Maybe &lengths, const Maybe &initial, const bool silu, const bool want_state) {
@@ -374,7 +385,7 @@ torch::Tensor causal_conv_step(const torch::Tensor &input, torch::Tensor state, 
     const torch::Tensor go = flags_of(advance, x, "causal_conv_step");
     const torch::Tensor w = as_float(weight), b = given(bias) ? as_float(*bias) : torch::Tensor();
     const DeviceGuard guard(device_of(x));
-    auto out = torch::empty(x.sizes(), x.options());
+    auto out = fresh(x.sizes(), x);
     warpctct_conv_step_t p = {};
     p.dtype = type_of(x);
     p.N = int_size(x, 0, "causal_conv_step");
@@ -438,16 +449,16 @@ std::tuple<tensor_list, torch::Tensor> scan_forward(const ScanInputs &in, bool s
     const DeviceGuard guard(device_of(in.x));
     auto p = in.call();
     p.softplus = softplus ? 1 : 0;
-    tensor_list outs = {torch::empty(in.x.sizes(), in.x.options())};
+    tensor_list outs = {fresh(in.x.sizes(), in.x)};
     if (want_state)
-        outs.push_back(torch::empty({p.N, p.E, p.S}, in.x.options().dtype(at::ScalarType::Float)));
+        outs.push_back(fresh({p.N, p.E, p.S}, kFloat, in.x));
     p.out = outs[0].data_ptr();
     p.last = want_state ? floats(outs[1]) : nullptr;
     torch::Tensor keep;
-    if (for_backward) keep = bytes_like(in.x, warpctct_selective_scan_keep_bytes(p.N, p.L, p.E, p.S));
+    if (for_backward) keep = fresh_bytes(warpctct_selective_scan_keep_bytes(p.N, p.L, p.E, p.S), in.x);
     const size_t scratch = warpctct_selective_scan_workspace_bytes(p.N, p.L, p.E, p.S, p.G, 0);
     torch::Tensor workspace;
-    if (scratch > 0) workspace = bytes_like(in.x, scratch);
+    if (scratch > 0) workspace = fresh_bytes(scratch, in.x);
     check_rc(warpctct_selective_scan(&p, keep.defined() ? keep.data_ptr() : nullptr, keep.defined() ? keep.numel() : 0,
                                      workspace.defined() ? workspace.data_ptr() : nullptr, scratch, current_stream()),
              "selective_scan");
@@ -485,13 +496,14 @@ class SelectiveScan : public torch::autograd::Function<SelectiveScan> {
             grad_outputs[0].defined() ? dense_last(grad_outputs[0]) : torch::zeros(x.sizes(), x.options());
         torch::Tensor glast;
         if (grad_outputs.size() > 1 && grad_outputs[1].defined()) glast = grad_outputs[1].contiguous();
-        const auto f32 = x.options().dtype(at::ScalarType::Float);
-        torch::Tensor gx = torch::empty(x.sizes(), x.options()), gdt = torch::empty(x.sizes(), x.options()), gz,
-                      gb = torch::empty(in.b.sizes(), x.options()), gc = torch::empty(in.c.sizes(), x.options()),
-                      ga = torch::empty({p.E, p.S}, f32), two = torch::empty({2, p.E}, f32), ginitial;
-        if (in.gate.defined()) gz = torch::empty(x.sizes(), x.options());
-        if (ctx->saved_data["track_initial"].toBool()) ginitial = torch::empty({p.N, p.E, p.S}, f32);
-        auto workspace = bytes_like(x, warpctct_selective_scan_workspace_bytes(p.N, p.L, p.E, p.S, p.G, 1));
+        torch::Tensor gx = fresh(x.sizes(), x), gdt = fresh(x.sizes(), x), gb = fresh(in.b.sizes(), x),
+                      gc = fresh(in.c.sizes(), x), ga = fresh({p.E, p.S}, kFloat, x), gz, gskip, gbias, ginitial;
+        if (in.gate.defined()) gz = fresh(x.sizes(), x);
+        if (in.skip.defined()) gskip = fresh({p.E}, kFloat, x);
+        if (in.dt_bias.defined()) gbias = fresh({p.E}, kFloat, x);
+        if (ctx->saved_data["track_initial"].toBool()) ginitial = fresh({p.N, p.E, p.S}, kFloat, x);
+        const auto workspace =
+            fresh_bytes(warpctct_selective_scan_workspace_bytes(p.N, p.L, p.E, p.S, p.G, 1), x);
         warpctct_scan_grad_t g = {};
         g.grad_n = up.stride(0);
         g.grad_t = up.stride(1);
@@ -503,14 +515,14 @@ class SelectiveScan : public torch::autograd::Function<SelectiveScan> {
         g.grad_b = gb.data_ptr();
         g.grad_c = gc.data_ptr();
         g.grad_a = floats(ga);
-        g.grad_skip_bias = floats(two);
+        g.grad_skip = floats(gskip);
+        g.grad_dt_bias = floats(gbias);
         g.grad_initial = floats(ginitial);
         check_rc(warpctct_selective_scan_grad(&p, &g, keep.data_ptr(), keep.numel(), workspace.data_ptr(),
                                               workspace.numel(), current_stream()),
                  "selective_scan");
-        return {gx, gdt, ga, gb, gc, in.skip.defined() ? two.select(0, 0) : torch::Tensor(), gz,
-                in.dt_bias.defined() ? two.select(0, 1) : torch::Tensor(), ginitial, torch::Tensor(),
-                torch::Tensor(), torch::Tensor(), torch::Tensor()};
+        return {gx, gdt, ga, gb, gc, gskip, gz, gbias, ginitial, torch::Tensor(), torch::Tensor(), torch::Tensor(),
+                torch::Tensor()};
     }
 };
 
@@ -613,7 +625,7 @@ torch::Tensor selective_scan_step(const torch::Tensor &input, torch::Tensor stat
     check_on(state, x, "state");
     const torch::Tensor go = flags_of(advance, x, what);
     const DeviceGuard guard(device_of(x));
-    auto out = torch::empty(x.sizes(), x.options());
+    auto out = fresh(x.sizes(), x);
     warpctct_scan_step_t p = {};
     p.dtype = type_of(x);
     p.N = int_size(x, 0, what);
@@ -659,7 +671,7 @@ struct Penalty {
                     " must be a number or one for each row");
         check_on(t, logits, name);
         refuse_if_tracked(t, name);
-        each = t.to(at::ScalarType::Float).contiguous();
+        each = t.scalar_type() == kFloat && t.is_contiguous() ? t : t.to(kFloat).contiguous();
     }
     static void refuse_if_tracked(const torch::Tensor &t, const char *name) {
         TORCH_CHECK(!tracked(t), "adjust_logits: not differentiable (", name, "); call it under torch.no_grad()");
@@ -733,7 +745,7 @@ torch::Tensor adjust_logits(const torch::Tensor &input, const Maybe &tokens, con
         p.allowed = mask.data_ptr();
     }
     const DeviceGuard guard(device_of(x));
-    auto out = torch::empty(x.sizes(), x.options());
+    auto out = fresh(x.sizes(), x);
     p.out = out.data_ptr();
     check_rc(warpctct_adjust_logits(&p, current_stream()), "adjust_logits");
     return out;

@@ -27,9 +27,8 @@ __device__ __forceinline__ void store_as(void *p, int type, int at, float v) {
 }
 
 __global__ __launch_bounds__(64 * kStrands) void column_sums_kernel(const float *__restrict__ partial, long rows,
-                                                                    int columns, int split,
-                                                                    void *__restrict__ first, int first_type,
-                                                                    void *__restrict__ second, int second_type) {
+                                                                    int columns, SumsTo first, SumsTo second,
+                                                                    SumsTo third) {
     __shared__ float strands[kStrands][64];
     const int lane = threadIdx.x & 63, strand = threadIdx.x >> 6, k = blockIdx.x * 64 + lane;
     // the rows of this part (all of them where gridDim.y is 1)
@@ -45,11 +44,16 @@ __global__ __launch_bounds__(64 * kStrands) void column_sums_kernel(const float 
     if (strand != 0 || k >= columns) return;
     for (int s = 1; s < kStrands; ++s) sum += strands[s][lane];
     if (gridDim.y > 1) {
-        static_cast<float *>(first)[(long)blockIdx.y * columns + k] = sum;
-    } else if (k < split) {
-        if (first) store_as(first, first_type, k, sum);
-    } else if (second) {
-        store_as(second, second_type, k - split, sum);
+        static_cast<float *>(first.p)[(long)blockIdx.y * columns + k] = sum;
+        return;
+    }
+    const int j = k - first.count;
+    if (j < 0) {
+        if (first.p) store_as(first.p, first.type, k, sum);
+    } else if (j < second.count) {
+        if (second.p) store_as(second.p, second.type, j, sum);
+    } else if (third.p) {
+        store_as(third.p, third.type, j - second.count, sum);
     }
 }
 
@@ -59,18 +63,20 @@ size_t column_sums_floats(long rows, long columns) {
     return (size_t)(rows > kDirect ? rows + kParts : rows) * (size_t)columns;
 }
 
-hipError_t launch_column_sums(float *partial, long rows, int columns, int split, void *first, int first_type,
-                              void *second, int second_type, hipStream_t stream) {
+hipError_t launch_column_sums(float *partial, long rows, SumsTo first, SumsTo second, SumsTo third,
+                              hipStream_t stream) {
+    const int columns = first.count + second.count + third.count;
     const unsigned groups = (columns + 63) / 64;
     if (rows > kDirect) {
         float *fewer = partial + (size_t)rows * columns;
+        const SumsTo all = {fewer, columns, kIoF32}, none = {};
         TIMED_LAUNCH(column_sums_kernel, dim3(groups, kParts), dim3(64 * kStrands), 0, stream, partial, rows,
-                     columns, columns, fewer, kIoF32, nullptr, kIoF32);
+                     columns, all, none, none);
         partial = fewer;
         rows = kParts;
     }
-    TIMED_LAUNCH(column_sums_kernel, dim3(groups), dim3(64 * kStrands), 0, stream, partial, rows, columns, split,
-                 first, first_type, second, second_type);
+    TIMED_LAUNCH(column_sums_kernel, dim3(groups), dim3(64 * kStrands), 0, stream, partial, rows, columns, first,
+                 second, third);
     return hipGetLastError();
 }
 

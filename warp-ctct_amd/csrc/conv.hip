@@ -375,8 +375,8 @@ hipError_t launch_conv_grad(const warpctct_conv_t &p, const warpctct_conv_grad_t
     if (p.N > 0) e = by_type(p.dtype, p.K, p, g, partial, stream);
     if (e != hipSuccess || !(g.grad_weight || g.grad_bias)) return e;
     // (of no sequences the sums are zero: the launch reads nothing then)
-    return launch_column_sums(partial, (long)p.N * conv_grad_tiles(p.N, p.L, p.E), p.E * (p.K + 1), p.E * p.K,
-                              g.grad_weight, kIoF32, g.grad_bias, kIoF32, stream);
+    return launch_column_sums(partial, (long)p.N * conv_grad_tiles(p.N, p.L, p.E), {g.grad_weight, p.E * p.K, kIoF32},
+                              {g.grad_bias, p.E, kIoF32}, {}, stream);
 }
 
 hipError_t launch_conv_step(const warpctct_conv_step_t &p, hipStream_t stream) {

@@ -17,14 +17,19 @@ int norm_grad_groups(long rows, int width);
 hipError_t launch_layer_norm_grad(const warpctct_norm_t &p, const warpctct_norm_grad_t &g,
                                   float *partial, hipStream_t stream);
 
-// out[column] = sum over `rows` rows of partial (rows, columns), in a fixed
-// order; the first `split` columns go to `first`, the others to `second`, in
-// the element type given for each (either pointer may be null).  `partial`
-// holds column_sums_floats(rows, columns) floats: the rows, and behind them room
-// for a second level where there are many.
+// Where the sums of a run of columns go: `count` of them in an element type, or
+// nowhere (null).
+struct SumsTo {
+    void *p;
+    int count, type;
+};
+// Sums down `rows` rows of partial (rows, columns), in a fixed order; the columns
+// are those of to[0], then to[1], then to[2].  `partial` holds
+// column_sums_floats(rows, columns) floats: the rows, and behind them room for a
+// second level where there are many.
 size_t column_sums_floats(long rows, long columns);
-hipError_t launch_column_sums(float *partial, long rows, int columns, int split, void *first,
-                              int first_type, void *second, int second_type, hipStream_t stream);
+hipError_t launch_column_sums(float *partial, long rows, SumsTo first, SumsTo second, SumsTo third,
+                              hipStream_t stream);
 
 hipError_t launch_conv(const warpctct_conv_t &p, hipStream_t stream);
 // tiles of time that a sequence is cut into by the backward pass, each of which

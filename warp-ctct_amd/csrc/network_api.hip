@@ -70,8 +70,8 @@ int warpctct_layer_norm_grad(const warpctct_norm_t *p, const warpctct_norm_grad_
     float *partial = columns ? static_cast<float *>(workspace) : nullptr;
     if (p->rows == 0) {     // the sums of no rows: zeros
         if (!columns) return WARPCTCT_OK;
-        return done(launch_column_sums(partial, 0, 2 * p->width, p->width, g->grad_weight, p->weight_dtype,
-                                       g->grad_bias, p->weight_dtype, as_stream(stream)));
+        return done(launch_column_sums(partial, 0, {g->grad_weight, p->width, p->weight_dtype},
+                                       {g->grad_bias, p->width, p->weight_dtype}, {}, as_stream(stream)));
     }
     if (!g->grad_x && !columns) return WARPCTCT_OK;
     return done(launch_layer_norm_grad(*p, *g, partial, as_stream(stream)));
@@ -150,7 +150,7 @@ int warpctct_selective_scan(const warpctct_scan_t *p, void *keep, size_t keep_by
 
 int warpctct_selective_scan_grad(const warpctct_scan_t *p, const warpctct_scan_grad_t *g, const void *keep,
                                  size_t keep_bytes, void *workspace, size_t workspace_bytes, void *stream) {
-    if (!scan_ok(p) || !g || !g->grad_a || !g->grad_skip_bias) return WARPCTCT_EINVAL;
+    if (!scan_ok(p) || !g || !g->grad_a) return WARPCTCT_EINVAL;
     if (p->N > 0 && p->L > 0 &&
         (!g->grad_out || !g->grad_x || !g->grad_dt || !g->grad_b || !g->grad_c || (p->gate && !g->grad_gate) || !keep ||
          !workspace))

@@ -95,10 +95,7 @@ struct Slots {
         for (int j = 0; j < NV; ++j) {
             const int at = first(j, t, threads);
             if (at < width) {
-                if (VEC)
-                    store_vec(row + at, x + j * EV);
-                else
-                    row[at] = from_float<IO>(x[j]);
+                store_n<EV>(row + at, x + j * EV);
             }
         }
     }
@@ -461,8 +458,8 @@ hipError_t launch_layer_norm_grad(const warpctct_norm_t &p, const warpctct_norm_
     else
         e = same ? start_grad<bf16, bf16>(p, g, partial, stream) : start_grad<bf16, float>(p, g, partial, stream);
     if (e != hipSuccess || !partial) return e;
-    return launch_column_sums(partial, norm_grad_groups(p.rows, p.width), 2 * p.width, p.width, g.grad_weight,
-                              p.weight_dtype, g.grad_bias, p.weight_dtype, stream);
+    return launch_column_sums(partial, norm_grad_groups(p.rows, p.width), {g.grad_weight, p.width, p.weight_dtype},
+                              {g.grad_bias, p.width, p.weight_dtype}, {}, stream);
 }
 
 }  // namespace wctct

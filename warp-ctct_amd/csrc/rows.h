@@ -21,29 +21,6 @@ __device__ __forceinline__ float to_float(IO v) { return (float)v; }
 template <typename IO>
 __device__ __forceinline__ IO from_float(float v) { return (IO)v; }
 
-template <typename IO>
-__device__ __forceinline__ raw16 load16(const IO *p) { return *reinterpret_cast<const raw16 *>(p); }
-
-__device__ __forceinline__ void unpack16(const float *, raw16 v, float *x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(v[i]);
-}
-__device__ __forceinline__ void unpack16(const f16 *, raw16 v, float *x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const unsigned word = v[i];
-        x[2 * i] = (float)__builtin_bit_cast(f16, (unsigned short)(word & 0xffffu));
-        x[2 * i + 1] = (float)__builtin_bit_cast(f16, (unsigned short)(word >> 16));
-    }
-}
-__device__ __forceinline__ void unpack16(const bf16 *, raw16 v, float *x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = __uint_as_float(v[i] << 16);
-        x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
-    }
-}
-
 // two floats rounded to nearest even into one word of 2-byte elements
 __device__ __forceinline__ unsigned pack_two(const f16 *, float a, float b) {
     typedef float f2 __attribute__((ext_vector_type(2)));
@@ -64,28 +41,16 @@ __device__ __forceinline__ raw16 pack16(const IO *p, const float *x) {
     return raw16{pack_two(p, x[0], x[1]), pack_two(p, x[2], x[3]), pack_two(p, x[4], x[5]),
                  pack_two(p, x[6], x[7])};
 }
-template <typename IO>
-__device__ __forceinline__ void load_vec(const IO *p, float *x) { unpack16(p, load16(p), x); }
-template <typename IO>
-__device__ __forceinline__ void store_vec(IO *p, const float *x) {
-    *reinterpret_cast<raw16 *>(p) = pack16(p, x);
-}
-
-// N elements next to each other, N * sizeof(IO) bytes aligned to themselves:
-// 1 element, 4 elements, or a 16-byte vector
+// N elements next to each other (1, 2, 4, or a 16-byte vector), aligned to their size
 template <int N, typename IO>
 __device__ __forceinline__ void load_n(const IO *p, float *x) {
     if constexpr (N == 1) {
         x[0] = to_float(*p);
-    } else if constexpr (N == kVec<IO>) {
-        load_vec(p, x);
     } else {
-        static_assert(N == 4 && sizeof(IO) == 2, "half a vector of 2-byte elements");
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        float y[8];
-        unpack16(p, raw16{v.x, v.y, 0u, 0u}, y);
+        typedef IO piece __attribute__((ext_vector_type(N)));
+        const piece v = *reinterpret_cast<const piece *>(p);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = y[i];
+        for (int i = 0; i < N; ++i) x[i] = (float)v[i];
     }
 }
 template <int N, typename IO>
@@ -93,10 +58,18 @@ __device__ __forceinline__ void store_n(IO *p, const float *x) {
     if constexpr (N == 1) {
         *p = from_float<IO>(x[0]);
     } else if constexpr (N == kVec<IO>) {
-        store_vec(p, x);
-    } else {
-        static_assert(N == 4 && sizeof(IO) == 2, "half a vector of 2-byte elements");
+        *reinterpret_cast<raw16 *>(p) = pack16(p, x);
+    } else if constexpr (sizeof(IO) == 4) {
+        typedef IO piece __attribute__((ext_vector_type(N)));
+        piece v;
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = x[i];
+        *reinterpret_cast<piece *>(p) = v;
+    } else if constexpr (N == 4) {
         *reinterpret_cast<uint2 *>(p) = make_uint2(pack_two(p, x[0], x[1]), pack_two(p, x[2], x[3]));
+    } else {
+        static_assert(N == 2, "1, 2, 4 elements or a vector");
+        *reinterpret_cast<unsigned *>(p) = pack_two(p, x[0], x[1]);
     }
 }
 

@@ -763,55 +763,74 @@ __global__ __launch_bounds__(kThreads) void scan_grad_bc_kernel(warpctct_scan_t 
     to[((long)n * p.L + t) * GS + v] = from_float<IO>(sum);
 }
 
-// One step of N sequences; a channel lies on kLanes lanes.
-template <typename IO, int LANES>
-__global__ __launch_bounds__(kThreads) void scan_step_kernel(warpctct_scan_step_t p) {
-    const long i0 = ((long)blockIdx.x * kThreads + threadIdx.x) / LANES;
-    if (i0 >= (long)p.N * p.E) return;             // all lanes of a channel
-    const int n = (int)(i0 / p.E), e = (int)(i0 - (long)n * p.E), q = threadIdx.x % LANES;
-    IO *out = static_cast<IO *>(p.out) + (long)n * p.E + e;
-    if (p.advance && !p.advance[n]) {
-        if (q == 0) *out = from_float<IO>(0.0f);
-        return;
-    }
-    const float x = to_float(static_cast<const IO *>(p.x)[(long)n * p.x_n + e]);
-    float d = to_float(static_cast<const IO *>(p.dt)[(long)n * p.dt_n + e]) + (p.dt_bias ? p.dt_bias[e] : 0.0f);
-    if (p.softplus) d = softplus(d).value;
-    const int grp = e / (p.E / p.G);
-    const IO *b = static_cast<const IO *>(p.b) + (long)n * p.b_n + (long)grp * p.b_g + q * kStates;
-    const IO *c = static_cast<const IO *>(p.c) + (long)n * p.c_n + (long)grp * p.c_g + q * kStates;
-    float *h = p.state + i0 * p.S + q * kStates;
-    const float *a = p.a + (long)e * p.S + q * kStates;
-    const float dx = d * x;
-    float y = 0.0f;
-    if (p.S == kStates * LANES && (reinterpret_cast<uintptr_t>(p.state) & 15u) == 0 &&
-        (reinterpret_cast<uintptr_t>(p.a) & 15u) == 0) {
-        const float4 h4 = *reinterpret_cast<const float4 *>(h), a4 = *reinterpret_cast<const float4 *>(a);
-        float hv[4] = {h4.x, h4.y, h4.z, h4.w};
-        const float av[4] = {a4.x, a4.y, a4.z, a4.w};
+// One step of N sequences; a channel lies on kLanes lanes, and a thread takes its
+// four states of `BATCH` sequences, so that a is read once for them.  wide: b, c,
+// a and the states in pieces of four.
+template <typename IO, int LANES, int BATCH>
+__global__ __launch_bounds__(kThreads) void scan_step_kernel(warpctct_scan_step_t p, bool wide) {
+    const long i0 = (long)blockIdx.x * kThreads + threadIdx.x;
+    if (i0 >= (long)p.E * LANES) return;           // all lanes of a channel
+    const int e = (int)(i0 / LANES), q = threadIdx.x % LANES, s0 = q * kStates, grp = e / (p.E / p.G);
+    const int most = max(min(kStates, p.S - s0) - 1, 0), s1 = min(s0, p.S - 1);
+    const float *ap = p.a + (long)e * p.S + s1;
+    float a[kStates];
+    Raw<float, kStates> ar;
+    ar.load(ap, wide, most);
 #pragma unroll
-        for (int i = 0; i < kStates; ++i) {
-            hv[i] = fmaf(exp2_hw(d * (av[i] * kLog2e)), hv[i], dx * to_float(b[i]));
-            y = fmaf(to_float(c[i]), hv[i], y);
-        }
-        *reinterpret_cast<float4 *>(h) = make_float4(hv[0], hv[1], hv[2], hv[3]);
-    } else {
+    for (int i = 0; i < kStates; ++i) a[i] = ar[i] * kLog2e;
+    const float bias = p.dt_bias ? p.dt_bias[e] : 0.0f, skip = p.skip ? p.skip[e] : 0.0f;
+    for (long n0 = (long)blockIdx.y * BATCH; n0 < p.N; n0 += (long)gridDim.y * BATCH) {
+        Raw<float, kStates> h[BATCH];
+        Raw<IO, kStates> b[BATCH], c[BATCH];
+        IO x[BATCH], d[BATCH], z[BATCH];
+        bool go[BATCH];
 #pragma unroll
-        for (int i = 0; i < kStates; ++i) {
-            if (q * kStates + i >= p.S) continue;
-            const float hv = fmaf(exp2_hw(d * (a[i] * kLog2e)), h[i], dx * to_float(b[i]));
-            y = fmaf(to_float(c[i]), hv, y);
-            h[i] = hv;
+        for (int k = 0; k < BATCH; ++k) {
+            const long n = min(n0 + k, (long)p.N - 1);
+            // (the same for the whole workgroup: a sequence that stays is not read)
+            go[k] = __builtin_amdgcn_readfirstlane(n0 + k < p.N && (!p.advance || p.advance[n]));
+            if (!go[k]) continue;
+            h[k].load(p.state + (n * p.E + e) * p.S + s1, wide, most);
+            b[k].load(static_cast<const IO *>(p.b) + n * p.b_n + grp * p.b_g + s1, wide, most);
+            c[k].load(static_cast<const IO *>(p.c) + n * p.c_n + grp * p.c_g + s1, wide, most);
+            x[k] = static_cast<const IO *>(p.x)[n * p.x_n + e];
+            d[k] = static_cast<const IO *>(p.dt)[n * p.dt_n + e];
+            if (p.gate) z[k] = static_cast<const IO *>(p.gate)[n * p.gate_n + e];
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+            if (n0 + k >= p.N) break;
+            IO *out = static_cast<IO *>(p.out) + (n0 + k) * p.E + e;
+            if (!go[k]) {
+                if (q == 0) *out = from_float<IO>(0.0f);
+                continue;
+            }
+            const float xv = to_float(x[k]);
+            float dv = to_float(d[k]) + bias;
+            if (p.softplus) dv = softplus(dv).value;
+            const float dx = dv * xv;
+            float y = 0.0f, hv[kStates];
+#pragma unroll
+            for (int i = 0; i < kStates; ++i) {
+                hv[i] = fmaf(exp2_hw(dv * a[i]), h[k][i], dx * b[k][i]);
+                y = s0 + i < p.S ? fmaf(c[k][i], hv[i], y) : y;
+            }
+            float *to = p.state + ((n0 + k) * p.E + e) * p.S + s0;
+            if (wide) {
+                store_n<kStates>(to, hv);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kStates; ++i)
+                    if (s0 + i < p.S) to[i] = hv[i];
+            }
+            y = fmaf(skip, xv, channel_sum<LANES>(y));
+            if (p.gate) {
+                const float zv = to_float(z[k]);
+                y *= zv * sigmoid(zv);
+            }
+            if (q == 0) *out = from_float<IO>(y);
         }
     }
-    y = channel_sum<LANES>(y);
-    if (q != 0) return;
-    if (p.skip) y = fmaf(p.skip[e], x, y);
-    if (p.gate) {
-        const float z = to_float(static_cast<const IO *>(p.gate)[(long)n * p.gate_n + e]);
-        y *= z * sigmoid(z);
-    }
-    *out = from_float<IO>(y);
 }
 
 // steps, rounded up to whole tiles of the backward pass
@@ -931,12 +950,23 @@ hipError_t start(const warpctct_scan_t &p, const warpctct_scan_grad_t &g, const 
     return hipGetLastError();
 }
 
+template <typename IO, int LANES, int BATCH>
+hipError_t start_step(const warpctct_scan_step_t &p, hipStream_t stream) {
+    const long groups = ((long)p.E * LANES + kThreads - 1) / kThreads, batches = ((long)p.N + BATCH - 1) / BATCH;
+    const size_t four = kStates * sizeof(IO);
+    const bool wide = p.S == kStates * LANES && aligned16(p.state) && aligned16(p.a) && p.b_n % kStates == 0 &&
+                      p.b_g % kStates == 0 && p.c_n % kStates == 0 && p.c_g % kStates == 0 &&
+                      (reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.c)) % four == 0;
+    auto kernel = scan_step_kernel<IO, LANES, BATCH>;
+    TIMED_LAUNCH(kernel, dim3((unsigned)groups, (unsigned)std::min(batches, 65535L)), dim3(kThreads), 0, stream, p,
+                 wide);
+    return hipGetLastError();
+}
 template <typename IO, int LANES>
 hipError_t start(const warpctct_scan_step_t &p, hipStream_t stream) {
-    const long threads = (long)p.N * p.E * LANES;
-    auto kernel = scan_step_kernel<IO, LANES>;
-    TIMED_LAUNCH(kernel, dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, p);
-    return hipGetLastError();
+    // two sequences a thread once there are eight workgroups a compute unit with them
+    const long groups = ((long)p.E * LANES + kThreads - 1) / kThreads * p.N;
+    return groups >= 4096 ? start_step<IO, LANES, 2>(p, stream) : start_step<IO, LANES, 1>(p, stream);
 }
 
 template <typename IO, typename... Args>
@@ -985,9 +1015,8 @@ hipError_t launch_scan_grad(const warpctct_scan_t &p, const warpctct_scan_grad_t
     float *part_bc = workspace, *local = part_bc + part_bc_floats(p), *part_sums = local + chunk_floats(p, true);
     const hipError_t e = by_type(p.dtype, p.S, p, g, keep, part_bc, part_sums, local, stream);
     if (e != hipSuccess) return e;
-    // (the skip's and the bias's gradients lie next to each other)
-    return launch_column_sums(part_sums, (long)p.N * cut_of(p, true).count, p.E * (p.S + 2), p.E * p.S, g.grad_a, kIoF32,
-                              g.grad_skip_bias, kIoF32, stream);
+    return launch_column_sums(part_sums, (long)p.N * cut_of(p, true).count, {g.grad_a, p.E * p.S, kIoF32},
+                              {g.grad_skip, p.E, kIoF32}, {g.grad_dt_bias, p.E, kIoF32}, stream);
 }
 
 hipError_t launch_scan_step(const warpctct_scan_step_t &p, hipStream_t stream) {
