@@ -192,22 +192,22 @@ struct Sides {
     __device__ __forceinline__ void advance(int steps) { at += steps * stride; }
 };
 
-// A thread's elements of x, dt, gate or grad_out, tile after tile.  Where it has
-// none it reads row `safe`, or the workgroup's first channels, and masks what it
-// makes of them.
+// A thread's elements of x, dt, gate or grad_out, tile after tile, from a row that
+// counts.  In the tile that ends the sequence some threads have none: they are
+// shifted onto its last row for that load, and mask what they make of it, as do
+// threads past the workgroup's channels, which read its first ones.
 template <typename IO, int EPT>
 struct Column {
-    const IO *at, *safe;
+    const IO *at;
     long stride;
-    __device__ __forceinline__ Column(const void *base, long start, long t_stride, long row, int safe_row) {
-        const IO *p = static_cast<const IO *>(base) + start;
+    __device__ __forceinline__ Column(const void *base, long start, long t_stride, long row) {
         stride = t_stride;
-        at = p + row * stride;
-        safe = p + safe_row * stride;
+        at = static_cast<const IO *>(base) + start + row * stride;
     }
+    __device__ __forceinline__ void shift(long rows) { at += rows * stride; }
     // the present row, and on by `steps`
-    __device__ __forceinline__ void next(Raw<IO, EPT> &v, bool on, bool wide, int most, int steps) {
-        v.load(on ? at : safe, wide, most);
+    __device__ __forceinline__ void next(Raw<IO, EPT> &v, bool wide, int most, int steps) {
+        v.load(at, wide, most);
         at += steps * stride;
     }
 };
@@ -309,18 +309,23 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
     const int el0 = have > 0 ? e0 : w.first, most = max(have - 1, 0), t1 = w.from + el.j;
     const bool gated = !CARRY && p.gate;
     typedef Raw<IO, EPT> Row;
-    Column<IO, EPT> xs(p.x, (long)w.n * p.x_n + el0, p.x_t, t1, w.from);
-    Column<IO, EPT> ds(p.dt, (long)w.n * p.dt_n + el0, p.dt_t, t1, w.from);
-    Column<IO, EPT> zs(p.gate, (long)w.n * p.gate_n + el0, p.gate_t, t1, w.from);
+    Column<IO, EPT> xs(p.x, (long)w.n * p.x_n + el0, p.x_t, t1);
+    Column<IO, EPT> ds(p.dt, (long)w.n * p.dt_n + el0, p.dt_t, t1);
+    Column<IO, EPT> zs(p.gate, (long)w.n * p.gate_n + el0, p.gate_t, t1);
     IO *out = static_cast<IO *>(p.out) + ((long)w.n * p.L + t1) * p.E + e0;
     typedef Sides<IO, LANES, kSteps> Side;
     Side sides(p, w, w.from, w.from);
     Row x, d, z;
     auto request = [&](int t0) {
-        const bool on = t0 + el.j < w.to;
-        xs.next(x, on, wide, most, kSteps);
-        ds.next(d, on, wide, most, kSteps);
-        if (gated) zs.next(z, on, wide, most, kSteps);
+        if (t0 + kSteps > w.to) {       // the last tile
+            const long past = min(w.to - 1 - t0 - el.j, 0);
+            xs.shift(past);
+            ds.shift(past);
+            zs.shift(past);
+        }
+        xs.next(x, wide, most, kSteps);
+        ds.next(d, wide, most, kSteps);
+        if (gated) zs.next(z, wide, most, kSteps);
         sides.load(t0, w.len);
         sides.advance(kSteps);
     };
@@ -460,7 +465,8 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     const Place w = place_of<LANES>(p, chunk_tiles);
     const Elements<LANES, STEPS> el;
     const int ch = threadIdx.x / LANES, q = threadIdx.x % LANES, e = w.first + ch;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row16 = lane >> 4;
+    const int s_at = q * kStates + (row16 & 1) * 2 + (row16 >> 1);      // see sum_over_channels
     const bool live = e < w.end;
     const int tiles = (p.L + STEPS - 1) / STEPS;
     float a[kStates], carry[kStates], ga[kStates];
@@ -501,10 +507,11 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     const int el0 = have > 0 ? e0 : w.first, most = max(have - 1, 0);
     const bool gated = p.gate;
     typedef Raw<IO, EPT> Row;
-    Column<IO, EPT> xs(p.x, (long)w.n * p.x_n + el0, p.x_t, t1, w.from);
-    Column<IO, EPT> ds(p.dt, (long)w.n * p.dt_n + el0, p.dt_t, t1, w.from);
-    Column<IO, EPT> zs(p.gate, (long)w.n * p.gate_n + el0, p.gate_t, t1, w.from);
-    Column<IO, EPT> us(g.grad_out, (long)w.n * g.grad_n + el0, g.grad_t, t1, w.from);
+    const long past = max(t1 - (w.to - 1), 0L);      // rows from the last one that counts
+    Column<IO, EPT> xs(p.x, (long)w.n * p.x_n + el0, p.x_t, t1 - past);
+    Column<IO, EPT> ds(p.dt, (long)w.n * p.dt_n + el0, p.dt_t, t1 - past);
+    Column<IO, EPT> zs(p.gate, (long)w.n * p.gate_n + el0, p.gate_t, t1 - past);
+    Column<IO, EPT> us(g.grad_out, (long)w.n * g.grad_n + el0, g.grad_t, t1 - past);
     const float *fronts = keep + (((long)w.n * tiles + top) * p.E + (live ? e : w.first)) * SP + q * kStates;
     long row = t1 * p.E;         // of the tile that is written next
     typedef Sides<IO, LANES, STEPS> Side;
@@ -512,17 +519,22 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     Row x, raw, z, u;
     float4 front;
     auto request = [&](int tile) {
-        const bool on = tile * STEPS + el.j < w.to;
-        xs.next(x, on, wide, most, -STEPS);
-        ds.next(raw, on, wide, most, -STEPS);
-        us.next(u, on, wide, most, -STEPS);
-        if (gated) zs.next(z, on, wide, most, -STEPS);
+        xs.next(x, wide, most, -STEPS);
+        ds.next(raw, wide, most, -STEPS);
+        us.next(u, wide, most, -STEPS);
+        if (gated) zs.next(z, wide, most, -STEPS);
         sides.load(tile * STEPS, w.len);
         front = *reinterpret_cast<const float4 *>(fronts);
         fronts -= (long)p.E * SP;
         sides.advance(-STEPS);
     };
-    if (top >= bottom) request(top);
+    if (top >= bottom) {
+        request(top);
+        xs.shift(past);
+        ds.shift(past);
+        us.shift(past);
+        zs.shift(past);
+    }
     for (int tile = top; tile >= bottom; --tile) {
         const bool on = tile * STEPS + el.j < w.to;
         float d[EPT], slope[EPT];
@@ -551,7 +563,6 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
         float k[STEPS][kStates], h[STEPS][kStates];
 #pragma unroll
         for (int j0 = 0; j0 < STEPS; j0 += 4) {
-            __builtin_amdgcn_sched_barrier(0);
             float y[4];
 #pragma unroll
             for (int j = j0; j < j0 + 4; ++j) {
@@ -575,7 +586,6 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
         }
 #pragma unroll
         for (int j0 = STEPS - 4; j0 >= 0; j0 -= 4) {
-            __builtin_amdgcn_sched_barrier(0);
             float ghb[4], akh[4];
 #pragma unroll
             for (int j = j0 + 3; j >= j0; --j) {
@@ -597,11 +607,9 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
                     ga[i] = fmaf(s.x, r, ga[i]);
                 }
                 const float sb = sum_over_channels<LANES>(vb), sc = sum_over_channels<LANES>(vc);
-                if ((lane & 15) < LANES) {
-                    const int row = lane >> 4, s_at = (lane % LANES) * kStates + (row & 1) * 2 + (row >> 1);
-                    sums[wave][j][s_at] = sb;
-                    sums[wave][j][SP + s_at] = sc;
-                }
+                // (lanes of a row that hold the same sum write it to the same place)
+                sums[wave][j][s_at] = sb;
+                sums[wave][j][SP + s_at] = sc;
             }
             float rb[StepSums<LANES>::kept], ra[StepSums<LANES>::kept];
             StepSums<LANES>::add(ghb, q, rb);
@@ -694,21 +702,26 @@ __global__ __launch_bounds__(kThreads) void scan_grad_carry_kernel(warpctct_scan
     const long t1 = last + el.j;
     const int el0 = have > 0 ? e0 : w.first, most = max(have - 1, 0);
     const bool gated = p.gate;
-    Column<IO, EPT> ds(p.dt, (long)w.n * p.dt_n + el0, p.dt_t, t1, w.from);
-    Column<IO, EPT> zs(p.gate, (long)w.n * p.gate_n + el0, p.gate_t, t1, w.from);
-    Column<IO, EPT> us(g.grad_out, (long)w.n * g.grad_n + el0, g.grad_t, t1, w.from);
+    const long past = max(t1 - (w.to - 1), 0L);
+    Column<IO, EPT> ds(p.dt, (long)w.n * p.dt_n + el0, p.dt_t, t1 - past);
+    Column<IO, EPT> zs(p.gate, (long)w.n * p.gate_n + el0, p.gate_t, t1 - past);
+    Column<IO, EPT> us(g.grad_out, (long)w.n * g.grad_n + el0, g.grad_t, t1 - past);
     typedef Sides<IO, LANES, kSteps> Side;
     Side sides(p, w, last, w.from);
     Raw<IO, EPT> d, u, z;
     auto request = [&](int t0) {
-        const bool on = t0 + el.j < w.to;
-        ds.next(d, on, wide, most, -kSteps);
-        us.next(u, on, wide, most, -kSteps);
-        if (gated) zs.next(z, on, wide, most, -kSteps);
+        ds.next(d, wide, most, -kSteps);
+        us.next(u, wide, most, -kSteps);
+        if (gated) zs.next(z, wide, most, -kSteps);
         sides.load(t0, w.len);
         sides.advance(-kSteps);
     };
-    if (w.from < w.to) request(last);
+    if (w.from < w.to) {
+        request(last);
+        ds.shift(past);
+        us.shift(past);
+        zs.shift(past);
+    }
     for (int t0 = w.from < w.to ? last : -1; t0 >= w.from; t0 -= kSteps) {
         const bool on = t0 + el.j < w.to;
 #pragma unroll
