@@ -84,7 +84,7 @@ def make(shape, dtype, params, seed=0):
     return x, weight, bias, g
 
 
-SHAPES = [(1, 1), (3, 2), (4, 7), (5, 64), (2, 3, 129), (9, 512), (3, 641), (2, 2048), (3, 2049), (2, 5000), (3, 8192),
+SHAPES = [(1, 1), (3, 2), (4, 7), (5, 64), (2, 3, 129), (9, 512), (3, 641), (2, 2048), (3, 2049), (2, 4097), (2, 5000), (3, 8192),
           (2, 8200), (2, 16384), (2, 16385), (1, 20000), (700, 40), (5000, 256)]
 
 

@@ -20,7 +20,6 @@ namespace {
 
 constexpr int kThreads = 256;        // of a workgroup whose wavefronts take a row each
 constexpr int kWide = 1024;          // the largest number of threads on one row
-constexpr int kMostInRegisters = 16 * kWide;
 constexpr unsigned kGroups = 1024;   // workgroups of the forward pass, at most
 constexpr int kGradGroups = 512;     // and of the backward pass, two on a compute unit
 
@@ -336,14 +335,19 @@ bool rows_aligned(const void *p, const RowAddress &a, size_t size) {
            (a.inner == 0u || a.outer_stride % (long)ev == 0);
 }
 
-// Threads on a row: a wavefront up to `most` elements a lane, then a workgroup of
-// 256, or of 1024 above 8192 elements (a lane of so large a workgroup has 128
-// registers).  A wavefront alone saves the exchanges through LDS; the backward
-// pass, which holds five values an element, is better off with more threads from
-// 1025 elements on (12800 rows of 2048 bfloat16: forward 24.2 against 27.4 us for
-// 256 threads, backward 50.3 against 42.2).
-constexpr int kMostForward = 32, kMostBackward = 16;
-int threads_for(int width, int most) { return width <= most * 64 ? 64 : width <= 32 * kThreads ? kThreads : kWide; }
+// Threads on a row and elements of each: a wavefront, 256 or 1024 threads, with as
+// many elements as leave them their registers (a lane of 1024 threads has 128).
+// A wavefront alone saves the exchanges through LDS; the backward pass, which
+// holds five values an element, and rows that are not loaded in vectors, whose
+// elements take a register each until they are used, are better off with more
+// threads (12800 rows of 2048 bfloat16: forward 24.2 us by wavefronts against 27.4
+// by 256 threads, backward 50.3 against 42.2).  0: no shape holds the row.
+int threads_for(int width, bool backward, bool vec) {
+    const int most = !backward && vec ? 32 : 16;
+    if (width <= most * 64) return 64;
+    if (width <= most * kThreads) return kThreads;
+    return width <= most / 2 * kWide ? kWide : 0;
+}
 
 template <typename IO, typename W, bool VEC, int CAP, int BLOCK>
 hipError_t start(const warpctct_norm_t &p, const RowAddress &at, int threads, hipStream_t stream) {
@@ -360,27 +364,26 @@ hipError_t start(const warpctct_norm_t &p, const RowAddress &at, int threads, hi
 template <typename IO, typename W>
 hipError_t start(const warpctct_norm_t &p, hipStream_t stream) {
     const RowAddress at = address(p.rows, p.x_inner_rows, p.x_outer_stride, p.x_inner_stride);
-    if (p.width > kMostInRegisters) {
+    const bool vec = p.width % kVec<IO> == 0 && rows_aligned(p.x, at, sizeof(IO)) &&
+                     (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
+    const int threads = threads_for(p.width, false, vec);
+    if (threads == 0) {
         auto kernel = norm_wide_kernel<IO, W>;
         TIMED_LAUNCH(kernel, dim3((unsigned)p.rows), dim3(kWide), 0, stream, static_cast<const IO *>(p.x), at,
                      static_cast<const W *>(p.weight), static_cast<const W *>(p.bias), p.eps,
                      static_cast<IO *>(p.out), p.stats, p.width);
         return hipGetLastError();
     }
-    const int threads = threads_for(p.width, kMostForward);
-    const bool vec = p.width % kVec<IO> == 0 && rows_aligned(p.x, at, sizeof(IO)) &&
-                     (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
     if (threads == kWide)
         return vec ? start<IO, W, true, 16, kWide>(p, at, threads, stream)
-                   : start<IO, W, false, 16, kWide>(p, at, threads, stream);
+                   : start<IO, W, false, 8, kWide>(p, at, threads, stream);
     if (p.width <= 8 * threads)
         return vec ? start<IO, W, true, 8, kThreads>(p, at, threads, stream)
                    : start<IO, W, false, 8, kThreads>(p, at, threads, stream);
     if (p.width <= 16 * threads)
         return vec ? start<IO, W, true, 16, kThreads>(p, at, threads, stream)
                    : start<IO, W, false, 16, kThreads>(p, at, threads, stream);
-    return vec ? start<IO, W, true, 32, kThreads>(p, at, threads, stream)
-               : start<IO, W, false, 32, kThreads>(p, at, threads, stream);
+    return start<IO, W, true, 32, kThreads>(p, at, threads, stream);
 }
 
 template <typename IO, typename W, bool VEC, int CAP, int BLOCK>
@@ -399,7 +402,11 @@ template <typename IO, typename W>
 hipError_t start_grad(const warpctct_norm_t &p, const warpctct_norm_grad_t &g, float *partial, hipStream_t stream) {
     const RowAddress x_at = address(p.rows, p.x_inner_rows, p.x_outer_stride, p.x_inner_stride);
     const RowAddress g_at = address(p.rows, g.inner_rows, g.outer_stride, g.inner_stride);
-    if (p.width > kMostInRegisters) {
+    const bool vec = p.width % kVec<IO> == 0 && rows_aligned(p.x, x_at, sizeof(IO)) &&
+                     rows_aligned(g.grad_out, g_at, sizeof(IO)) &&
+                     (reinterpret_cast<uintptr_t>(g.grad_x) & 15u) == 0;
+    const int threads = threads_for(p.width, true, vec);
+    if (threads == 0) {
         if (g.grad_x) {
             auto kernel = norm_wide_grad_kernel<IO, W>;
             TIMED_LAUNCH(kernel, dim3((unsigned)p.rows), dim3(kWide), 0, stream, static_cast<const IO *>(p.x), x_at,
@@ -415,27 +422,20 @@ hipError_t start_grad(const warpctct_norm_t &p, const warpctct_norm_grad_t &g, f
         }
         return hipGetLastError();
     }
-    const int threads = threads_for(p.width, kMostBackward);
-    const bool vec = p.width % kVec<IO> == 0 && rows_aligned(p.x, x_at, sizeof(IO)) &&
-                     rows_aligned(g.grad_out, g_at, sizeof(IO)) &&
-                     (reinterpret_cast<uintptr_t>(g.grad_x) & 15u) == 0;
     if (threads == kWide)
-        return vec ? start_grad<IO, W, true, 16, kWide>(p, g, x_at, g_at, threads, partial, stream)
-                   : start_grad<IO, W, false, 16, kWide>(p, g, x_at, g_at, threads, partial, stream);
+        return vec ? start_grad<IO, W, true, 8, kWide>(p, g, x_at, g_at, threads, partial, stream)
+                   : start_grad<IO, W, false, 8, kWide>(p, g, x_at, g_at, threads, partial, stream);
     if (p.width <= 8 * threads)
         return vec ? start_grad<IO, W, true, 8, kThreads>(p, g, x_at, g_at, threads, partial, stream)
                    : start_grad<IO, W, false, 8, kThreads>(p, g, x_at, g_at, threads, partial, stream);
-    if (p.width <= 16 * threads)
-        return vec ? start_grad<IO, W, true, 16, kThreads>(p, g, x_at, g_at, threads, partial, stream)
-                   : start_grad<IO, W, false, 16, kThreads>(p, g, x_at, g_at, threads, partial, stream);
-    return vec ? start_grad<IO, W, true, 32, kThreads>(p, g, x_at, g_at, threads, partial, stream)
-               : start_grad<IO, W, false, 32, kThreads>(p, g, x_at, g_at, threads, partial, stream);
+    return vec ? start_grad<IO, W, true, 16, kThreads>(p, g, x_at, g_at, threads, partial, stream)
+               : start_grad<IO, W, false, 16, kThreads>(p, g, x_at, g_at, threads, partial, stream);
 }
 
 }  // namespace
 
 int norm_grad_groups(long rows, int width) {
-    const long per = width <= kMostBackward * 64 ? 4 : 1;      // rows of a workgroup at a time
+    const long per = threads_for(width, true, false) == 64 ? 4 : 1;      // rows of a workgroup at a time
     const long groups = (rows + per - 1) / per;
     return (int)(groups < kGradGroups ? groups : kGradGroups);
 }

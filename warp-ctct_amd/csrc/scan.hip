@@ -154,6 +154,17 @@ __device__ __forceinline__ void store_row(IO *p, int have, bool wide, const floa
     }
 }
 
+// Zeros to the elements of rows [from + j, to) of every `by`: the steps that do not
+// count.  (The zeros are opaque to the compiler, which would otherwise write them
+// again between two wide stores of them.)
+template <int N, typename IO>
+__device__ __forceinline__ void clear_rows(IO *p, long stride, int from, int to, int by, int have, bool wide) {
+    float zero[N] = {};
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(zero[i]));
+    for (int t = from; t < to; t += by) store_row<N>(p + t * stride, have, wide, zero);
+}
+
 // The tile's rows of b and c, STEPS x 2 SP values, by all threads: a thread has
 // one column of b or of c, and of every kRows steps one.  Where there is nothing
 // to read (behind the sequence, past the states) it reads row `safe` of its
@@ -397,9 +408,8 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
     }
     if (blockIdx.z + 1 != gridDim.z) return;
     // the steps that do not count
-    const float zero[EPT] = {};
     out = static_cast<IO *>(p.out) + (long)w.n * p.L * p.E + e0;
-    for (int t = w.len + el.j; t < p.L; t += kSteps) store_row<EPT>(out + (long)t * p.E, have, wide, zero);
+    clear_rows<EPT>(out, p.E, w.len + el.j, p.L, kSteps, have, wide);
     if (p.last && live) {
 #pragma unroll
         for (int i = 0; i < kStates; ++i)
@@ -494,11 +504,10 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     IO *gx = static_cast<IO *>(g.grad_x) + rows, *gd = static_cast<IO *>(g.grad_dt) + rows;
     IO *gz = p.gate ? static_cast<IO *>(g.grad_gate) + rows : nullptr;
 
-    const float zero[EPT] = {};
-    for (int t = blockIdx.z + 1 == gridDim.z ? w.len + el.j : p.L; t < p.L; t += STEPS) {
-        store_row<EPT>(gx + (long)t * p.E, have, wide, zero);
-        store_row<EPT>(gd + (long)t * p.E, have, wide, zero);
-        if (gz) store_row<EPT>(gz + (long)t * p.E, have, wide, zero);
+    if (blockIdx.z + 1 == gridDim.z) {
+        clear_rows<EPT>(gx, p.E, w.len + el.j, p.L, STEPS, have, wide);
+        clear_rows<EPT>(gd, p.E, w.len + el.j, p.L, STEPS, have, wide);
+        if (gz) clear_rows<EPT>(gz, p.E, w.len + el.j, p.L, STEPS, have, wide);
     }
     // the rows of a tile and the states in front of it are asked for while the
     // tile behind it is worked on
@@ -777,10 +786,10 @@ __global__ __launch_bounds__(kThreads) void scan_grad_bc_kernel(warpctct_scan_t 
 }
 
 // One step of N sequences; a channel lies on kLanes lanes, and a thread takes its
-// four states of `BATCH` sequences, so that a is read once for them.  wide: b, c,
+// four states of `BATCH` sequences, so that a is read once for them.  WIDE: b, c,
 // a and the states in pieces of four.
-template <typename IO, int LANES, int BATCH>
-__global__ __launch_bounds__(kThreads) void scan_step_kernel(warpctct_scan_step_t p, bool wide) {
+template <typename IO, int LANES, int BATCH, bool WIDE>
+__global__ __launch_bounds__(kThreads) void scan_step_kernel(warpctct_scan_step_t p) {
     const long i0 = (long)blockIdx.x * kThreads + threadIdx.x;
     if (i0 >= (long)p.E * LANES) return;           // all lanes of a channel
     const int e = (int)(i0 / LANES), q = threadIdx.x % LANES, s0 = q * kStates, grp = e / (p.E / p.G);
@@ -788,7 +797,7 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(warpctct_scan_step_
     const float *ap = p.a + (long)e * p.S + s1;
     float a[kStates];
     Raw<float, kStates> ar;
-    ar.load(ap, wide, most);
+    ar.load(ap, WIDE, most);
 #pragma unroll
     for (int i = 0; i < kStates; ++i) a[i] = ar[i] * kLog2e;
     const float bias = p.dt_bias ? p.dt_bias[e] : 0.0f, skip = p.skip ? p.skip[e] : 0.0f;
@@ -803,9 +812,9 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(warpctct_scan_step_
             // (the same for the whole workgroup: a sequence that stays is not read)
             go[k] = __builtin_amdgcn_readfirstlane(n0 + k < p.N && (!p.advance || p.advance[n]));
             if (!go[k]) continue;
-            h[k].load(p.state + (n * p.E + e) * p.S + s1, wide, most);
-            b[k].load(static_cast<const IO *>(p.b) + n * p.b_n + grp * p.b_g + s1, wide, most);
-            c[k].load(static_cast<const IO *>(p.c) + n * p.c_n + grp * p.c_g + s1, wide, most);
+            h[k].load(p.state + (n * p.E + e) * p.S + s1, WIDE, most);
+            b[k].load(static_cast<const IO *>(p.b) + n * p.b_n + grp * p.b_g + s1, WIDE, most);
+            c[k].load(static_cast<const IO *>(p.c) + n * p.c_n + grp * p.c_g + s1, WIDE, most);
             x[k] = static_cast<const IO *>(p.x)[n * p.x_n + e];
             d[k] = static_cast<const IO *>(p.dt)[n * p.dt_n + e];
             if (p.gate) z[k] = static_cast<const IO *>(p.gate)[n * p.gate_n + e];
@@ -813,35 +822,33 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(warpctct_scan_step_
 #pragma unroll
         for (int k = 0; k < BATCH; ++k) {
             if (n0 + k >= p.N) break;
-            IO *out = static_cast<IO *>(p.out) + (n0 + k) * p.E + e;
-            if (!go[k]) {
-                if (q == 0) *out = from_float<IO>(0.0f);
-                continue;
-            }
-            const float xv = to_float(x[k]);
-            float dv = to_float(d[k]) + bias;
-            if (p.softplus) dv = softplus(dv).value;
-            const float dx = dv * xv;
-            float y = 0.0f, hv[kStates];
+            float y = 0.0f;
+            if (go[k]) {
+                const float xv = to_float(x[k]);
+                float dv = to_float(d[k]) + bias;
+                if (p.softplus) dv = softplus(dv).value;
+                const float dx = dv * xv;
+                float hv[kStates];
 #pragma unroll
-            for (int i = 0; i < kStates; ++i) {
-                hv[i] = fmaf(exp2_hw(dv * a[i]), h[k][i], dx * b[k][i]);
-                y = s0 + i < p.S ? fmaf(c[k][i], hv[i], y) : y;
-            }
-            float *to = p.state + ((n0 + k) * p.E + e) * p.S + s0;
-            if (wide) {
-                store_n<kStates>(to, hv);
-            } else {
+                for (int i = 0; i < kStates; ++i) {
+                    hv[i] = fmaf(exp2_hw(dv * a[i]), h[k][i], dx * b[k][i]);
+                    y = s0 + i < p.S ? fmaf(c[k][i], hv[i], y) : y;
+                }
+                float *to = p.state + ((n0 + k) * p.E + e) * p.S + s0;
+                if (WIDE) {
+                    store_n<kStates>(to, hv);
+                } else {
 #pragma unroll
-                for (int i = 0; i < kStates; ++i)
-                    if (s0 + i < p.S) to[i] = hv[i];
+                    for (int i = 0; i < kStates; ++i)
+                        if (s0 + i < p.S) to[i] = hv[i];
+                }
+                y = fmaf(skip, xv, channel_sum<LANES>(y));
+                if (p.gate) {
+                    const float zv = to_float(z[k]);
+                    y *= zv * sigmoid(zv);
+                }
             }
-            y = fmaf(skip, xv, channel_sum<LANES>(y));
-            if (p.gate) {
-                const float zv = to_float(z[k]);
-                y *= zv * sigmoid(zv);
-            }
-            if (q == 0) *out = from_float<IO>(y);
+            if (q == 0) static_cast<IO *>(p.out)[(n0 + k) * p.E + e] = from_float<IO>(y);
         }
     }
 }
@@ -970,9 +977,8 @@ hipError_t start_step(const warpctct_scan_step_t &p, hipStream_t stream) {
     const bool wide = p.S == kStates * LANES && aligned16(p.state) && aligned16(p.a) && p.b_n % kStates == 0 &&
                       p.b_g % kStates == 0 && p.c_n % kStates == 0 && p.c_g % kStates == 0 &&
                       (reinterpret_cast<uintptr_t>(p.b) | reinterpret_cast<uintptr_t>(p.c)) % four == 0;
-    auto kernel = scan_step_kernel<IO, LANES, BATCH>;
-    TIMED_LAUNCH(kernel, dim3((unsigned)groups, (unsigned)std::min(batches, 65535L)), dim3(kThreads), 0, stream, p,
-                 wide);
+    auto kernel = wide ? scan_step_kernel<IO, LANES, BATCH, true> : scan_step_kernel<IO, LANES, BATCH, false>;
+    TIMED_LAUNCH(kernel, dim3((unsigned)groups, (unsigned)std::min(batches, 65535L)), dim3(kThreads), 0, stream, p);
     return hipGetLastError();
 }
 template <typename IO, int LANES>
