@@ -27,6 +27,7 @@
 // them one after the other, and the second pass starts every chunk from its own
 // states; the reverse recurrence of gh alike.
 #include <algorithm>
+#include <cmath>
 
 #include "network.h"
 #include "rows.h"
@@ -106,10 +107,11 @@ __device__ __forceinline__ float sum_over_channels(const float (&v)[kStates]) {
     return s;
 }
 
-// Where a workgroup works: sequence n, channels [first, end) of group g, steps
-// [from, to) of the `len` that count (chunk blockIdx.z of the sequence).
+// Where a workgroup works: sequence n, channels [first, end) of group g, chunk
+// blockIdx.z of the sequence: steps [from, to) of the `len` that count and
+// [clear, over) of those that do not.
 struct Place {
-    int n, g, block, first, end, len, from, to;
+    int n, g, block, first, end, len, from, to, clear, over;
 };
 template <int LANES>
 __device__ __forceinline__ Place place_of(const warpctct_scan_t &p, int chunk_tiles) {
@@ -122,8 +124,11 @@ __device__ __forceinline__ Place place_of(const warpctct_scan_t &p, int chunk_ti
     w.first = w.g * per + (blockIdx.x - w.g * blocks) * CH;
     w.end = (w.g + 1) * per;
     w.len = p.lengths ? min(max(p.lengths[w.n], 0), p.L) : p.L;
-    w.from = min((int)blockIdx.z * chunk_tiles * kSteps, w.len);
-    w.to = blockIdx.z + 1 == gridDim.z ? w.len : min(w.from + chunk_tiles * kSteps, w.len);
+    const int first = min((int)blockIdx.z * chunk_tiles * kSteps, p.L);
+    w.over = blockIdx.z + 1 == gridDim.z ? p.L : min(first + chunk_tiles * kSteps, p.L);
+    w.from = min(first, w.len);
+    w.to = min(w.over, w.len);
+    w.clear = max(first, w.len);
     return w;
 }
 
@@ -406,10 +411,9 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
         }
         return;
     }
-    if (blockIdx.z + 1 != gridDim.z) return;
-    // the steps that do not count
     out = static_cast<IO *>(p.out) + (long)w.n * p.L * p.E + e0;
-    clear_rows<EPT>(out, p.E, w.len + el.j, p.L, kSteps, have, wide);
+    clear_rows<EPT>(out, p.E, w.clear + el.j, w.over, kSteps, have, wide);
+    if (blockIdx.z + 1 != gridDim.z) return;
     if (p.last && live) {
 #pragma unroll
         for (int i = 0; i < kStates; ++i)
@@ -419,7 +423,9 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
 
 // Joins chunks: turns what each makes of zeros into what stands in front of it,
 // in place; backwards for the reverse recurrence, whose end (in front of the
-// sequence) goes to `end`.  A thread has one state.
+// sequence) goes to `end`.  A thread has one state, and asks for kJoin chunks while
+// it joins the kJoin in front of them.
+constexpr int kJoin = 16;
 __global__ __launch_bounds__(kThreads) void scan_join_kernel(const float *__restrict__ a, const float *__restrict__ first,
                                                              Chunks chunks, int count, int E, int S, int SP,
                                                              bool backwards, float *__restrict__ end) {
@@ -430,23 +436,31 @@ __global__ __launch_bounds__(kThreads) void scan_join_kernel(const float *__rest
     const float rate = a[(long)e * S + k] * kLog2e;
     const long state = ((long)n * E + e) * S + k;
     float h = first ? first[state] : 0.0f;
-    for (int c0 = 0; c0 < count; c0 += 8) {
-        float local[8], total[8];
+    float local[2][kJoin], total[2][kJoin];
+    auto request = [&](int c0, float (&l)[kJoin], float (&d)[kJoin]) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            if (c0 + c >= count) break;
-            const int at = backwards ? count - 1 - c0 - c : c0 + c;
+        for (int c = 0; c < kJoin; ++c) {
+            const int i = min(c0 + c, count - 1), at = backwards ? count - 1 - i : i;
             const long chunk = ((long)n * count + at) * E + e;
-            local[c] = chunks.local[chunk * SP + k];
-            total[c] = chunks.total[chunk];
+            l[c] = chunks.local[chunk * SP + k];
+            d[c] = chunks.total[chunk];
         }
+    };
+    auto join = [&](int c0, const float (&l)[kJoin], const float (&d)[kJoin]) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < kJoin; ++c) {
             if (c0 + c >= count) break;
             const int at = backwards ? count - 1 - c0 - c : c0 + c;
             chunks.local[(((long)n * count + at) * E + e) * SP + k] = h;
-            h = fmaf(exp2_hw(rate * total[c]), h, local[c]);
+            h = fmaf(exp2_hw(rate * d[c]), h, l[c]);
         }
+    };
+    request(0, local[0], total[0]);
+    for (int c0 = 0; c0 < count; c0 += 2 * kJoin) {
+        if (c0 + kJoin < count) request(c0 + kJoin, local[1], total[1]);
+        join(c0, local[0], total[0]);
+        if (c0 + 2 * kJoin < count) request(c0 + 2 * kJoin, local[0], total[0]);
+        join(c0 + kJoin, local[1], total[1]);
     }
     if (end) end[state] = h;
 }
@@ -504,11 +518,9 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     IO *gx = static_cast<IO *>(g.grad_x) + rows, *gd = static_cast<IO *>(g.grad_dt) + rows;
     IO *gz = p.gate ? static_cast<IO *>(g.grad_gate) + rows : nullptr;
 
-    if (blockIdx.z + 1 == gridDim.z) {
-        clear_rows<EPT>(gx, p.E, w.len + el.j, p.L, STEPS, have, wide);
-        clear_rows<EPT>(gd, p.E, w.len + el.j, p.L, STEPS, have, wide);
-        if (gz) clear_rows<EPT>(gz, p.E, w.len + el.j, p.L, STEPS, have, wide);
-    }
+    clear_rows<EPT>(gx, p.E, w.clear + el.j, w.over, STEPS, have, wide);
+    clear_rows<EPT>(gd, p.E, w.clear + el.j, w.over, STEPS, have, wide);
+    if (gz) clear_rows<EPT>(gz, p.E, w.clear + el.j, w.over, STEPS, have, wide);
     // the rows of a tile and the states in front of it are asked for while the
     // tile behind it is worked on
     const int top = (w.to + STEPS - 1) / STEPS - 1, bottom = w.from < w.to ? w.from / STEPS : top + 1;
@@ -890,7 +902,9 @@ bool rows_wide(const warpctct_scan_t &p, int ept) {
 // steps (us, uncut / cut): forwards 512 wavefronts 186 / 102, 768 186 / 139, 1024
 // 188 / 178, 1536 245 / 272; backwards 1024 595 / 454, 1536 746 / 711, 2048
 // 751 / 885; with 300 steps forwards 768 41 / 45, backwards 1024 130 / 111, 1536
-// 157 / 162.  Fewer than 8 tiles are not worth the two launches more.
+// 157 / 162.  Fewer than 8 tiles are not worth the two launches more, and more
+// than 8 sqrt(tiles) chunks take longer to join than they save (2 us a tile for a
+// wavefront on its own).
 struct Cut {
     int count, tiles;
 };
@@ -898,7 +912,7 @@ Cut cut_of(const warpctct_scan_t &p, bool backward) {
     const long waves = (long)p.N * p.G * blocks_of(p) * (kThreads / 64), tiles = ((long)p.L + kSteps - 1) / kSteps;
     Cut c = {1, (int)tiles};
     if (waves <= 0 || waves > (backward ? 1024 : 768) || tiles < 8) return c;
-    const long count = std::min(8192 / waves, tiles / 2);
+    const long count = std::min(std::min(8192 / waves, tiles / 2), (long)(8.0 * std::sqrt((double)tiles)));
     c.tiles = (int)((tiles + count - 1) / count);
     c.count = (int)((tiles + c.tiles - 1) / c.tiles);
     return c;
