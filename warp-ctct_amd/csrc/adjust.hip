@@ -4,13 +4,14 @@
 //   count > 0:  l = l > 0 ? l / repetition : l * repetition
 //               l = l - presence - frequency * count
 //   l = l + bias[v];  not allowed: l = -infinity
-// Bound by HBM, or by the launch where the logits are few.  A workgroup takes
-// kVectors 16-byte vectors a thread (4096 columns of 2-byte elements) of a row,
-// asks for them first, counts meanwhile those of the row's tokens that fall into
-// its columns in LDS (integers: the order does not matter), and applies the rules.
-// More columns a workgroup would read the history less often, but 16384 of them
-// take 64 KB of LDS for the counts, which leaves 8 wavefronts on a compute unit:
-// 20.3 us instead of 11.5 for 128 rows of 65536 bfloat16 logits with 300 tokens each.
+// Bound by HBM, or by the launch where the logits are few.  A workgroup takes one
+// 16-byte vector a thread (2048 columns of 2-byte elements) of a row, asks for
+// everything that belongs to it first, counts meanwhile those of the row's tokens
+// that fall into its columns in LDS (integers: the order does not matter), and
+// applies the rules.  More columns a workgroup would read the history less often,
+// but fewer wavefronts would share a compute unit: 128 rows of 65536 bfloat16
+// logits with 300 tokens each take 10.5 us with one vector a thread, 11.5 with two,
+// 13.2 with four.
 #include "network.h"
 #include "rows.h"
 
@@ -19,7 +20,7 @@ namespace wctct {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kVectors = 2;      // 16-byte vectors of a thread
+constexpr int kVectors = 1;      // 16-byte vectors of a thread
 
 // EV columns of a bias of any of the three types, all of them asked for at once
 template <typename B, int EV>

@@ -14,7 +14,7 @@ namespace {
 // kParts rows (4096 rows of 380 columns: 6 workgroups alone would walk down 256
 // rows each).
 constexpr int kStrands = 16;
-constexpr long kDirect = 512;
+constexpr long kDirect = 1024;
 constexpr int kParts = 64;
 
 __device__ __forceinline__ void store_as(void *p, int type, int at, float v) {

@@ -21,7 +21,10 @@ namespace {
 constexpr int kThreads = 256;        // of a workgroup whose wavefronts take a row each
 constexpr int kWide = 1024;          // the largest number of threads on one row
 constexpr unsigned kGroups = 1024;   // workgroups of the forward pass, at most
-constexpr int kGradGroups = 512;     // and of the backward pass, two on a compute unit
+// and of the backward pass: four on a compute unit where they take a row each, two
+// where their wavefronts do (12800 rows of 2048 elements: 36.6 us with 1024, 42.0
+// with 512; 2592 rows of 641: 16.2 with 1024, 11.4 with 512)
+constexpr int kGradGroups = 1024, kGradGroupsOfWaves = 512;
 
 // Sums of two values over the threads of a row: a wavefront (threads == 64) or
 // the whole workgroup.  `shared` holds 2 floats per wavefront and is free again
@@ -437,7 +440,8 @@ hipError_t start_grad(const warpctct_norm_t &p, const warpctct_norm_grad_t &g, f
 int norm_grad_groups(long rows, int width) {
     const long per = threads_for(width, true, false) == 64 ? 4 : 1;      // rows of a workgroup at a time
     const long groups = (rows + per - 1) / per;
-    return (int)(groups < kGradGroups ? groups : kGradGroups);
+    const long most = per == 1 ? kGradGroups : kGradGroupsOfWaves;
+    return (int)(groups < most ? groups : most);
 }
 
 hipError_t launch_layer_norm(const warpctct_norm_t &p, hipStream_t stream) {
