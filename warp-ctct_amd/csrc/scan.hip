@@ -70,7 +70,6 @@ __device__ __forceinline__ Softplus softplus(float v) {
     s = fmaf(s, r2, 1.0f);
     Softplus p;
     p.value = fmaf(2.0f * r, s, fmaxf(v, 0.0f));
-    if (v != v) p.value = v;
     const float inv = __builtin_amdgcn_rcpf(1.0f + q);
     p.slope = v >= 0.0f ? inv : q * inv;
     return p;
