@@ -175,6 +175,19 @@ def test_parameters_in_the_inputs_type_and_the_state_alone(dtype):
 
 
 @gpu
+def test_gradients_of_some_of_the_inputs_and_twice():
+    args = make(3, 40, 24, 4, torch.float16)
+    want = run(*args)
+    for keep, name in enumerate(("gx", "gw", "gb", "ginitial")):
+        some = [leaf(t) if i == keep else t.detach() for i, t in enumerate(args[:4])]
+        out, state = warp_ctct.causal_conv(some[0], some[1], some[2], None, some[3], "silu", return_state=True)
+        for again in (True, False):     # the state does not depend on the parameters
+            ends, ups = ([out, state], args[4:]) if state.requires_grad else ([out], args[4:5])
+            got, = torch.autograd.grad(ends, some[keep], ups, retain_graph=again)
+            assert torch.equal(got, want[name])
+
+
+@gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("E,K", [(24, 4), (7, 3), (16, 1), (8, 8)])
 def test_steps_and_pieces_are_the_whole(E, K, dtype):

@@ -4,7 +4,8 @@ Tolerances.  With h the normalised value, every h the kernel forms is off by at
 most ~64 units of 2^-24 (1 + |h|): the deviations from the first mean are exact
 to half a unit each, the mean of them and of their squares is a sum of at most
 54 additions in sequence (32 in a lane, 6 across a wavefront, 16 across a
-workgroup), and the root and the two products add four roundings.  A result rounded to a type is off by half a step of it, eps/2 |value|."""
+workgroup), and the root and the two products add four roundings.  A result
+rounded to a type is off by half a step of it, eps/2 |value|."""
 import pytest
 import torch
 
@@ -84,8 +85,8 @@ def make(shape, dtype, params, seed=0):
     return x, weight, bias, g
 
 
-SHAPES = [(1, 1), (3, 2), (4, 7), (5, 64), (2, 3, 129), (9, 512), (3, 641), (2, 2048), (3, 2049), (2, 4097), (2, 5000), (3, 8192),
-          (2, 8200), (2, 16384), (2, 16385), (1, 20000), (700, 40), (5000, 256)]
+SHAPES = [(1, 1), (3, 2), (4, 7), (5, 64), (2, 3, 129), (9, 512), (3, 641), (2, 2048), (3, 2049), (2, 4097),
+          (2, 5000), (3, 8192), (2, 8200), (2, 16384), (2, 16385), (1, 20000), (700, 40), (5000, 256)]
 
 
 @gpu
@@ -208,12 +209,25 @@ def test_gradient_against_differences():
 
 
 @gpu
+@pytest.mark.parametrize("shape", [(50, 96), (3, 20000)])
+def test_gradients_of_some_of_the_inputs_and_twice(shape):
+    args = make(shape, torch.bfloat16, "f32")
+    _, want = run(*args)
+    for keep in range(3):
+        some = [leaf(t) if i == keep else t.detach() for i, t in enumerate(args[:3])]
+        out = warp_ctct.layer_norm(*some)
+        first = torch.autograd.grad(out, some[keep], args[3], retain_graph=True)[0]
+        assert torch.equal(first, want[keep])
+        assert torch.equal(first, torch.autograd.grad(out, some[keep], args[3])[0])
+
+
+@gpu
 def test_refusals_on_the_gpu():
     x, weight, bias, g = make((4, 12), torch.float32, "f32")
     for bad in (dict(weight=torch.ones(11, device="cuda")), dict(bias=torch.ones(12, 1, device="cuda")),
-                dict(weight=torch.ones(12)), dict(eps=-1.0)):
+                dict(weight=torch.ones(12)), dict(eps=-1.0), dict(x=torch.ones(4, 12, device="cuda", dtype=torch.cfloat))):
         with pytest.raises(RuntimeError):
-            warp_ctct.layer_norm(x, **bad)
+            warp_ctct.layer_norm(**{**dict(x=x), **bad})
     with pytest.raises(RuntimeError):
         warp_ctct.layer_norm(torch.zeros(4, 0, device="cuda"))
     with pytest.raises(RuntimeError, match="create_graph"):

@@ -255,6 +255,37 @@ def test_strided_inputs_and_gradients(dtype):
 
 
 @gpu
+def test_gradients_of_some_of_the_inputs_and_twice():
+    case = Case(3, 40, 24, 16, 2, torch.bfloat16)
+    want = case.run()
+    for name in list(case.args):
+        some = {k: v.detach().requires_grad_(k == name) for k, v in case.args.items()}
+        out, state = warp_ctct.selective_scan(**some, softplus=True, return_state=True)
+        for again in (True, False):
+            got, = torch.autograd.grad([out, state], some[name], [case.g, case.glast], retain_graph=again)
+            assert torch.equal(got, want["grad_" + name]), name
+
+
+@gpu
+def test_the_state_alone_and_parameters_of_another_type():
+    case = Case(2, 40, 24, 16, dtype=torch.float16)
+    for name in ("a", "skip", "dt_bias"):
+        case.args[name] = case.args[name].to(torch.bfloat16)
+    case.track()
+    val, tol = oracle(case)
+    got = case.run()
+    assert got["grad_a"].dtype == torch.bfloat16
+    for name in got:
+        check(got[name], val, tol, name)
+    case.g = torch.zeros_like(case.g)
+    val, tol = oracle(case)
+    _, state = case.call()
+    names = ("x", "dt", "a", "b", "dt_bias", "initial_state")
+    for name, g in zip(names, torch.autograd.grad(state, [case.args[k] for k in names], case.glast)):
+        check(g, val, tol, "grad_" + name)
+
+
+@gpu
 def test_extreme_steps():
     case = Case(2, 40, 16, 16, softplus=True)
     with torch.no_grad():

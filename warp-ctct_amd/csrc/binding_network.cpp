@@ -28,7 +28,10 @@ int type_of(const torch::Tensor &t) {
 
 // float32, float16 and bfloat16 as they are, any other type as float32 (as the
 // losses take their inputs)
-torch::Tensor native(const torch::Tensor &t) { return is_native(t) ? t : t.to(at::ScalarType::Float); }
+torch::Tensor native(const torch::Tensor &t) {
+    TORCH_CHECK(!t.is_complex(), "complex tensors are not supported");
+    return is_native(t) ? t : t.to(at::ScalarType::Float);
+}
 
 void check_on(const torch::Tensor &t, const torch::Tensor &like, const char *name) {
     TORCH_CHECK(t.device() == like.device(), name, " must be located on the same GPU as the input");

@@ -5,7 +5,10 @@
 // Bound by HBM: x is read and out written once, in the backward x and g read and
 // gx written.  A thread takes a few channels next to each other and walks down a
 // tile of time with the last K-1 inputs in registers, so that every row is
-// loaded once but for the K-1 rows where two tiles meet.
+// loaded once but for the K-1 rows where two tiles meet.  Four channels a thread:
+// with eight of 2-byte elements there are too few wavefronts to keep the memory
+// busy (32 ragged sequences of up to 400 steps, 2048 channels, bfloat16: forward
+// 39.5 us instead of 26, 3.5 TB/s; backward 41 us, 3.2 TB/s).
 #include "network.h"
 #include "rows.h"
 
