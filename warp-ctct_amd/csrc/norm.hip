@@ -122,8 +122,8 @@ struct Slots {
 template <typename IO, typename W, bool VEC, int CAP, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void norm_kernel(const IO *__restrict__ x, RowAddress at,
                                                      const W *__restrict__ weight, const W *__restrict__ bias,
-                                                     float eps, IO *__restrict__ out, float *__restrict__ stats, unsigned rows, int width,
-                                                     int threads) {
+                                                     float eps, IO *__restrict__ out, float *__restrict__ stats,
+                                                     unsigned rows, int width, int threads) {
     typedef Slots<IO, VEC, CAP> S;
     __shared__ float shared[2 * kWide / 64];
     const int t = threads == 64 ? threadIdx.x & 63 : threadIdx.x;

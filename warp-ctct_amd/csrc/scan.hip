@@ -29,8 +29,8 @@
 //
 // Measured with 16 states, bfloat16 and a gate: 32 ragged sequences of up to 400
 // steps, 1024 channels: forward 62 us, backward 155 us, of which the vector units
-// cannot do without 39 and 109 (SQ_ACTIVE_INST_VALU); one sequence of 16384 steps,
-// 2048 channels: 246 us in two passes, 228 of them the vector units'; one step of
+// cannot do without 38 and 109 (SQ_ACTIVE_INST_VALU); one sequence of 16384 steps,
+// 2048 channels: 245 us in two passes, 224 of them the vector units'; one step of
 // 256 sequences, 2048 channels: 12.6 us, 5.6 TB/s.
 #include <algorithm>
 #include <cmath>
@@ -53,9 +53,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Steps of a tile of the backward pass, which is also how far apart the states
 // lie that the forward pass keeps for it: the states and factors of a tile take
 // 8 registers a step, and a thread has up to 4 elements.  With 8 steps the kernel
-// takes 181 registers, two wavefronts on a SIMD; with 16 it spilled (training on
+// takes 188 registers, two wavefronts on a SIMD; with 16 it spilled (training on
 // the sequences above: 708 us instead of 392 at the time).
 constexpr int back_steps(int lanes) { return lanes == 1 ? 4 : lanes == 16 ? 16 : 8; }
+
+// Channels of a row in LDS that the lanes of a channel write at four steps at a
+// time: as far apart as a wavefront's channels, so that the four fall into
+// different banks.
+constexpr int padded(int lanes) { return kThreads / lanes + 64 / lanes; }
 
 __device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
 
@@ -124,7 +129,11 @@ __device__ __forceinline__ Place place_of(const warpctct_scan_t &p, int chunk_ti
     constexpr int CH = kThreads / LANES;
     const int per = p.E / p.G, blocks = (per + CH - 1) / CH;
     Place w;
-    w.n = blockIdx.y;
+    // First one half of the batch, then the other from its end: of a batch sorted
+    // by length a CU that takes two workgroups is given a long sequence and a short
+    // one (training on 32 sequences of 200 to 400 steps: 225 us, in order 227).
+    const int half = (p.N + 1) / 2;
+    w.n = (int)blockIdx.y < half ? blockIdx.y : p.N - 1 - (blockIdx.y - half);
     w.block = blockIdx.x;
     w.g = blockIdx.x / blocks;
     w.first = w.g * per + (blockIdx.x - w.g * blocks) * CH;
@@ -298,9 +307,10 @@ template <typename IO, int LANES, bool CARRY>
 __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float *__restrict__ keep, Chunks chunks,
                                                         const float *__restrict__ starts, bool wide) {
     constexpr int CH = kThreads / LANES, SP = kStates * LANES, EPT = Elements<LANES, kSteps>::EPT;
+    constexpr int PAD = padded(LANES);
     __shared__ float2 steps[kSteps][CH];           // d, d x
     __shared__ __align__(16) float bc[kSteps][2 * SP];
-    __shared__ float ys[kSteps][CARRY ? 1 : CH];
+    __shared__ float ys[kSteps][CARRY ? 1 : PAD];
     constexpr int BACK = back_steps(LANES);
     const Place w = place_of<LANES>(p, chunks.tiles);
     const Elements<LANES, kSteps> el;
@@ -432,7 +442,8 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
 // sequence) goes to `end`.  A thread has one state, and asks for kJoin chunks while
 // it joins the kJoin in front of them.
 constexpr int kJoin = 16;
-__global__ __launch_bounds__(kThreads) void scan_join_kernel(const float *__restrict__ a, const float *__restrict__ first,
+__global__ __launch_bounds__(kThreads) void scan_join_kernel(const float *__restrict__ a,
+                                                             const float *__restrict__ first,
                                                              Chunks chunks, int count, int E, int S, int SP,
                                                              bool backwards, float *__restrict__ end) {
     const long i = (long)blockIdx.x * kThreads + threadIdx.x;
@@ -486,10 +497,10 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     constexpr int STEPS = back_steps(LANES);
     constexpr int CH = kThreads / LANES, SP = kStates * LANES, EPT = Elements<LANES, STEPS>::EPT;
     constexpr int WAVES = kThreads / 64;
-    // d, d x, gy, and y without the skip; on the way back the first two give way
-    // to sum gh b and sum a gh k h (a channel's lanes lie in one wavefront, which
-    // has read a step before it overwrites it)
-    __shared__ float4 steps[STEPS][CH];
+    constexpr int PAD = padded(LANES);
+    __shared__ float4 steps[STEPS][CH];             // d, d x, gy, -
+    __shared__ float ys[STEPS][PAD];                // y without the skip
+    __shared__ float2 back[STEPS][PAD];             // sum gh b, sum a gh k h
     __shared__ __align__(16) float bc[STEPS][2 * SP];
     __shared__ float sums[WAVES][STEPS][2 * SP];   // gb, gc of a wavefront
     const Place w = place_of<LANES>(p, chunk_tiles);
@@ -608,7 +619,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
                 float r[StepSums<LANES>::kept];
                 StepSums<LANES>::add(y, q, r);
 #pragma unroll
-                for (int j = 0; j < StepSums<LANES>::kept; ++j) steps[j0 + StepSums<LANES>::step(q) + j][ch].w = r[j];
+                for (int j = 0; j < StepSums<LANES>::kept; ++j) ys[j0 + StepSums<LANES>::step(q) + j][ch] = r[j];
             }
         }
 #pragma unroll
@@ -643,20 +654,20 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
             StepSums<LANES>::add(akh, q, ra);
 #pragma unroll
             for (int j = 0; j < StepSums<LANES>::kept; ++j)
-                *reinterpret_cast<float2 *>(&steps[j0 + StepSums<LANES>::step(q) + j][ch]) = make_float2(rb[j], ra[j]);
+                back[j0 + StepSums<LANES>::step(q) + j][ch] = make_float2(rb[j], ra[j]);
         }
         __syncthreads();
         if (on) {
             float ox[EPT], od[EPT], oz[EPT];
 #pragma unroll
             for (int i = 0; i < EPT; ++i) {
-                const float4 s = steps[el.j][el.c + i];
-                ox[i] = fmaf(d[i], s.x, skip[i] * s.z);
+                const float2 s = back[el.j][el.c + i];
+                ox[i] = fmaf(d[i], s.x, skip[i] * steps[el.j][el.c + i].z);
                 od[i] = fmaf(xk[i], s.x, s.y) * slope[i];
                 if (i < have) gbias[i] += od[i];
                 if (gated) {
                     const float sg = sigmoid(zk[i]);
-                    oz[i] = uk[i] * fmaf(skip[i], xk[i], s.w) * (sg * fmaf(zk[i], 1.0f - sg, 1.0f));
+                    oz[i] = uk[i] * fmaf(skip[i], xk[i], ys[el.j][el.c + i]) * (sg * fmaf(zk[i], 1.0f - sg, 1.0f));
                 }
             }
             store_row<EPT>(gx + row, have, wide, ox);
@@ -894,8 +905,8 @@ int blocks_of(const warpctct_scan_t &p) {      // of a group
 template <typename IO>
 bool rows_wide(const warpctct_scan_t &p, int ept) {
     constexpr int V = kVec<IO>;
-    return p.E % V == 0 && (p.E / p.G) % V == 0 && (p.E / p.G) % ept == 0 && p.x_n % V == 0 && p.x_t % V == 0 && p.dt_n % V == 0 &&
-           p.dt_t % V == 0 && p.gate_n % V == 0 && p.gate_t % V == 0 && aligned16(p.x) && aligned16(p.dt) &&
+    return p.E % V == 0 && (p.E / p.G) % V == 0 && (p.E / p.G) % ept == 0 && p.x_n % V == 0 &&
+           p.x_t % V == 0 && p.dt_n % V == 0 && p.dt_t % V == 0 && p.gate_n % V == 0 && p.gate_t % V == 0 && aligned16(p.x) && aligned16(p.dt) &&
            aligned16(p.gate) && aligned16(p.out);
 }
 
@@ -955,7 +966,8 @@ hipError_t start(const warpctct_scan_t &p, float *keep, float *workspace, hipStr
         if (e != hipSuccess) return e;
     }
     auto kernel = scan_kernel<IO, LANES, false>;
-    TIMED_LAUNCH(kernel, grid, dim3(kThreads), 0, stream, p, keep, chunks, cut.count > 1 ? chunks.local : nullptr, wide);
+    TIMED_LAUNCH(kernel, grid, dim3(kThreads), 0, stream, p, keep, chunks, cut.count > 1 ? chunks.local : nullptr,
+                 wide);
     return hipGetLastError();
 }
 
@@ -963,7 +975,8 @@ template <typename IO, int LANES>
 hipError_t start(const warpctct_scan_t &p, const warpctct_scan_grad_t &g, const float *keep, float *part_bc,
                  float *part_sums, float *workspace, hipStream_t stream) {
     constexpr int V = kVec<IO>;
-    const bool wide = rows_wide<IO>(p, Elements<LANES, kSteps>::EPT) && g.grad_n % V == 0 && g.grad_t % V == 0 && aligned16(g.grad_out) &&
+    const bool wide = rows_wide<IO>(p, Elements<LANES, kSteps>::EPT) && g.grad_n % V == 0 &&
+                      g.grad_t % V == 0 && aligned16(g.grad_out) &&
                       aligned16(g.grad_x) && aligned16(g.grad_dt) && aligned16(g.grad_gate);
     const int blocks = blocks_of(p);
     if (p.N == 0) return hipSuccess;
