@@ -291,6 +291,19 @@ def test_refusals_on_the_gpu():
         torch.autograd.grad(warp_ctct.causal_conv(x, weight), [x], g, create_graph=True)
 
 
+@gpu
+def test_a_step_counts_up_the_version_of_its_state():
+    x, weight, bias, first, _, _ = make(2, 10, 8, 4, torch.float32)
+    state = torch.ones(2, 3, 8, device="cuda")
+    out = warp_ctct.causal_conv(x, weight, bias, initial_state=state)
+    with torch.no_grad():
+        warp_ctct.causal_conv_step(x[:, 0], state, weight, bias)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()      # the graph had saved the state
+    with torch.no_grad(), pytest.raises(RuntimeError, match="complex"):
+        warp_ctct.causal_conv_step(x[:, 0], state, weight.to(torch.complex64), bias)
+
+
 def test_refusals_without_a_gpu():
     with pytest.raises(RuntimeError, match="GPU"):
         warp_ctct.causal_conv(torch.zeros(1, 2, 3), torch.zeros(3, 4))

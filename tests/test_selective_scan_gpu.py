@@ -433,6 +433,17 @@ def test_refusals_on_the_gpu():
         torch.autograd.grad(case.call()[0], [case.args["x"]], case.g, create_graph=True)
 
 
+@gpu
+def test_a_step_counts_up_the_version_of_its_state():
+    x, b = torch.rand(2, 10, 8, device="cuda"), torch.rand(2, 10, 16, device="cuda")
+    a, state = -torch.rand(8, 16, device="cuda"), torch.ones(2, 8, 16, device="cuda")
+    out = warp_ctct.selective_scan(x.requires_grad_(True), x, a, b, b, initial_state=state)
+    with torch.no_grad():
+        warp_ctct.selective_scan_step(x[:, 0], state, x[:, 0], a, b[:, 0], b[:, 0])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()      # the graph had saved the state
+
+
 def test_refusals_without_a_gpu():
     t = torch.zeros
     with pytest.raises(RuntimeError, match="GPU"):

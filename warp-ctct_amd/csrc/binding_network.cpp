@@ -191,8 +191,8 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
 torch::Tensor layer_norm(const torch::Tensor &input, Maybe weight, Maybe bias, const double eps) {
     CHECK_DEVICE(input);
     TORCH_CHECK(input.dim() >= 1 && input.size(-1) >= 1, "layer_norm: the input needs a last dimension");
-    TORCH_CHECK(input.size(-1) < (1L << 30) && input.numel() / input.size(-1) < (1L << 31),
-                "layer_norm: at most 2^31 - 1 rows of fewer than 2^30 elements");
+    TORCH_CHECK(input.size(-1) <= (1L << 27) - 32 && input.numel() / input.size(-1) < (1L << 31),
+                "layer_norm: at most 2^31 - 1 rows of at most 2^27 - 32 elements");
     TORCH_CHECK(eps >= 0, "layer_norm: eps must not be negative");
     const torch::Tensor x = native(input);
     bool same = true;      // parameters in the input's type; otherwise all of them in float32
@@ -206,7 +206,7 @@ torch::Tensor layer_norm(const torch::Tensor &input, Maybe weight, Maybe bias, c
     }
     for (Maybe *p : {&weight, &bias})
         if (given(*p) && !((same || (*p)->scalar_type() == kFloat) && (*p)->is_contiguous()))
-            *p = (same ? **p : (*p)->to(kFloat)).contiguous();
+            *p = (same ? **p : native(**p).to(kFloat)).contiguous();
     const bool tx = tracked(x), tw = tracked(weight), tb = tracked(bias);
     if (tx || tw || tb) return LayerNorm::apply(x, weight, bias, eps, tx, tw, tb);
     NormCall call(x, given(weight) ? *weight : torch::Tensor(), given(bias) ? *bias : torch::Tensor(), eps);
@@ -242,7 +242,8 @@ torch::Tensor flags_of(const Maybe &advance, const torch::Tensor &x, const char 
     return advance->contiguous();
 }
 
-// A step updates its state in place and has no backward pass.
+// A step updates its state in place and has no backward pass.  (It counts up the
+// state's version first, so that a graph that saved the state refuses to use it.)
 void refuse_gradient(std::initializer_list<const Maybe *> inputs, const char *what) {
     for (const Maybe *t : inputs)
         TORCH_CHECK(!tracked(*t), what, ": not differentiable; call it under torch.no_grad()");
@@ -344,6 +345,7 @@ void check_taps(const torch::Tensor &weight, const Maybe &bias, const torch::Ten
     check_on(*bias, x, "bias");
 }
 torch::Tensor as_float(const torch::Tensor &t) {
+    TORCH_CHECK(!t.is_complex(), "complex tensors are not supported");
     return t.scalar_type() == kFloat && t.is_contiguous() ? t : t.to(kFloat).contiguous();
 }
 
@@ -354,8 +356,8 @@ tensor_list causal_conv(const torch::Tensor &input, const torch::Tensor &weight,
     const torch::Tensor x = dense_last(native(input));
     check_taps(weight, bias, x, "causal_conv");
     const int L = int_size(x, 1, "causal_conv"), E = int_size(x, 2, "causal_conv");
-    TORCH_CHECK(x.size(0) <= 65535 && static_cast<long>(L) * E < (1L << 38),
-                "causal_conv: at most 65535 sequences of fewer than 2^38 elements");
+    TORCH_CHECK(x.size(0) <= 65535 && L <= (1L << 30) && static_cast<long>(L) * E <= (1L << 32) - 1024,
+                "causal_conv: at most 65535 sequences of at most 2^30 steps and 2^32 - 1024 elements");
     ConvInputs in = {x, as_float(weight), given(bias) ? as_float(*bias) : torch::Tensor(),
                      lengths_of(lengths, x, "causal_conv"), torch::Tensor()};
     if (given(initial)) {
@@ -388,6 +390,7 @@ torch::Tensor causal_conv_step(const torch::Tensor &input, torch::Tensor state, 
     const torch::Tensor go = flags_of(advance, x, "causal_conv_step");
     const torch::Tensor w = as_float(weight), b = given(bias) ? as_float(*bias) : torch::Tensor();
     const DeviceGuard guard(device_of(x));
+    torch::autograd::impl::bump_version(state);
     auto out = fresh(x.sizes(), x);
     warpctct_conv_step_t p = {};
     p.dtype = type_of(x);
@@ -571,7 +574,7 @@ ScanInputs scan_inputs(const torch::Tensor &input, const torch::Tensor &dt, cons
                 what, ": a must be (channels, states) with 1 to ", static_cast<int>(WARPCTCT_SCAN_MAX_STATES),
                 " states");
     check_on(a, in.x, "a");
-    TORCH_CHECK(in.x.size(-1) <= (1 << 24), what, ": at most 2^24 channels");
+    TORCH_CHECK(in.x.size(-1) < (1 << 24), what, ": fewer than 2^24 channels");
     in.a = as_float(a);
     in.dt = like_input(dt, in.x, "dt", what);
     in.b = groups_of(b, in.x, a.size(1), "b", what);
@@ -628,6 +631,7 @@ torch::Tensor selective_scan_step(const torch::Tensor &input, torch::Tensor stat
     check_on(state, x, "state");
     const torch::Tensor go = flags_of(advance, x, what);
     const DeviceGuard guard(device_of(x));
+    torch::autograd::impl::bump_version(state);
     auto out = fresh(x.sizes(), x);
     warpctct_scan_step_t p = {};
     p.dtype = type_of(x);
@@ -674,7 +678,7 @@ struct Penalty {
                     " must be a number or one for each row");
         check_on(t, logits, name);
         refuse_if_tracked(t, name);
-        each = t.scalar_type() == kFloat && t.is_contiguous() ? t : t.to(kFloat).contiguous();
+        each = as_float(t);
     }
     static void refuse_if_tracked(const torch::Tensor &t, const char *name) {
         TORCH_CHECK(!tracked(t), "adjust_logits: not differentiable (", name, "); call it under torch.no_grad()");

@@ -2,13 +2,13 @@
 the rules put on the joiner's logits before a token is taken from them.
 
 The losses start from scores.  These are the operators on either side of them
-that a model of the same kind runs: :func:`layer_norm`,
-:func:`causal_conv` and :func:`selective_scan` for a prediction network or an
-encoder, in training and over prompts, :func:`causal_conv_step` and
-:func:`selective_scan_step` for decoding a token at a time;
-:func:`adjust_logits` before a token is taken.  Hand-written HIP kernels like the losses', through the same binding: float32, float16 and bfloat16 are
-read as they are (another type is converted to float32), sums and states are
-kept in float32, a result is rounded once.  Nothing synchronises with the host;
+that a model of the same kind runs: :func:`layer_norm`, :func:`causal_conv` and
+:func:`selective_scan` for a prediction network or an encoder, in training and
+over prompts, :func:`causal_conv_step` and :func:`selective_scan_step` for
+decoding a token at a time; :func:`adjust_logits` before a token is taken.
+Hand-written HIP kernels like the losses', through the same binding: float32,
+float16 and bfloat16 are read as they are (another type is converted to
+float32), sums and states are kept in float32, a result is rounded once.  Nothing synchronises with the host;
 work is enqueued on the current stream of the input's GPU.  A wrong shape, type
 or device raises RuntimeError.  The backward passes are not differentiable
 themselves (``create_graph=True`` raises).  Forward and backward can be captured
