@@ -519,7 +519,7 @@ int warpctct_joiner_linear_lattice(int from_frames);
  * x_inner_stride (x_inner_rows = rows for rows a fixed distance apart).  weight,
  * bias: width elements each of weight_dtype (that of x, or WARPCTCT_F32), or
  * NULL for 1 and 0.  out (rows, width) is dense.  stats: 3 * rows floats
- * that the backward pass reads, or NULL.  rows < 2^31. */
+ * that the backward pass reads, or NULL.  rows < 2^31, width <= 2^27 - 32. */
 typedef struct {
     int dtype, weight_dtype, width;
     float eps;
@@ -532,8 +532,8 @@ int warpctct_layer_norm(const warpctct_norm_t *p, void *stream);
 
 /* Gradients for grad_out, addressed like x by the three numbers in front of it:
  * grad_x (rows, width) dense in the type of x, grad_weight and grad_bias in
- * weight_dtype; each may be NULL.  `out`, `bias` and `eps` of p are not used.  The column sums are
- * added up in a fixed order, through `workspace`
+ * weight_dtype; each may be NULL.  `out`, `bias` and `eps` of p are not used.  The
+ * column sums are added up in a fixed order, through `workspace`
  * (warpctct_layer_norm_workspace_bytes, needed where grad_weight or grad_bias
  * is given). */
 typedef struct {
@@ -555,7 +555,8 @@ int warpctct_layer_norm_grad(const warpctct_norm_t *p, const warpctct_norm_grad_
  * others are not read, and out is zero there.  last (N, K-1, E), may be NULL:
  * the K-1 inputs before step lengths[n], the `initial` of a call that goes on
  * from there.  weight (E, K), bias (E, may be NULL): float.  out, initial, last:
- * dense, in the type of x.  N <= 65535. */
+ * dense, in the type of x.  N <= 65535, L <= 2^30, L E <= 2^32 - 1024,
+ * E (K + 1) <= 2^28 - 64. */
 enum { WARPCTCT_CONV_MAX_TAPS = 8 };
 typedef struct {
     int dtype, N, L, E, K, silu;
@@ -616,7 +617,8 @@ int warpctct_causal_conv_step(const warpctct_conv_step_t *p, void *stream);
  * backward pass) receives the states in front of every few steps.
  * workspace: warpctct_selective_scan_workspace_bytes(..., 0), 16-byte aligned (0
  * bytes, may be NULL, unless few long sequences are cut into chunks).
- * N <= 65535. */
+ * N <= 65535, L <= 2^30, E < 2^24, E (S + 2) <= 2^28 - 64,
+ * L G S <= 2^31 - 512. */
 enum { WARPCTCT_SCAN_MAX_STATES = 64 };
 typedef struct {
     int dtype, N, L, E, S, G, softplus;

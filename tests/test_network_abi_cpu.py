@@ -242,3 +242,16 @@ def test_selective_scan_gradient_and_step_arguments():
                 dict(b=None), dict(c=None), dict(state=None), dict(out=None)):
         assert step(**bad) == EINVAL, bad
     assert step(N=0, x=None, state=None) == 0
+
+
+def test_sizes_that_no_launch_holds():
+    lib = hip_lib.lib()
+    none = ctypes.c_size_t(0)
+    assert lib.warpctct_layer_norm(ctypes.byref(norm(width=(1 << 27) - 31)), P(0)) == EINVAL
+    for bad in (dict(L=(1 << 30) + 1, E=1), dict(L=1 << 20, E=1 << 12), dict(L=1, E=1 << 26, K=4)):
+        assert lib.warpctct_causal_conv(ctypes.byref(conv(**bad)), P(0)) == EINVAL, bad
+    p = ConvStep(dtype=F16, N=1 << 17, E=1 << 15, K=4, x=SOME, state=SOME, weight=SOME, out=SOME)
+    assert lib.warpctct_causal_conv_step(ctypes.byref(p), P(0)) == EINVAL
+    for bad in (dict(E=1 << 24, S=1, G=1), dict(E=1 << 23, S=64, G=1), dict(L=(1 << 30) + 1, E=1, S=1, G=1),
+                dict(L=1 << 20, E=32, S=64, G=32)):
+        assert lib.warpctct_selective_scan(ctypes.byref(scan(**bad)), P(0), none, P(0), none, P(0)) == EINVAL, bad

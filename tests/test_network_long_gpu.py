@@ -80,3 +80,18 @@ def test_adjust_logits():
     part = slice(N - 4, N)
     assert torch.equal(out[part], warp_ctct.adjust_logits(logits[part], tokens[part], repetition_penalty=1.5,
                                                           presence_penalty=0.5, bias=bias))
+
+
+def test_layer_norm_of_more_wide_rows_than_workgroups():
+    rows, width, many = 5, 8193, 2 ** 20 + 5      # rows in no multiple of a vector, a workgroup each
+    x, g = big(rows, width).half(), big(rows, width).half()
+    x[1:], g[1:] = x[0], g[0]
+    few, weight = leaf(x), leaf(torch.randn(width, device="cuda"))
+    small = warp_ctct.layer_norm(few, weight)
+    gsmall, = torch.autograd.grad(small, few, g)
+    row = leaf(x[:1])
+    out = warp_ctct.layer_norm(row.expand(many, width), weight)
+    assert bool((out[:5] == small).all()) and bool((out[many - 5:] == small).all())
+    wide = leaf(x[:1].expand(many, width))
+    gx, = torch.autograd.grad(warp_ctct.layer_norm(wide, weight), wide, g[:1].expand(many, width))
+    assert bool((gx[:5] == gsmall).all()) and bool((gx[many - 5:] == gsmall).all())

@@ -19,23 +19,26 @@ inline int done(hipError_t e) {
 
 constexpr long kMostRows = 0x7fffffffL;
 constexpr int kMostBatch = 65535;      // a grid dimension, as for the losses
+// A launch has fewer than 2^32 threads: the sums down columns take 16 a column,
+// other kernels one a value.
+constexpr long kMostColumns = (1L << 28) - 64, kMostThreads = (1L << 32) - 1024;
 
 bool norm_ok(const warpctct_norm_t *p) {
     return p && io_valid(p->dtype) && (p->weight_dtype == p->dtype || p->weight_dtype == WARPCTCT_F32) &&
-           p->width >= 1 && p->width <= 0x3fffffff && p->rows >= 0 && p->rows <= kMostRows &&
+           p->width >= 1 && 2L * p->width <= kMostColumns && p->rows >= 0 && p->rows <= kMostRows &&
            (p->rows == 0 || (p->x && p->x_inner_rows >= 1));
 }
 
 bool conv_ok(const warpctct_conv_t *p) {
     return p && io_valid(p->dtype) && p->N >= 0 && p->N <= kMostBatch && p->L >= 0 && p->E >= 1 && p->K >= 1 &&
-           p->K <= WARPCTCT_CONV_MAX_TAPS && (long)p->E * (p->K + 1) < (1L << 30) && (long)p->L * p->E < (1L << 38) &&
-           (p->N == 0 || (p->weight && (p->x || p->L == 0)));
+           p->K <= WARPCTCT_CONV_MAX_TAPS && (long)p->E * (p->K + 1) <= kMostColumns && p->L <= (1 << 30) &&
+           (long)p->L * p->E <= kMostThreads && (p->N == 0 || (p->weight && (p->x || p->L == 0)));
 }
 
 bool scan_sizes_ok(int dtype, int N, int L, int E, int S, int G) {
-    return io_valid(dtype) && N >= 0 && N <= kMostBatch && L >= 0 && E >= 1 && E <= (1 << 24) && S >= 1 &&
-           S <= WARPCTCT_SCAN_MAX_STATES && G >= 1 && E % G == 0 && (long)L * G * S < (1L << 36) &&
-           L <= (1 << 30);
+    return io_valid(dtype) && N >= 0 && N <= kMostBatch && L >= 0 && E >= 1 && E < (1 << 24) && S >= 1 &&
+           S <= WARPCTCT_SCAN_MAX_STATES && G >= 1 && E % G == 0 && 2L * L * G * S <= kMostThreads &&
+           (long)E * (S + 2) <= kMostColumns && L <= (1 << 30);
 }
 bool scan_ok(const warpctct_scan_t *p) {
     return p && scan_sizes_ok(p->dtype, p->N, p->L, p->E, p->S, p->G) &&
@@ -103,7 +106,7 @@ int warpctct_causal_conv_grad(const warpctct_conv_t *p, const warpctct_conv_grad
 
 int warpctct_causal_conv_step(const warpctct_conv_step_t *p, void *stream) {
     if (!p || !io_valid(p->dtype) || p->N < 0 || p->E < 1 || p->K < 1 || p->K > WARPCTCT_CONV_MAX_TAPS ||
-        (long)p->N * p->E >= (1L << 38))
+        (long)p->N * p->E > kMostThreads)
         return WARPCTCT_EINVAL;
     if (p->N == 0) return WARPCTCT_OK;
     if (!p->x || !p->weight || !p->out || (p->K > 1 && !p->state)) return WARPCTCT_EINVAL;

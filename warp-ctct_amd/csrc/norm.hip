@@ -22,6 +22,7 @@ namespace {
 constexpr int kThreads = 256;        // of a workgroup whose wavefronts take a row each
 constexpr int kWide = 1024;          // the largest number of threads on one row
 constexpr unsigned kGroups = 1024;   // workgroups of the forward pass, at most
+constexpr unsigned kWideGroups = 1u << 20;      // and where a row does not fit into their registers
 // and of the backward pass: four on a compute unit where they take a row each, two
 // where their wavefronts do (12800 rows of 2048 elements: 36.6 us with 1024, 42.0
 // with 512; 2592 rows of 641: 16.2 with 1024, 11.4 with 512)
@@ -171,33 +172,37 @@ __global__ __launch_bounds__(BLOCK) void norm_kernel(const IO *__restrict__ x, R
 }
 
 // Rows too wide for the registers of one workgroup: three passes over the row.
+// (As in the backward pass, a workgroup takes more rows than one where there are
+// more than a launch has workgroups.)
 template <typename IO, typename W>
 __global__ __launch_bounds__(kWide) void norm_wide_kernel(const IO *__restrict__ x, RowAddress at,
                                                           const W *__restrict__ weight,
                                                           const W *__restrict__ bias, float eps,
-                                                          IO *__restrict__ out, float *__restrict__ stats, int width) {
+                                                          IO *__restrict__ out, float *__restrict__ stats, unsigned rows,
+                                                          int width) {
     __shared__ float shared[2 * kWide / 64];
-    const unsigned row = blockIdx.x;
-    const IO *in = x + at.at(row);
     const float inv = 1.0f / (float)width;
-    float sum = 0.0f, none = 0.0f;
-    for (int k = threadIdx.x; k < width; k += kWide) sum += to_float(in[k]);
-    row_sums(sum, none, kWide, shared);
-    const float m = sum * inv;
-    float off = 0.0f, sq = 0.0f;
-    for (int k = threadIdx.x; k < width; k += kWide) {
-        const float d = to_float(in[k]) - m;
-        off += d;
-        sq = fmaf(d, d, sq);
-    }
-    row_sums(off, sq, kWide, shared);
-    const float c = off * inv;
-    const float r = 1.0f / sqrtf(fmaxf(sq * inv - c * c, 0.0f) + eps);
-    if (stats && threadIdx.x == 0) keep_stats(stats, row, m, c, r);
-    for (int k = threadIdx.x; k < width; k += kWide) {
-        float v = (to_float(in[k]) - m - c) * r * (weight ? to_float(weight[k]) : 1.0f);
-        if (bias) v += to_float(bias[k]);
-        out[(long)row * width + k] = from_float<IO>(v);
+    for (unsigned row = blockIdx.x; row < rows; row += gridDim.x) {
+        const IO *in = x + at.at(row);
+        float sum = 0.0f, none = 0.0f;
+        for (int k = threadIdx.x; k < width; k += kWide) sum += to_float(in[k]);
+        row_sums(sum, none, kWide, shared);
+        const float m = sum * inv;
+        float off = 0.0f, sq = 0.0f;
+        for (int k = threadIdx.x; k < width; k += kWide) {
+            const float d = to_float(in[k]) - m;
+            off += d;
+            sq = fmaf(d, d, sq);
+        }
+        row_sums(off, sq, kWide, shared);
+        const float c = off * inv;
+        const float r = 1.0f / sqrtf(fmaxf(sq * inv - c * c, 0.0f) + eps);
+        if (stats && threadIdx.x == 0) keep_stats(stats, row, m, c, r);
+        for (int k = threadIdx.x; k < width; k += kWide) {
+            float v = (to_float(in[k]) - m - c) * r * (weight ? to_float(weight[k]) : 1.0f);
+            if (bias) v += to_float(bias[k]);
+            out[(long)row * width + k] = from_float<IO>(v);
+        }
     }
 }
 
@@ -286,24 +291,25 @@ template <typename IO, typename W>
 __global__ __launch_bounds__(kWide) void norm_wide_grad_kernel(
     const IO *__restrict__ x, RowAddress x_at, const IO *__restrict__ g, RowAddress g_at,
     const W *__restrict__ weight, const float *__restrict__ stats,
-    IO *__restrict__ gx, int width) {
+    IO *__restrict__ gx, unsigned rows, int width) {
     __shared__ float shared[2 * kWide / 64];
-    const unsigned row = blockIdx.x;
-    const IO *in = x + x_at.at(row), *up = g + g_at.at(row);
     const float inv = 1.0f / (float)width;
-    const RowStats s = row_stats(stats, row);
-    float su = 0.0f, suh = 0.0f;
-    for (int k = threadIdx.x; k < width; k += kWide) {
-        const float u = to_float(up[k]) * (weight ? to_float(weight[k]) : 1.0f);
-        su += u;
-        suh = fmaf(u, s.normalise(to_float(in[k])), suh);
-    }
-    row_sums(su, suh, kWide, shared);
-    su *= inv;
-    suh *= inv;
-    for (int k = threadIdx.x; k < width; k += kWide) {
-        const float u = to_float(up[k]) * (weight ? to_float(weight[k]) : 1.0f);
-        gx[(long)row * width + k] = from_float<IO>(s.r * (u - su - s.normalise(to_float(in[k])) * suh));
+    for (unsigned row = blockIdx.x; row < rows; row += gridDim.x) {
+        const IO *in = x + x_at.at(row), *up = g + g_at.at(row);
+        const RowStats s = row_stats(stats, row);
+        float su = 0.0f, suh = 0.0f;
+        for (int k = threadIdx.x; k < width; k += kWide) {
+            const float u = to_float(up[k]) * (weight ? to_float(weight[k]) : 1.0f);
+            su += u;
+            suh = fmaf(u, s.normalise(to_float(in[k])), suh);
+        }
+        row_sums(su, suh, kWide, shared);
+        su *= inv;
+        suh *= inv;
+        for (int k = threadIdx.x; k < width; k += kWide) {
+            const float u = to_float(up[k]) * (weight ? to_float(weight[k]) : 1.0f);
+            gx[(long)row * width + k] = from_float<IO>(s.r * (u - su - s.normalise(to_float(in[k])) * suh));
+        }
     }
 }
 template <typename IO>
@@ -373,9 +379,10 @@ hipError_t start(const warpctct_norm_t &p, hipStream_t stream) {
     const int threads = threads_for(p.width, false, vec);
     if (threads == 0) {
         auto kernel = norm_wide_kernel<IO, W>;
-        TIMED_LAUNCH(kernel, dim3((unsigned)p.rows), dim3(kWide), 0, stream, static_cast<const IO *>(p.x), at,
-                     static_cast<const W *>(p.weight), static_cast<const W *>(p.bias), p.eps,
-                     static_cast<IO *>(p.out), p.stats, p.width);
+        const unsigned rows = (unsigned)p.rows;
+        TIMED_LAUNCH(kernel, dim3(rows < kWideGroups ? rows : kWideGroups), dim3(kWide), 0, stream,
+                     static_cast<const IO *>(p.x), at, static_cast<const W *>(p.weight),
+                     static_cast<const W *>(p.bias), p.eps, static_cast<IO *>(p.out), p.stats, rows, p.width);
         return hipGetLastError();
     }
     if (threads == kWide)
@@ -411,18 +418,18 @@ hipError_t start_grad(const warpctct_norm_t &p, const warpctct_norm_grad_t &g, f
                      (reinterpret_cast<uintptr_t>(g.grad_x) & 15u) == 0;
     const int threads = threads_for(p.width, true, vec);
     if (threads == 0) {
+        const unsigned rows = (unsigned)p.rows;
         if (g.grad_x) {
             auto kernel = norm_wide_grad_kernel<IO, W>;
-            TIMED_LAUNCH(kernel, dim3((unsigned)p.rows), dim3(kWide), 0, stream, static_cast<const IO *>(p.x), x_at,
-                         static_cast<const IO *>(g.grad_out), g_at, static_cast<const W *>(p.weight), p.stats,
-                         static_cast<IO *>(g.grad_x), p.width);
+            TIMED_LAUNCH(kernel, dim3(rows < kWideGroups ? rows : kWideGroups), dim3(kWide), 0, stream,
+                         static_cast<const IO *>(p.x), x_at, static_cast<const IO *>(g.grad_out), g_at,
+                         static_cast<const W *>(p.weight), p.stats, static_cast<IO *>(g.grad_x), rows, p.width);
         }
         if (partial) {
             auto kernel = norm_wide_columns_kernel<IO>;
             const dim3 grid((p.width + kThreads - 1) / kThreads, norm_grad_groups(p.rows, p.width));
             TIMED_LAUNCH(kernel, grid, dim3(kThreads), 0, stream, static_cast<const IO *>(p.x), x_at,
-                         static_cast<const IO *>(g.grad_out), g_at, p.stats, partial, (unsigned)p.rows,
-                         p.width);
+                         static_cast<const IO *>(g.grad_out), g_at, p.stats, partial, rows, p.width);
         }
         return hipGetLastError();
     }

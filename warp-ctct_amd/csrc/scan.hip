@@ -906,8 +906,8 @@ template <typename IO>
 bool rows_wide(const warpctct_scan_t &p, int ept) {
     constexpr int V = kVec<IO>;
     return p.E % V == 0 && (p.E / p.G) % V == 0 && (p.E / p.G) % ept == 0 && p.x_n % V == 0 &&
-           p.x_t % V == 0 && p.dt_n % V == 0 && p.dt_t % V == 0 && p.gate_n % V == 0 && p.gate_t % V == 0 && aligned16(p.x) && aligned16(p.dt) &&
-           aligned16(p.gate) && aligned16(p.out);
+           p.x_t % V == 0 && p.dt_n % V == 0 && p.dt_t % V == 0 && p.gate_n % V == 0 && p.gate_t % V == 0 &&
+           aligned16(p.x) && aligned16(p.dt) && aligned16(p.gate) && aligned16(p.out);
 }
 
 // Chunks that a sequence is cut into.  Two passes cost twice the arithmetic
