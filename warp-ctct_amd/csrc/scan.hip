@@ -28,9 +28,9 @@
 // states; the reverse recurrence of gh alike.
 //
 // Measured with 16 states, bfloat16 and a gate: 32 ragged sequences of up to 400
-// steps, 1024 channels: forward 62 us, backward 155 us, of which the vector units
-// cannot do without 38 and 109 (SQ_ACTIVE_INST_VALU); one sequence of 16384 steps,
-// 2048 channels: 245 us in two passes, 224 of them the vector units'; one step of
+// steps, 1024 channels: forward 58 us, backward 147 us, of which the vector units
+// cannot do without 39 and 112 (SQ_ACTIVE_INST_VALU); one sequence of 16384 steps,
+// 2048 channels: 242 us in two passes, 224 of them the vector units'; one step of
 // 256 sequences, 2048 channels: 12.6 us, 5.6 TB/s.
 #include <algorithm>
 #include <cmath>
@@ -53,7 +53,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Steps of a tile of the backward pass, which is also how far apart the states
 // lie that the forward pass keeps for it: the states and factors of a tile take
 // 8 registers a step, and a thread has up to 4 elements.  With 8 steps the kernel
-// takes 188 registers, two wavefronts on a SIMD; with 16 it spilled (training on
+// takes 184 registers, two wavefronts on a SIMD; with 16 it spilled (training on
 // the sequences above: 708 us instead of 392 at the time).
 constexpr int back_steps(int lanes) { return lanes == 1 ? 4 : lanes == 16 ? 16 : 8; }
 
@@ -61,6 +61,13 @@ constexpr int back_steps(int lanes) { return lanes == 1 ? 4 : lanes == 16 ? 16 :
 // time: as far apart as a wavefront's channels, so that the four fall into
 // different banks.
 constexpr int padded(int lanes) { return kThreads / lanes + 64 / lanes; }
+
+// Tiles in LDS at a time.  With two, a tile's results are formed while the next
+// tile is worked on, and one barrier a tile is enough; with few or many states they
+// take the LDS of the second or third workgroup of a compute unit (32 sequences
+// of 400 steps, 1024 channels, training, one / two: 16 states 271 / 264 us, 32
+// states 461 / 454; 64 states 861 / 866, forwards 180 / 182).
+constexpr int buffers(int lanes) { return lanes == 4 || lanes == 8 ? 2 : 1; }
 
 __device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
 
@@ -308,9 +315,10 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
                                                         const float *__restrict__ starts, bool wide) {
     constexpr int CH = kThreads / LANES, SP = kStates * LANES, EPT = Elements<LANES, kSteps>::EPT;
     constexpr int PAD = padded(LANES);
-    __shared__ float2 steps[kSteps][CH];           // d, d x
-    __shared__ __align__(16) float bc[kSteps][2 * SP];
-    __shared__ float ys[kSteps][CARRY ? 1 : PAD];
+    constexpr int BUFS = buffers(LANES);
+    __shared__ float2 steps[BUFS][kSteps][CH];     // d, d x
+    __shared__ __align__(16) float bc[BUFS][kSteps][2 * SP];
+    __shared__ float ys[CARRY ? 1 : BUFS][kSteps][CARRY ? 1 : PAD];
     constexpr int BACK = back_steps(LANES);
     const Place w = place_of<LANES>(p, chunks.tiles);
     const Elements<LANES, kSteps> el;
@@ -361,23 +369,42 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
         sides.load(t0, w.len);
         sides.advance(kSteps);
     };
+    // the results of a tile whose sums are in ys
+    Row xk, zk;
+    bool on = false;
+    auto emit = [&](int buf) {
+        if (on) {
+            float o[EPT];
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) {
+                o[i] = fmaf(skip[i], xk[i], ys[buf][el.j][el.c + i]);
+                if (gated) o[i] *= zk[i] * sigmoid(zk[i]);
+            }
+            store_row<EPT>(out, have, wide, o);
+        }
+        out += (long)kSteps * p.E;
+    };
     if (w.from < w.to) request(w.from);
+    int buf = 0;
     for (int t0 = w.from; t0 < w.to; t0 += kSteps) {
-        const bool on = t0 + el.j < w.to;
+        const bool counts = t0 + el.j < w.to;
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
             float v = d[i] + bias[i];
             if (p.softplus) v = softplus(v).value;
-            const bool in = on && i < have;         // otherwise a step that leaves the state as it is
+            const bool in = counts && i < have;     // otherwise a step that leaves the state as it is
             v = in ? v : 0.0f;
-            steps[el.j][el.c + i] = make_float2(v, in ? v * x[i] : 0.0f);
+            steps[buf][el.j][el.c + i] = make_float2(v, in ? v * x[i] : 0.0f);
         }
-        const Row xk = x, zk = z;
-        sides.put(bc, t0, w.len);
+        sides.put(bc[buf], t0, w.len);
         __syncthreads();
+        if (!CARRY && BUFS == 2 && t0 > w.from) emit(buf ^ 1);
+        on = counts;
+        xk = x;
+        zk = z;
         if (t0 + kSteps < w.to) request(t0 + kSteps);
         Four f[2];
-        load_four<LANES, !CARRY>(f[0], steps, bc, 0, ch, q);
+        load_four<LANES, !CARRY>(f[0], steps[buf], bc[buf], 0, ch, q);
 #pragma unroll
         for (int j0 = 0; j0 < kSteps; j0 += 4) {
             if (t0 + j0 >= w.to) break;
@@ -386,7 +413,7 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
                     keep + (((long)w.n * ((p.L + BACK - 1) / BACK) + (t0 + j0) / BACK) * p.E + e) * SP + q * kStates) =
                     make_float4(h[0], h[1], h[2], h[3]);
             const Four &g = f[(j0 / 4) & 1];
-            if (j0 + 4 < kSteps) load_four<LANES, !CARRY>(f[(j0 / 4 + 1) & 1], steps, bc, j0 + 4, ch, q);
+            if (j0 + 4 < kSteps) load_four<LANES, !CARRY>(f[(j0 / 4 + 1) & 1], steps[buf], bc[buf], j0 + 4, ch, q);
             float y[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -404,20 +431,19 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
                 // (with more than four lanes a channel, groups of four write the same)
 #pragma unroll
                 for (int j = 0; j < StepSums<LANES>::kept; ++j)
-                    ys[j0 + StepSums<LANES>::step(q) + j][ch] = r[j];
+                    ys[buf][j0 + StepSums<LANES>::step(q) + j][ch] = r[j];
             }
         }
+        if (BUFS == 1) {
+            __syncthreads();
+            if (!CARRY) emit(0);
+        } else {
+            buf ^= 1;
+        }
+    }
+    if (!CARRY && BUFS == 2 && w.from < w.to) {
         __syncthreads();
-        if (!CARRY && on) {
-            float o[EPT];
-#pragma unroll
-            for (int i = 0; i < EPT; ++i) {
-                o[i] = fmaf(skip[i], xk[i], ys[el.j][el.c + i]);
-                if (gated) o[i] *= zk[i] * sigmoid(zk[i]);
-            }
-            store_row<EPT>(out, have, wide, o);
-        }
-        out += (long)kSteps * p.E;
+        emit(buf ^ 1);
     }
     if (CARRY) {
         if (live) {
@@ -498,11 +524,12 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     constexpr int CH = kThreads / LANES, SP = kStates * LANES, EPT = Elements<LANES, STEPS>::EPT;
     constexpr int WAVES = kThreads / 64;
     constexpr int PAD = padded(LANES);
-    __shared__ float4 steps[STEPS][CH];             // d, d x, gy, -
-    __shared__ float ys[STEPS][PAD];                // y without the skip
-    __shared__ float2 back[STEPS][PAD];             // sum gh b, sum a gh k h
-    __shared__ __align__(16) float bc[STEPS][2 * SP];
-    __shared__ float sums[WAVES][STEPS][2 * SP];   // gb, gc of a wavefront
+    constexpr int BUFS = buffers(LANES);
+    __shared__ float4 steps[BUFS][STEPS][CH];       // d, d x, gy, -
+    __shared__ float ys[BUFS][STEPS][PAD];          // y without the skip
+    __shared__ float2 back[BUFS][STEPS][PAD];       // sum gh b, sum a gh k h
+    __shared__ __align__(16) float bc[BUFS][STEPS][2 * SP];
+    __shared__ float sums[BUFS][WAVES][STEPS][2 * SP];     // gb, gc of a wavefront
     const Place w = place_of<LANES>(p, chunk_tiles);
     const Elements<LANES, STEPS> el;
     const int ch = threadIdx.x / LANES, q = threadIdx.x % LANES, e = w.first + ch;
@@ -573,30 +600,72 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
         us.shift(past);
         zs.shift(past);
     }
+    // the results of a tile whose sums are in `back`, `ys` and `sums`
+    float d[EPT], slope[EPT];
+    Row xk, uk, zk;
+    bool on = false;
+    auto emit = [&](int buf, int tile) {
+        if (on) {
+            float ox[EPT], od[EPT], oz[EPT];
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) {
+                const float2 s = back[buf][el.j][el.c + i];
+                ox[i] = fmaf(d[i], s.x, skip[i] * steps[buf][el.j][el.c + i].z);
+                od[i] = fmaf(xk[i], s.x, s.y) * slope[i];
+                if (i < have) gbias[i] += od[i];
+                if (gated) {
+                    const float sg = sigmoid(zk[i]);
+                    oz[i] = uk[i] * fmaf(skip[i], xk[i], ys[buf][el.j][el.c + i]) *
+                            (sg * fmaf(zk[i], 1.0f - sg, 1.0f));
+                }
+            }
+            store_row<EPT>(gx + row, have, wide, ox);
+            store_row<EPT>(gd + row, have, wide, od);
+            if (gz) store_row<EPT>(gz + row, have, wide, oz);
+        }
+        row -= (long)STEPS * p.E;
+        float *to = part_bc + (((long)w.n * gridDim.x + w.block) * tiles + tile) * (STEPS * 2 * SP);
+        for (int at = threadIdx.x; at < STEPS * 2 * SP; at += kThreads) {
+            float s = 0.0f;
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) s += sums[buf][v][at / (2 * SP)][at % (2 * SP)];
+            to[at] = s;
+        }
+    };
+    int buf = 0;
     for (int tile = top; tile >= bottom; --tile) {
-        const bool on = tile * STEPS + el.j < w.to;
-        float d[EPT], slope[EPT];
+        const bool counts = tile * STEPS + el.j < w.to;
+        float dk[EPT], slopek[EPT];
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
             const float v = raw[i] + bias[i];
-            d[i] = v;
-            slope[i] = 1.0f;
+            dk[i] = v;
+            slopek[i] = 1.0f;
             if (p.softplus) {
                 const Softplus s = softplus(v);
-                d[i] = s.value;
-                slope[i] = s.slope;
+                dk[i] = s.value;
+                slopek[i] = s.slope;
             }
             float gy = u[i], xi = x[i];
             if (gated) gy *= z[i] * sigmoid(z[i]);
-            if (!(on && i < have)) d[i] = gy = xi = 0.0f;
-            steps[el.j][el.c + i] = make_float4(d[i], d[i] * xi, gy, 0.0f);
+            if (!(counts && i < have)) dk[i] = gy = xi = 0.0f;
+            steps[buf][el.j][el.c + i] = make_float4(dk[i], dk[i] * xi, gy, 0.0f);
             gskip[i] = fmaf(gy, xi, gskip[i]);
         }
-        const Row xk = x, uk = u, zk = z;
-        sides.put(bc, tile * STEPS, w.len);
+        sides.put(bc[buf], tile * STEPS, w.len);
         const float h0[kStates] = {live ? front.x : 0.0f, live ? front.y : 0.0f, live ? front.z : 0.0f,
                                    live ? front.w : 0.0f};
         __syncthreads();
+        if (BUFS == 2 && tile < top) emit(buf ^ 1, tile + 1);
+        on = counts;
+        xk = x;
+        uk = u;
+        zk = z;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+            d[i] = dk[i];
+            slope[i] = slopek[i];
+        }
         if (tile > bottom) request(tile - 1);
         float k[STEPS][kStates], h[STEPS][kStates];
 #pragma unroll
@@ -604,22 +673,22 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
             float y[4];
 #pragma unroll
             for (int j = j0; j < j0 + 4; ++j) {
-                const float2 s = *reinterpret_cast<const float2 *>(&steps[j][ch]);
-                const float4 b4 = *reinterpret_cast<const float4 *>(&bc[j][q * kStates]);
+                const float2 s = *reinterpret_cast<const float2 *>(&steps[buf][j][ch]);
+                const float4 b4 = *reinterpret_cast<const float4 *>(&bc[buf][j][q * kStates]);
                 const float b[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
                 for (int i = 0; i < kStates; ++i) {
                     k[j][i] = exp2_hw(s.x * (a[i] * kLog2e));
                     h[j][i] = fmaf(k[j][i], j ? h[j - 1][i] : h0[i], s.y * b[i]);
                 }
-                const float4 c4 = *reinterpret_cast<const float4 *>(&bc[j][SP + q * kStates]);
+                const float4 c4 = *reinterpret_cast<const float4 *>(&bc[buf][j][SP + q * kStates]);
                 y[j - j0] = fmaf(c4.w, h[j][3], fmaf(c4.z, h[j][2], fmaf(c4.y, h[j][1], c4.x * h[j][0])));
             }
             if (gated) {
                 float r[StepSums<LANES>::kept];
                 StepSums<LANES>::add(y, q, r);
 #pragma unroll
-                for (int j = 0; j < StepSums<LANES>::kept; ++j) ys[j0 + StepSums<LANES>::step(q) + j][ch] = r[j];
+                for (int j = 0; j < StepSums<LANES>::kept; ++j) ys[buf][j0 + StepSums<LANES>::step(q) + j][ch] = r[j];
             }
         }
 #pragma unroll
@@ -627,9 +696,9 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
             float ghb[4], akh[4];
 #pragma unroll
             for (int j = j0 + 3; j >= j0; --j) {
-                const float4 s = steps[j][ch];
-                const float4 b4 = *reinterpret_cast<const float4 *>(&bc[j][q * kStates]);
-                const float4 c4 = *reinterpret_cast<const float4 *>(&bc[j][SP + q * kStates]);
+                const float4 s = steps[buf][j][ch];
+                const float4 b4 = *reinterpret_cast<const float4 *>(&bc[buf][j][q * kStates]);
+                const float4 c4 = *reinterpret_cast<const float4 *>(&bc[buf][j][SP + q * kStates]);
                 const float b[4] = {b4.x, b4.y, b4.z, b4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
                 float vb[kStates], vc[kStates];
                 ghb[j - j0] = akh[j - j0] = 0.0f;
@@ -646,42 +715,26 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
                 }
                 const float sb = sum_over_channels<LANES>(vb), sc = sum_over_channels<LANES>(vc);
                 // (lanes of a row that hold the same sum write it to the same place)
-                sums[wave][j][s_at] = sb;
-                sums[wave][j][SP + s_at] = sc;
+                sums[buf][wave][j][s_at] = sb;
+                sums[buf][wave][j][SP + s_at] = sc;
             }
             float rb[StepSums<LANES>::kept], ra[StepSums<LANES>::kept];
             StepSums<LANES>::add(ghb, q, rb);
             StepSums<LANES>::add(akh, q, ra);
 #pragma unroll
             for (int j = 0; j < StepSums<LANES>::kept; ++j)
-                back[j0 + StepSums<LANES>::step(q) + j][ch] = make_float2(rb[j], ra[j]);
+                back[buf][j0 + StepSums<LANES>::step(q) + j][ch] = make_float2(rb[j], ra[j]);
         }
+        if (BUFS == 1) {
+            __syncthreads();
+            emit(0, tile);
+        } else {
+            buf ^= 1;
+        }
+    }
+    if (BUFS == 2 && top >= bottom) {
         __syncthreads();
-        if (on) {
-            float ox[EPT], od[EPT], oz[EPT];
-#pragma unroll
-            for (int i = 0; i < EPT; ++i) {
-                const float2 s = back[el.j][el.c + i];
-                ox[i] = fmaf(d[i], s.x, skip[i] * steps[el.j][el.c + i].z);
-                od[i] = fmaf(xk[i], s.x, s.y) * slope[i];
-                if (i < have) gbias[i] += od[i];
-                if (gated) {
-                    const float sg = sigmoid(zk[i]);
-                    oz[i] = uk[i] * fmaf(skip[i], xk[i], ys[el.j][el.c + i]) * (sg * fmaf(zk[i], 1.0f - sg, 1.0f));
-                }
-            }
-            store_row<EPT>(gx + row, have, wide, ox);
-            store_row<EPT>(gd + row, have, wide, od);
-            if (gz) store_row<EPT>(gz + row, have, wide, oz);
-        }
-        row -= (long)STEPS * p.E;
-        float *to = part_bc + (((long)w.n * gridDim.x + w.block) * tiles + tile) * (STEPS * 2 * SP);
-        for (int at = threadIdx.x; at < STEPS * 2 * SP; at += kThreads) {
-            float s = 0.0f;
-#pragma unroll
-            for (int v = 0; v < WAVES; ++v) s += sums[v][at / (2 * SP)][at % (2 * SP)];
-            to[at] = s;
-        }
+        emit(buf ^ 1, bottom);
     }
     if (g.grad_initial && !starts && live) {
 #pragma unroll
@@ -697,15 +750,15 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) steps[el.j][el.c + i] = make_float4(gskip[i], gbias[i], 0.0f, 0.0f);
+    for (int i = 0; i < EPT; ++i) steps[0][el.j][el.c + i] = make_float4(gskip[i], gbias[i], 0.0f, 0.0f);
     __syncthreads();
     for (int c = threadIdx.x; c < CH; c += kThreads) {
         if (w.first + c >= w.end) continue;
         float s = 0.0f, b = 0.0f;
 #pragma unroll
         for (int j = 0; j < STEPS; ++j) {
-            s += steps[j][c].x;
-            b += steps[j][c].y;
+            s += steps[0][j][c].x;
+            b += steps[0][j][c].y;
         }
         mine[(long)p.E * p.S + w.first + c] = s;
         mine[(long)p.E * p.S + p.E + w.first + c] = b;
