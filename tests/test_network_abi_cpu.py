@@ -255,3 +255,20 @@ def test_sizes_that_no_launch_holds():
     for bad in (dict(E=1 << 24, S=1, G=1), dict(E=1 << 23, S=64, G=1), dict(L=(1 << 30) + 1, E=1, S=1, G=1),
                 dict(L=1 << 20, E=32, S=64, G=32)):
         assert lib.warpctct_selective_scan(ctypes.byref(scan(**bad)), P(0), none, P(0), none, P(0)) == EINVAL, bad
+
+
+def test_the_scans_gradient_of_no_steps_takes_scratch_too():
+    # the parameters' partial sums (zeros) go through it where there are sequences
+    lib = hip_lib.lib()
+    size = lib.warpctct_selective_scan_workspace_bytes
+    size.restype = ctypes.c_size_t
+    need = size(2, 0, 8, 16, 2, 1)
+    assert need > 0 and size(0, 20, 8, 16, 2, 1) == 0
+    grads = ScanGrad(grad_a=SOME)
+
+    def call(workspace, have):
+        return lib.warpctct_selective_scan_grad(ctypes.byref(scan(L=0)), ctypes.byref(grads), P(0), ctypes.c_size_t(0),
+                                                P(workspace), ctypes.c_size_t(have), P(0))
+
+    assert call(0, need) == EINVAL and call(0, 0) == EINVAL
+    assert call(ALIGNED, need - 1) == EWORKSPACE

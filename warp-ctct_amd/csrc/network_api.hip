@@ -155,12 +155,13 @@ int warpctct_selective_scan_grad(const warpctct_scan_t *p, const warpctct_scan_g
                                  size_t keep_bytes, void *workspace, size_t workspace_bytes, void *stream) {
     if (!scan_ok(p) || !g || !g->grad_a) return WARPCTCT_EINVAL;
     if (p->N > 0 && p->L > 0 &&
-        (!g->grad_out || !g->grad_x || !g->grad_dt || !g->grad_b || !g->grad_c || (p->gate && !g->grad_gate) || !keep ||
-         !workspace))
+        (!g->grad_out || !g->grad_x || !g->grad_dt || !g->grad_b || !g->grad_c || (p->gate && !g->grad_gate) || !keep))
         return WARPCTCT_EINVAL;
     if ((reinterpret_cast<uintptr_t>(keep) | reinterpret_cast<uintptr_t>(workspace)) & 15u) return WARPCTCT_EINVAL;
-    if (keep_bytes < scan_keep_floats(p->N, p->L, p->E, p->S) * sizeof(float) ||
-        workspace_bytes < scan_grad_floats(*p) * sizeof(float))
+    // (without steps too, the sequences' partial sums go through it)
+    const size_t need = scan_grad_floats(*p) * sizeof(float);
+    if (need > 0 && !workspace) return WARPCTCT_EINVAL;
+    if (keep_bytes < scan_keep_floats(p->N, p->L, p->E, p->S) * sizeof(float) || workspace_bytes < need)
         return WARPCTCT_EWORKSPACE;
     return done(launch_scan_grad(*p, *g, static_cast<const float *>(keep), static_cast<float *>(workspace),
                                  as_stream(stream)));
