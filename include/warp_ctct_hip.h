@@ -683,7 +683,7 @@ int warpctct_selective_scan_step(const warpctct_scan_step_t *p, void *stream);
  * values in front of them.  allowed: bytes, or with allowed_packed 32-bit words
  * of which bit v % 32 of word v / 32 is that of column v; row n allowed_n bytes
  * or words further on (0: one for all rows); NULL: everything.  A row that
- * allows nothing is -infinity throughout.  N <= 65535, V <= 2^30. */
+ * allows nothing is -infinity throughout.  N <= 65535, V <= 2^30, H <= 2^30. */
 typedef struct {
     int dtype, N, V, H, tokens_64, bias_dtype, allowed_packed;
     float repetition, presence, frequency;

@@ -272,3 +272,11 @@ def test_the_scans_gradient_of_no_steps_takes_scratch_too():
 
     assert call(0, need) == EINVAL and call(0, 0) == EINVAL
     assert call(ALIGNED, need - 1) == EWORKSPACE
+
+
+def test_histories_that_no_index_holds():
+    # a workgroup walks over the history in steps of its 256 threads, counted in 32 bits
+    lib = hip_lib.lib()
+    for H in ((1 << 30) + 1, (1 << 31) - 1):
+        p = Adjust(dtype=F32, N=2, V=8, H=H, repetition=1.0, logits_n=8, logits=SOME, out=SOME, tokens=SOME)
+        assert lib.warpctct_adjust_logits(ctypes.byref(p), P(0)) == EINVAL, H

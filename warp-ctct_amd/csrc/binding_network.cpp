@@ -713,8 +713,8 @@ torch::Tensor adjust_logits(const torch::Tensor &input, const Maybe &tokens, con
     if (given(tokens)) {
         const auto type = tokens->scalar_type();
         TORCH_CHECK(tokens->dim() == 2 && tokens->size(0) == N && !tokens->is_floating_point() &&
-                        type != at::ScalarType::Bool && tokens->size(1) <= 0x7fffffff,
-                    "adjust_logits: tokens must be whole numbers, (rows, history)");
+                        type != at::ScalarType::Bool && tokens->size(1) <= (1L << 30),
+                    "adjust_logits: tokens must be whole numbers, (rows, history), a history of at most 2^30");
         check_on(*tokens, x, "tokens");
         const bool taken = type == at::ScalarType::Int || type == at::ScalarType::Long;
         history = dense_last(taken ? *tokens : tokens->to(at::ScalarType::Int));

@@ -115,7 +115,7 @@ int warpctct_causal_conv_step(const warpctct_conv_step_t *p, void *stream) {
 
 int warpctct_adjust_logits(const warpctct_adjust_t *p, void *stream) {
     if (!p || !io_valid(p->dtype) || p->N < 0 || p->N > kMostBatch || p->V < 1 || p->V > (1 << 30) || p->H < 0 ||
-        (p->bias && !io_valid(p->bias_dtype)))
+        p->H > (1 << 30) || (p->bias && !io_valid(p->bias_dtype)))
         return WARPCTCT_EINVAL;
     if (p->N == 0) return WARPCTCT_OK;
     if (!p->logits || !p->out) return WARPCTCT_EINVAL;

@@ -177,8 +177,8 @@ def adjust_logits(logits: torch.Tensor,
 
     Args:
         logits: (N, V).
-        tokens: (N, H) whole numbers, or None; values outside [0, V) (padding)
-            count for nothing.
+        tokens: (N, H) whole numbers, H up to 2^30, or None; values outside [0, V)
+            (padding) count for nothing.
         tokens_lengths: (N,) how many of a row's tokens count.  None: all H.
         repetition_penalty, presence_penalty, frequency_penalty: a number, or
             (N,) with one for each row.  A repetition penalty is positive.
