@@ -404,6 +404,45 @@ def test_gradient_against_differences():
         assert abs((value[0] - value[1]) / 8e-3 - want) < 0.02 * (1 + abs(want)), name
 
 
+def growing():
+    """400 steps of one sequence, cut into chunks of 48, with exponents above zero and nothing to grow.  What a chunk
+    does to a state goes by the sum of its d, formed one after the other: off by up to 24 units of the sum, where the
+    oracle allows every step 20 units of its d a and 4 more.  Twice the oracle's bound covers both; with d = 0.01
+    the 4 units a step do."""
+    case = Case(1, 400, 8, 16, gate=False, softplus=False, initial=False, dt_bias=False)
+    case.glast = None
+    with torch.no_grad():
+        case.args["a"].fill_(1.0)
+        case.args["x"].zero_()
+        case.args["dt"].fill_(0.01)
+    return case
+
+
+@gpu
+@pytest.mark.parametrize("first", [None, 1e-36])
+def test_growth_of_nothing_and_of_little_over_a_chunk(first):
+    case = growing()
+    with torch.no_grad():
+        case.args["dt"][:, :200 if first is None else 35] = 4.0      # 2^277 over a chunk, 2^202
+        if first is None:
+            case.args["x"][:, 200:] = 1.0
+        else:
+            case.args["initial_state"] = torch.full((1, 8, 16), first, device="cuda")
+        val, tol = oracle(case)
+        out, state = case.call()
+    for name, got in (("out", out), ("state", state)):
+        check(got, val, {name: 2 * tol[name]}, name)
+
+
+@gpu
+def test_growth_of_gradients_of_zero_over_a_chunk():
+    case = growing()
+    with torch.no_grad():
+        case.args["dt"][:, 200:] = 4.0
+    case.g[:, 200:] = 0
+    compare(case)
+
+
 @gpu
 def test_refusals_on_the_gpu():
     case = Case(2, 10, 8, 16)

@@ -463,6 +463,15 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
     }
 }
 
+// 2^x v as the steps that x is the sum of would leave it: the power alone may be
+// beyond the range where the product is not (2^200 times 0, or times 2^-120).
+// |x| > 300 takes every v to zero, or what is not zero out of range.
+__device__ __forceinline__ float times_exp2(float v, float x) {
+    x = fminf(fmaxf(x, -300.0f), 300.0f);
+    const float whole = rintf(x);
+    return ldexpf(v * exp2_hw(x - whole), (int)whole);
+}
+
 // Joins chunks: turns what each makes of zeros into what stands in front of it,
 // in place; backwards for the reverse recurrence, whose end (in front of the
 // sequence) goes to `end`.  A thread has one state, and asks for kJoin chunks while
@@ -495,7 +504,7 @@ __global__ __launch_bounds__(kThreads) void scan_join_kernel(const float *__rest
             if (c0 + c >= count) break;
             const int at = backwards ? count - 1 - c0 - c : c0 + c;
             chunks.local[(((long)n * count + at) * E + e) * SP + k] = h;
-            h = fmaf(exp2_hw(rate * d[c]), h, l[c]);
+            h = times_exp2(h, rate * d[c]) + l[c];
         }
     };
     request(0, local[0], total[0]);
