@@ -12,6 +12,8 @@ the sigmoids are formed from gives zero (or infinity, whose reciprocal is zero)
 where the result lies below TINY = 2^-126: such a factor is off by TINY, silu by
 |gate| TINY, its slope by (1 + |gate|) TINY, in absolute terms.  Products of two errors are left
 out and covered by the factor 1.1 at the end."""
+import math
+
 import pytest
 import torch
 
@@ -402,6 +404,41 @@ def test_gradient_against_differences():
             value.append(float((f64(out) * f64(case.g)).sum() + (f64(state) * f64(case.glast)).sum()))
         want = float((f64(got["grad_" + name]) * f64(way)).sum())
         assert abs((value[0] - value[1]) / 8e-3 - want) < 0.02 * (1 + abs(want)), name
+
+
+@gpu
+def test_rates_at_the_ends_of_the_range():
+    low = torch.finfo(torch.float32).min
+    for lengths in ([40, 18, 3], [40 * 8, 18 * 8, 0]):       # whole, and cut into chunks
+        case = Case(3, lengths[0], 16, 16, lengths=lengths)
+        with torch.no_grad():
+            case.args["a"][3], case.args["a"][4, 2], case.args["a"][5, 3:] = low, -3e38, -2.5e38
+        compare(case)
+        with torch.no_grad():
+            kept = case.call()
+            case.args["a"][3] = -math.inf
+            got = case.call()
+            assert torch.equal(got[0], kept[0]) and torch.equal(got[1], kept[1])
+            case.args["a"][7, 5] = math.nan
+            out = case.call()[0]
+            assert out[:2, 0, 7].isnan().all() and torch.equal(out[..., :7], kept[0][..., :7])
+            case.args["a"][7, 5] = -1.0
+            case.args["a"][3] = low
+            case.args["dt"][:, ::5] = -200.0      # d = 0: the state stays, whatever its rate
+            val, tol = oracle(case)
+            out, state = case.call()
+            check(out, val, tol, "out")
+            check(state, val, tol, "state")
+    case = Case(3, 1, 16, 16)
+    with torch.no_grad():
+        case.args["a"][3], case.args["dt"][1:] = low, -200.0
+        val, tol = oracle(case)
+        state = case.args["initial_state"].detach().clone()
+        steps = ("x", "dt", "b", "c", "gate")
+        fixed = {k: v for k, v in case.args.items() if k not in steps + ("initial_state",)}
+        out = warp_ctct.selective_scan_step(state=state, **fixed, **{k: case.args[k][:, 0] for k in steps}, softplus=True)
+        check(out[:, None], val, tol, "out")
+        check(state, val, tol, "state")
 
 
 def growing():

@@ -71,6 +71,14 @@ constexpr int buffers(int lanes) { return lanes == 4 || lanes == 8 ? 2 : 1; }
 
 __device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
 
+// v held within [-most, most]; not a number as it is
+__device__ __forceinline__ float within(float v, float most) { return fabsf(v) > most ? copysignf(most, v) : v; }
+
+// a of a state as the power of two that its factor is formed from, finite where a
+// log2 e is not: d = 0 (a step that does not count has it) leaves every state as
+// it is.
+__device__ __forceinline__ float rate_of(float a) { return within(a * kLog2e, 3.402823466e38f); }
+
 // log(1 + e^v) and its derivative.  log1p(q), q = e^-|v| in [0, 1], is
 // 2 atanh(q / (2 + q)), whose argument r is at most 1/3.  atanh(r) / r as a
 // polynomial of degree 4 in r^2, its coefficients found by Remez exchange for the
@@ -331,7 +339,7 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
 #pragma unroll
     for (int i = 0; i < kStates; ++i) {
         const bool in = live && q * kStates + i < p.S;
-        a[i] = in ? p.a[(long)e * p.S + q * kStates + i] * kLog2e : 0.0f;
+        a[i] = in ? rate_of(p.a[(long)e * p.S + q * kStates + i]) : 0.0f;
         h[i] = 0.0f;
         if (!CARRY && in && starts)
             h[i] = starts[chunk * SP + q * kStates + i];
@@ -467,7 +475,7 @@ __global__ __launch_bounds__(kThreads) void scan_kernel(warpctct_scan_t p, float
 // beyond the range where the product is not (2^200 times 0, or times 2^-120).
 // |x| > 300 takes every v to zero, or what is not zero out of range.
 __device__ __forceinline__ float times_exp2(float v, float x) {
-    x = fminf(fmaxf(x, -300.0f), 300.0f);
+    x = within(x, 300.0f);
     const float whole = rintf(x);
     return ldexpf(v * exp2_hw(x - whole), (int)whole);
 }
@@ -485,7 +493,7 @@ __global__ __launch_bounds__(kThreads) void scan_join_kernel(const float *__rest
     if (i >= (long)E * SP) return;
     const int n = blockIdx.y, e = (int)(i / SP), k = (int)(i - (long)e * SP);
     if (k >= S) return;
-    const float rate = a[(long)e * S + k] * kLog2e;
+    const float rate = rate_of(a[(long)e * S + k]);
     const long state = ((long)n * E + e) * S + k;
     float h = first ? first[state] : 0.0f;
     float local[2][kJoin], total[2][kJoin];
@@ -687,7 +695,7 @@ __global__ __launch_bounds__(kThreads, 2) void scan_grad_kernel(warpctct_scan_t 
                 const float b[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
                 for (int i = 0; i < kStates; ++i) {
-                    k[j][i] = exp2_hw(s.x * (a[i] * kLog2e));
+                    k[j][i] = exp2_hw(s.x * rate_of(a[i]));
                     h[j][i] = fmaf(k[j][i], j ? h[j - 1][i] : h0[i], s.y * b[i]);
                 }
                 const float4 c4 = *reinterpret_cast<const float4 *>(&bc[buf][j][SP + q * kStates]);
@@ -790,7 +798,7 @@ __global__ __launch_bounds__(kThreads) void scan_grad_carry_kernel(warpctct_scan
 #pragma unroll
     for (int i = 0; i < kStates; ++i) {
         const bool in = live && q * kStates + i < p.S;
-        a[i] = in ? p.a[(long)e * p.S + q * kStates + i] * kLog2e : 0.0f;
+        a[i] = in ? rate_of(p.a[(long)e * p.S + q * kStates + i]) : 0.0f;
         carry[i] = 0.0f;
     }
     const int e0 = w.first + el.c, have = max(0, min(EPT, w.end - e0));
@@ -889,7 +897,7 @@ __global__ __launch_bounds__(kThreads) void scan_step_kernel(warpctct_scan_step_
     Raw<float, kStates> ar;
     ar.load(ap, WIDE, most);
 #pragma unroll
-    for (int i = 0; i < kStates; ++i) a[i] = ar[i] * kLog2e;
+    for (int i = 0; i < kStates; ++i) a[i] = rate_of(ar[i]);
     const float bias = p.dt_bias ? p.dt_bias[e] : 0.0f, skip = p.skip ? p.skip[e] : 0.0f;
     for (long n0 = (long)blockIdx.y * BATCH; n0 < p.N; n0 += (long)gridDim.y * BATCH) {
         Raw<float, kStates> h[BATCH];
