@@ -47,6 +47,16 @@ void refuse_second_derivative(const char *name) {
                 "(create_graph=True)");
 }
 
+// Nor is there a forward-mode derivative: an input that carries a tangent is
+// refused, instead of giving a result without one.
+bool has_tangent(const torch::Tensor &t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const Maybe &t) { return given(t) && has_tangent(*t); }
+template <typename... Inputs>
+void refuse_tangents(const char *what, const Inputs &...inputs) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    TORCH_CHECK(!(has_tangent(inputs) || ...), what, ": the forward-mode derivative is not available");
+}
+
 const void *ptr(const torch::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 float *floats(const torch::Tensor &t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
 
@@ -194,6 +204,7 @@ torch::Tensor layer_norm(const torch::Tensor &input, Maybe weight, Maybe bias, c
     TORCH_CHECK(input.size(-1) <= (1L << 27) - 32 && input.numel() / input.size(-1) < (1L << 31),
                 "layer_norm: at most 2^31 - 1 rows of at most 2^27 - 32 elements");
     TORCH_CHECK(eps >= 0, "layer_norm: eps must not be negative");
+    refuse_tangents("layer_norm", input, weight, bias);
     const torch::Tensor x = native(input);
     bool same = true;      // parameters in the input's type; otherwise all of them in float32
     for (const Maybe *p : {&weight, &bias}) {
@@ -353,6 +364,7 @@ tensor_list causal_conv(const torch::Tensor &input, const torch::Tensor &weight,
                         const Maybe &lengths, const Maybe &initial, const bool silu, const bool want_state) {
     CHECK_DEVICE(input);
     TORCH_CHECK(input.dim() == 3 && input.size(2) >= 1, "causal_conv: the input must be (batch, time, channels)");
+    refuse_tangents("causal_conv", input, weight, bias, initial);
     const torch::Tensor x = dense_last(native(input));
     check_taps(weight, bias, x, "causal_conv");
     const int L = int_size(x, 1, "causal_conv"), E = int_size(x, 2, "causal_conv");
@@ -379,6 +391,7 @@ torch::Tensor causal_conv_step(const torch::Tensor &input, torch::Tensor state, 
                                const Maybe &bias, const bool silu, const Maybe &advance) {
     CHECK_DEVICE(input);
     TORCH_CHECK(input.dim() == 2 && input.size(1) >= 1, "causal_conv_step: the input must be (batch, channels)");
+    refuse_tangents("causal_conv_step", input, state, weight, bias);
     const torch::Tensor x = dense_last(native(input));
     check_taps(weight, bias, x, "causal_conv_step");
     const Maybe all[4] = {x, state, weight, bias};
@@ -595,6 +608,7 @@ tensor_list selective_scan(const torch::Tensor &input, const torch::Tensor &dt, 
     TORCH_CHECK(input.dim() == 3 && input.size(2) >= 1, "selective_scan: the input must be (batch, time, channels)");
     TORCH_CHECK(input.size(0) <= 65535 && input.size(1) < (1L << 30),
                 "selective_scan: at most 65535 sequences of fewer than 2^30 steps");
+    refuse_tangents(what, input, dt, a, b, c, skip, gate, dt_bias, initial);
     ScanInputs in = scan_inputs(input, dt, a, b, c, skip, gate, dt_bias, what);
     in.lengths = lengths_of(lengths, in.x, what);
     if (given(initial)) {
@@ -622,6 +636,7 @@ torch::Tensor selective_scan_step(const torch::Tensor &input, torch::Tensor stat
     TORCH_CHECK(input.dim() == 2 && input.size(1) >= 1, "selective_scan_step: the input must be (batch, channels)");
     const Maybe all[6] = {input, state, dt, a, b, c};
     refuse_gradient({&all[0], &all[1], &all[2], &all[3], &all[4], &all[5], &skip, &gate, &dt_bias}, what);
+    refuse_tangents(what, input, state, dt, a, b, c, skip, gate, dt_bias);
     const ScanInputs in = scan_inputs(input, dt, a, b, c, skip, gate, dt_bias, what);
     const torch::Tensor &x = in.x;
     TORCH_CHECK(state.dim() == 3 && state.size(0) == x.size(0) && state.size(1) == x.size(1) &&
@@ -682,6 +697,7 @@ struct Penalty {
     }
     static void refuse_if_tracked(const torch::Tensor &t, const char *name) {
         TORCH_CHECK(!tracked(t), "adjust_logits: not differentiable (", name, "); call it under torch.no_grad()");
+        refuse_tangents("adjust_logits", t);
     }
 };
 

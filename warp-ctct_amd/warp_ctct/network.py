@@ -11,7 +11,8 @@ float16 and bfloat16 are read as they are (another type is converted to
 float32), sums and states are kept in float32, a result is rounded once.  Nothing synchronises with the host;
 work is enqueued on the current stream of the input's GPU.  A wrong shape, type
 or device raises RuntimeError.  The backward passes are not differentiable
-themselves (``create_graph=True`` raises).  Forward and backward can be captured
+themselves (``create_graph=True`` raises), and inputs with a forward-mode tangent
+are refused.  Forward and backward can be captured
 into a graph; as with any operator of torch, an eager autograd graph that hangs
 on the same leaves must be gone before a backward pass is captured.
 
