@@ -39,3 +39,33 @@ def test_tangents_are_refused():
                         operator(**dual)
                 operator(**inputs)
             operator(**inputs)
+
+
+def with_lengths():
+    """Every operator with lengths, as a function of them: outputs over T steps or tokens of N rows."""
+    x, weight, dt, b = rand(N, T, E), rand(E, K), rand(N, T, E), rand(N, T, S)
+    a, logits, tokens = -rand(E, S), rand(N, 16), torch.randint(0, 16, (N, T), device="cuda")
+    return [lambda l: warp_ctct.causal_conv(x, weight, lengths=l, return_state=True),
+            lambda l: warp_ctct.selective_scan(x, dt, a, b, b, lengths=l, return_state=True),
+            lambda l: (warp_ctct.adjust_logits(logits, tokens, l, presence_penalty=0.5, frequency_penalty=0.1),)]
+
+
+def test_lengths_out_of_the_range_of_int32_are_clamped():
+    lengths = lambda values, dtype: torch.tensor(values, dtype=dtype).cuda()  # noqa: E731
+    for operator in with_lengths():
+        for dtype, values, clamped in (
+                (torch.int64, [2 ** 32, 2 ** 63 - 1, 2 ** 33 + 5], [T, T, T]),
+                (torch.int64, [-2 ** 32 - 5 + 2 ** 31, -2 ** 63, -2 ** 32 + 7], [0, 0, 0]),
+                (torch.int64, [T + 1, 3, 0], [T, 3, 0]), (torch.uint32, [2 ** 32 - 1, 2 ** 31, 3], [T, T, 3]),
+                (torch.uint64, [2 ** 64 - 1, 2 ** 63 + 2, 2 ** 32 + 4], [T, T, T]),
+                (torch.uint64, [7, 0, T], [7, 0, T]), (torch.uint16, [65535, 2, 0], [T, 2, 0]),
+                (torch.uint8, [255, 2, 0], [T, 2, 0]), (torch.int16, [-1, 300, 5], [0, T, 5])):
+            got, want = operator(lengths(values, dtype)), operator(lengths(clamped, torch.int32))
+            assert all(torch.equal(x, y) for x, y in zip(got, want)), (dtype, values)
+
+
+def test_lengths_that_are_no_whole_numbers_are_refused():
+    for operator in with_lengths():
+        for dtype in (torch.bool, torch.complex64, torch.float32):
+            with pytest.raises(RuntimeError, match="whole numbers"):
+                operator(torch.ones(N, device="cuda", dtype=dtype))

@@ -236,11 +236,20 @@ torch::Tensor dense_last(const torch::Tensor &t) {
     return t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
-torch::Tensor lengths_of(const Maybe &lengths, const torch::Tensor &x, const char *what) {
+// Lengths as int32.  The kernels clamp them into [0, most]; of types that hold
+// more than int32 does that has to come before the conversion.
+torch::Tensor lengths_of(const Maybe &lengths, const torch::Tensor &x, int64_t most, const char *what) {
     if (!given(lengths)) return torch::Tensor();
-    TORCH_CHECK(lengths->dim() == 1 && lengths->size(0) == x.size(0) && !lengths->is_floating_point(), what,
+    const auto type = lengths->scalar_type();
+    TORCH_CHECK(lengths->dim() == 1 && lengths->size(0) == x.size(0) && at::isIntegralType(type, false), what,
                 ": lengths must be whole numbers, one for each sequence");
     check_on(*lengths, x, "lengths");
+    if (type == at::ScalarType::Long) return as_int32(lengths->clamp(0, most));
+    if (type == at::ScalarType::UInt32) return as_int32(lengths->to(at::ScalarType::Long).clamp(0, most));
+    if (type == at::ScalarType::UInt64) {      // (from 2^63 on negative as int64)
+        const auto wide = lengths->to(at::ScalarType::Long);
+        return as_int32(wide.clamp(0, most).masked_fill(wide.lt(0), most));
+    }
     return as_int32(*lengths);
 }
 
@@ -371,7 +380,7 @@ tensor_list causal_conv(const torch::Tensor &input, const torch::Tensor &weight,
     TORCH_CHECK(x.size(0) <= 65535 && L <= (1L << 30) && static_cast<long>(L) * E <= (1L << 32) - 1024,
                 "causal_conv: at most 65535 sequences of at most 2^30 steps and 2^32 - 1024 elements");
     ConvInputs in = {x, as_float(weight), given(bias) ? as_float(*bias) : torch::Tensor(),
-                     lengths_of(lengths, x, "causal_conv"), torch::Tensor()};
+                     lengths_of(lengths, x, L, "causal_conv"), torch::Tensor()};
     if (given(initial)) {
         TORCH_CHECK(initial->dim() == 3 && initial->size(0) == x.size(0) &&
                         initial->size(1) == weight.size(1) - 1 && initial->size(2) == E &&
@@ -610,7 +619,7 @@ tensor_list selective_scan(const torch::Tensor &input, const torch::Tensor &dt, 
                 "selective_scan: at most 65535 sequences of fewer than 2^30 steps");
     refuse_tangents(what, input, dt, a, b, c, skip, gate, dt_bias, initial);
     ScanInputs in = scan_inputs(input, dt, a, b, c, skip, gate, dt_bias, what);
-    in.lengths = lengths_of(lengths, in.x, what);
+    in.lengths = lengths_of(lengths, in.x, in.x.size(1), what);
     if (given(initial)) {
         TORCH_CHECK(initial->dim() == 3 && initial->size(0) == in.x.size(0) && initial->size(1) == in.x.size(2) &&
                         initial->size(2) == a.size(1) && initial->scalar_type() == at::ScalarType::Float,
@@ -739,7 +748,7 @@ torch::Tensor adjust_logits(const torch::Tensor &input, const Maybe &tokens, con
         p.tokens_n = history.stride(0);
         p.tokens = history.data_ptr();
         if (given(tokens_lengths)) {
-            lengths = lengths_of(tokens_lengths, x, "adjust_logits");
+            lengths = lengths_of(tokens_lengths, x, p.H, "adjust_logits");
             p.tokens_lengths = lengths.data_ptr<int>();
         }
     } else {
