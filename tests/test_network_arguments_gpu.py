@@ -69,3 +69,17 @@ def test_lengths_that_are_no_whole_numbers_are_refused():
         for dtype in (torch.bool, torch.complex64, torch.float32):
             with pytest.raises(RuntimeError, match="whole numbers"):
                 operator(torch.ones(N, device="cuda", dtype=dtype))
+
+
+def test_tokens_of_other_types():
+    logits = rand(1, 8)
+    tokens = lambda values, dtype: torch.tensor([values], dtype=dtype).cuda()  # noqa: E731
+    rule = lambda t: warp_ctct.adjust_logits(logits, t, presence_penalty=0.5)  # noqa: E731
+    want = rule(tokens([3, -1, 9], torch.int32))
+    for dtype, values in ((torch.uint64, [3, 2 ** 32 + 5, 2 ** 64 - 7]), (torch.uint32, [3, 2 ** 32 - 6, 2 ** 31]),
+                          (torch.uint16, [3, 65530, 8]), (torch.uint8, [3, 250, 8]), (torch.int8, [3, -3, -8]),
+                          (torch.int16, [3, -3, 99]), (torch.int64, [3, 2 ** 32 + 5, -2 ** 63])):
+        assert torch.equal(rule(tokens(values, dtype)), want), dtype
+    for dtype in (torch.bool, torch.complex64, torch.float32):
+        with pytest.raises(RuntimeError, match="whole numbers"):
+            rule(torch.ones(1, 3, device="cuda", dtype=dtype))

@@ -737,12 +737,14 @@ torch::Tensor adjust_logits(const torch::Tensor &input, const Maybe &tokens, con
     torch::Tensor history, lengths, b, mask;
     if (given(tokens)) {
         const auto type = tokens->scalar_type();
-        TORCH_CHECK(tokens->dim() == 2 && tokens->size(0) == N && !tokens->is_floating_point() &&
-                        type != at::ScalarType::Bool && tokens->size(1) <= (1L << 30),
+        TORCH_CHECK(tokens->dim() == 2 && tokens->size(0) == N && at::isIntegralType(type, false) &&
+                        tokens->size(1) <= (1L << 30),
                     "adjust_logits: tokens must be whole numbers, (rows, history), a history of at most 2^30");
         check_on(*tokens, x, "tokens");
+        // (as int64 what int32 does not hold stays outside the vocabulary)
         const bool taken = type == at::ScalarType::Int || type == at::ScalarType::Long;
-        history = dense_last(taken ? *tokens : tokens->to(at::ScalarType::Int));
+        const bool wide = type == at::ScalarType::UInt32 || type == at::ScalarType::UInt64;
+        history = dense_last(taken ? *tokens : tokens->to(wide ? at::ScalarType::Long : at::ScalarType::Int));
         p.H = static_cast<int>(history.size(1));
         p.tokens_64 = history.scalar_type() == at::ScalarType::Long ? 1 : 0;
         p.tokens_n = history.stride(0);
