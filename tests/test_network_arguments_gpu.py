@@ -83,3 +83,36 @@ def test_tokens_of_other_types():
     for dtype in (torch.bool, torch.complex64, torch.float32):
         with pytest.raises(RuntimeError, match="whole numbers"):
             rule(torch.ones(1, 3, device="cuda", dtype=dtype))
+
+
+def test_float64_is_float32():
+    for operator, inputs in calls():
+        if "state" in inputs:       # moved on in place: never converted
+            narrow, wide = inputs["state"].clone(), inputs["state"].double()
+            rest = {k: v for k, v in inputs.items() if k != "state"}
+            want = operator(state=narrow, **rest)
+            assert torch.equal(operator(state=inputs["state"], **{k: v.double() for k, v in rest.items()}), want)
+            assert torch.equal(inputs["state"], narrow)
+            with pytest.raises(RuntimeError, match="state"):
+                operator(state=wide, **rest)
+            continue
+        leaves = {k: v.detach().requires_grad_(operator.__name__ != "<lambda>") for k, v in inputs.items()}
+        wide = {k: v.detach().double().requires_grad_(v.requires_grad) for k, v in leaves.items()}
+        want, got = operator(**leaves), operator(**wide)
+        assert got.dtype == torch.float32 and torch.equal(got, want)
+        if got.requires_grad:
+            g = torch.rand_like(got)
+            for x, y in zip(torch.autograd.grad(got, list(wide.values()), g),
+                            torch.autograd.grad(want, list(leaves.values()), g)):
+                assert x.dtype == torch.float64 and torch.equal(x.float(), y)
+
+
+def test_states_of_integers_and_of_narrow_types():
+    for operator, inputs in calls():
+        if "initial_state" not in inputs:
+            continue
+        whole = torch.randint(-3, 4, inputs["initial_state"].shape, device="cuda")
+        assert torch.equal(operator(**dict(inputs, initial_state=whole)),
+                           operator(**dict(inputs, initial_state=whole.float())))
+        with pytest.raises(RuntimeError, match="initial_state"):
+            operator(**dict(inputs, initial_state=whole.half()))

@@ -382,12 +382,12 @@ tensor_list causal_conv(const torch::Tensor &input, const torch::Tensor &weight,
     ConvInputs in = {x, as_float(weight), given(bias) ? as_float(*bias) : torch::Tensor(),
                      lengths_of(lengths, x, L, "causal_conv"), torch::Tensor()};
     if (given(initial)) {
-        TORCH_CHECK(initial->dim() == 3 && initial->size(0) == x.size(0) &&
-                        initial->size(1) == weight.size(1) - 1 && initial->size(2) == E &&
-                        initial->scalar_type() == x.scalar_type(),
+        const torch::Tensor first = native(*initial);
+        TORCH_CHECK(first.dim() == 3 && first.size(0) == x.size(0) && first.size(1) == weight.size(1) - 1 &&
+                        first.size(2) == E && first.scalar_type() == x.scalar_type(),
                     "causal_conv: initial_state must be (batch, taps - 1, channels) in the input's type");
-        check_on(*initial, x, "initial_state");
-        in.initial = initial->contiguous();
+        check_on(first, x, "initial_state");
+        in.initial = first.contiguous();
     }
     const bool tw = tracked(in.weight), tb = tracked(in.bias), ti = tracked(in.initial);
     if (!(tracked(in.x) || tw || tb || ti)) return conv_forward(in, silu, want_state);
@@ -621,11 +621,12 @@ tensor_list selective_scan(const torch::Tensor &input, const torch::Tensor &dt, 
     ScanInputs in = scan_inputs(input, dt, a, b, c, skip, gate, dt_bias, what);
     in.lengths = lengths_of(lengths, in.x, in.x.size(1), what);
     if (given(initial)) {
-        TORCH_CHECK(initial->dim() == 3 && initial->size(0) == in.x.size(0) && initial->size(1) == in.x.size(2) &&
-                        initial->size(2) == a.size(1) && initial->scalar_type() == at::ScalarType::Float,
+        const torch::Tensor first = native(*initial);
+        TORCH_CHECK(first.dim() == 3 && first.size(0) == in.x.size(0) && first.size(1) == in.x.size(2) &&
+                        first.size(2) == a.size(1) && first.scalar_type() == kFloat,
                     "selective_scan: initial_state must be (batch, channels, states) in float32");
-        check_on(*initial, in.x, "initial_state");
-        in.initial = initial->contiguous();
+        check_on(first, in.x, "initial_state");
+        in.initial = first.contiguous();
     }
     bool track = false;
     for (const auto *t : {&in.x, &in.dt, &in.a, &in.b, &in.c, &in.skip, &in.gate, &in.dt_bias, &in.initial})

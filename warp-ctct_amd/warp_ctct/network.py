@@ -67,7 +67,7 @@ def causal_conv(x: torch.Tensor,
         lengths: (N,) steps of each sequence; the steps behind them are not read
             and their outputs (and gradients) are zero.  None: all T.
         initial_state: (N, K-1, E), the inputs in front of ``x``, in the type of
-            ``x``.  None: zeros.
+            ``x`` (float32 or float64 where that is float64).  None: zeros.
         activation: None or ``'silu'``.
         return_state: also return (N, K-1, E), the last K-1 inputs of every
             sequence: the ``initial_state`` of a call that goes on from there, and
@@ -87,7 +87,8 @@ def causal_conv_step(x: torch.Tensor,
                      activation: Optional[str] = None,
                      advance: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One step of :func:`causal_conv` for N sequences: ``x`` (N, E) comes in,
-    ``state`` (N, K-1, E) moves on in place, out (N, E) is returned.
+    ``state`` (N, K-1, E), in the type of the result, moves on in place, out
+    (N, E) is returned.
 
     ``advance`` (N,) bool, None for all: a sequence that does not advance keeps
     its state, and its row of the result is zero (a hypothesis that took blank
@@ -123,8 +124,8 @@ def selective_scan(x: torch.Tensor,
         skip, dt_bias: (E,) or None.
         lengths: (N,) steps of each sequence; the steps behind them are not read
             and their outputs (and gradients) are zero.  None: all T.
-        initial_state: (N, E, S) float32, the states in front of the first step.
-            None: zeros.
+        initial_state: (N, E, S) float32 (or float64, converted), the states in
+            front of the first step.  None: zeros.
         return_state: also return the states behind the last step of every
             sequence, (N, E, S) float32: the ``initial_state`` of a call that goes
             on from there, and the ``state`` of :func:`selective_scan_step`.
