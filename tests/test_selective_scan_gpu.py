@@ -12,11 +12,13 @@ the sigmoids are formed from gives zero (or infinity, whose reciprocal is zero)
 where the result lies below TINY = 2^-126: such a factor is off by TINY, silu by
 |gate| TINY, its slope by (1 + |gate|) TINY, in absolute terms.  Products of two errors are left
 out and covered by the factor 1.1 at the end."""
+import ctypes
 import math
 
 import pytest
 import torch
 
+import hip_lib
 import warp_ctct
 
 gpu = pytest.mark.gpu
@@ -526,3 +528,56 @@ def test_refusals_without_a_gpu():
         warp_ctct.selective_scan(t(1, 2, 3), t(1, 2, 3), t(3, 4), t(1, 2, 4), t(1, 2, 4))
     with pytest.raises(RuntimeError, match="GPU"):
         warp_ctct.selective_scan_step(t(1, 3), t(1, 3, 4), t(1, 3), t(3, 4), t(1, 4), t(1, 4))
+
+
+# Few long sequences are cut into chunks, in both directions.  Two groups, odd and
+# even batches, rows in wide pieces and not, 1 to 16 lanes a channel; more channels
+# in a group than a workgroup takes; sequences that end inside an earlier chunk, at
+# the end of one and one step behind it, and that have one step or none.
+CUT = [(6, 250, 10, 3, 2), (6, 240, 64, 3, 2), (3, 400, 600, 4, 2), (6, 250, 24, 8, 2), (5, 260, 40, 16, 2),
+       (6, 230, 64, 16, 1), (6, 230, 20, 24, 2), (3, 200, 12, 64, 2), (5, 140, 40, 64, 2)]
+
+
+def chunk_steps(N, T, E, S, G):
+    """Steps of a chunk, forwards and backwards, from the scratch that the two passes take."""
+    size = hip_lib.lib().warpctct_selective_scan_workspace_bytes
+    size.restype = ctypes.c_size_t
+    lanes = next(n for n in (1, 2, 4, 8, 16) if 4 * n >= S)
+    tile, blocks = {1: 4, 16: 16}.get(lanes, 8), -(-(E // G) // (256 // lanes))
+    states, sums = E * (4 * lanes + 1), E * (S + 2)      # of a sequence and chunk
+    forward, rest = divmod(size(N, T, E, S, G, 0) // 4, N * states)
+    backward, left = divmod(size(N, T, E, S, G, 1) // 4 - N * G * blocks * -(-T // tile) * tile * 8 * lanes, N * (states + sums))
+    assert rest == left == 0 and forward > 1 and backward > 1      # (else it is not cut)
+    return [16 * -(-(-(-T // 16)) // n) for n in (forward, backward)]
+
+
+@pytest.mark.parametrize("shape", CUT)
+def test_the_shapes_below_are_cut(shape):
+    assert all(32 <= steps <= shape[1] - 16 for steps in chunk_steps(*shape))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", CUT)
+def test_few_long_sequences(shape, dtype):
+    # A chunk's factor goes by the sum of its d, formed one after the other: off by up to steps/2 units of the sum,
+    # where the oracle allows every step 20 units of its d a.
+    loose = 1 + max(chunk_steps(*shape)) / 40
+    N, T, E, S, G = shape
+    lengths = [T, T // 3, 0, 64, 65, 1][:N]
+    for start, end in ((True, False), (False, True)):
+        case = Case(*shape, dtype, seed=T, lengths=lengths, initial=start, gate=end)
+        if not end:
+            case.glast = None
+        with torch.no_grad():       # what lies behind a sequence is not read
+            for n, length in enumerate(lengths):
+                for rows in [case.args[k] for k in ("x", "dt", "b", "c")] + [case.g] + [case.args["gate"]] * end:
+                    rows[n, length:] = math.nan
+        val, tol = oracle(case)
+        got, again = case.run(), case.run()
+        for name in got:
+            check(got[name], val, {name: loose * tol[name]}, name)
+            assert torch.equal(got[name], again[name])
+        with torch.no_grad():
+            out, state = case.call()
+        assert torch.equal(out, got["out"]) and torch.equal(state, got["state"])
