@@ -41,7 +41,7 @@ __device__ __forceinline__ raw16 pack16(const IO *p, const float *x) {
     return raw16{pack_two(p, x[0], x[1]), pack_two(p, x[2], x[3]), pack_two(p, x[4], x[5]),
                  pack_two(p, x[6], x[7])};
 }
-// N elements next to each other (1, 2, 4, or a 16-byte vector), aligned to their size
+// N elements next to each other (1, 4, or a 16-byte vector), aligned to their size
 template <int N, typename IO>
 __device__ __forceinline__ void load_n(const IO *p, float *x) {
     if constexpr (N == 1) {
@@ -59,17 +59,9 @@ __device__ __forceinline__ void store_n(IO *p, const float *x) {
         *p = from_float<IO>(x[0]);
     } else if constexpr (N == kVec<IO>) {
         *reinterpret_cast<raw16 *>(p) = pack16(p, x);
-    } else if constexpr (sizeof(IO) == 4) {
-        typedef IO piece __attribute__((ext_vector_type(N)));
-        piece v;
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = x[i];
-        *reinterpret_cast<piece *>(p) = v;
-    } else if constexpr (N == 4) {
-        *reinterpret_cast<uint2 *>(p) = make_uint2(pack_two(p, x[0], x[1]), pack_two(p, x[2], x[3]));
     } else {
-        static_assert(N == 2, "1, 2, 4 elements or a vector");
-        *reinterpret_cast<unsigned *>(p) = pack_two(p, x[0], x[1]);
+        static_assert(N == 4 && sizeof(IO) == 2, "1, 4 elements or a vector");
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack_two(p, x[0], x[1]), pack_two(p, x[2], x[3]));
     }
 }
 
