@@ -25,7 +25,9 @@ constexpr unsigned kGroups = 1024;   // workgroups of the forward pass, at most
 constexpr unsigned kWideGroups = 1u << 20;      // and where a row does not fit into their registers
 // and of the backward pass: four on a compute unit where they take a row each, two
 // where their wavefronts do (12800 rows of 2048 elements: 36.6 us with 1024, 42.0
-// with 512; 2592 rows of 641: 16.2 with 1024, 11.4 with 512)
+// with 512; 2592 rows of 641: 16.2 with 1024, 11.4 with 512).  Measured at these
+// widths alone: at several times 2048 the 8 bytes a column that every workgroup
+// leaves come to as much as the rows.
 constexpr int kGradGroups = 1024, kGradGroupsOfWaves = 512;
 
 // Sums of two values over the threads of a row: a wavefront (threads == 64) or

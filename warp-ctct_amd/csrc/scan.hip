@@ -27,11 +27,12 @@
 // them one after the other, and the second pass starts every chunk from its own
 // states; the reverse recurrence of gh alike.
 //
-// Measured with 16 states, bfloat16 and a gate: 32 ragged sequences of up to 400
-// steps, 1024 channels: forward 58 us, backward 147 us, of which the vector units
-// cannot do without 39 and 112 (SQ_ACTIVE_INST_VALU); one sequence of 16384 steps,
-// 2048 channels: 242 us in two passes, 224 of them the vector units'; one step of
-// 256 sequences, 2048 channels: 12.6 us, 5.6 TB/s.
+// Measured with 16 states, bfloat16 and a gate: 32 ragged sequences of 200 to 400
+// steps, 1024 channels: forward 58 us, backward 147 us (65 and 176 beside a
+// profiler), of which the vector units cannot do without 39 and 112
+// (SQ_ACTIVE_INST_VALU); one sequence of 16384 steps, 2048 channels: 242 us in two
+// passes, 224 of them the vector units'; one step of 256 sequences, 70 % of which
+// advance, 2048 channels: 12.6 us, 4.0 TB/s of what is read and written.
 #include <algorithm>
 #include <cmath>
 
@@ -65,8 +66,9 @@ constexpr int padded(int lanes) { return kThreads / lanes + 64 / lanes; }
 // Tiles in LDS at a time.  With two, a tile's results are formed while the next
 // tile is worked on, and one barrier a tile is enough; with few or many states they
 // take the LDS of the second or third workgroup of a compute unit (32 sequences
-// of 400 steps, 1024 channels, training, one / two: 16 states 271 / 264 us, 32
-// states 461 / 454; 64 states 861 / 866, forwards 180 / 182).
+// all of 400 steps, 1024 channels, bfloat16, training, one / two: 16 states 273 /
+// 268 us, 32 states 465 / 456; 64 states 861 / 866, forwards 180 / 182; of 200 to
+// 400 steps, 16 states: 222 / 217).
 constexpr int buffers(int lanes) { return lanes == 4 || lanes == 8 ? 2 : 1; }
 
 __device__ __forceinline__ float exp2_hw(float v) { return __builtin_amdgcn_exp2f(v); }
@@ -82,7 +84,7 @@ __device__ __forceinline__ float rate_of(float a) { return within(a * kLog2e, 3.
 // log(1 + e^v) and its derivative.  log1p(q), q = e^-|v| in [0, 1], is
 // 2 atanh(q / (2 + q)), whose argument r is at most 1/3.  atanh(r) / r as a
 // polynomial of degree 4 in r^2, its coefficients found by Remez exchange for the
-// least relative error over [0, 1/9], is off by 4e-9; log2(1 + q) on the
+// least relative error over [0, 1/9], is off by 8e-9; log2(1 + q) on the
 // transcendental unit would lose q itself to the rounding of the sum.
 struct Softplus {
     float value, slope;
@@ -982,13 +984,14 @@ bool rows_wide(const warpctct_scan_t &p, int ept) {
 
 // Chunks that a sequence is cut into.  Two passes cost twice the arithmetic
 // forwards and a quarter more backwards, but a wavefront alone on its SIMD waits
-// most of the time: cutting pays up to 768 wavefronts of uncut sequences (1024
+// most of the time: sequences are cut up to 768 wavefronts of them uncut (1024
 // SIMDs) forwards and 1024 backwards, into as many chunks as put eight wavefronts
-// on each, of two tiles at least.  Measured with 1024 channels, 16 states, 1500
+// on each, of two tiles at least.  The limits are those that long sequences gain by
+// without short ones losing much.  Measured with 1024 channels, 16 states, 1500
 // steps (us, uncut / cut): forwards 512 wavefronts 186 / 102, 768 186 / 139, 1024
 // 188 / 178, 1536 245 / 272; backwards 1024 595 / 454, 1536 746 / 711, 2048
-// 751 / 885; with 300 steps forwards 768 41 / 45, backwards 1024 130 / 111, 1536
-// 157 / 162.  Fewer than 8 tiles are not worth the two launches more, and more
+// 751 / 885; with 300 steps forwards 768 41 / 45 (a loss), backwards 1024
+// 130 / 111, 1536 157 / 162.  Fewer than 8 tiles are not worth the two launches more, and more
 // than 8 sqrt(tiles) chunks take longer to join than they save (2 us a tile for a
 // wavefront on its own).
 struct Cut {

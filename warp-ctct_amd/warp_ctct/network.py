@@ -75,7 +75,8 @@ def causal_conv(x: torch.Tensor,
 
     Returns out (N, T, E), or ``(out, state)``.  Differentiable with respect to
     ``x``, ``weight``, ``bias`` and ``initial_state``, through both results; the
-    gradients of the parameters are added up in a fixed order."""
+    gradients of the parameters are added up in a fixed order.  The gradient of
+    ``x`` is formed whether it is asked for or not."""
     got = core.causal_conv(x, weight, bias, lengths, initial_state, _activation(activation), bool(return_state))
     return (got[0], got[1]) if return_state else got[0]
 
@@ -132,7 +133,7 @@ def selective_scan(x: torch.Tensor,
 
     Returns out (N, T, E), or ``(out, state)``.  Differentiable with respect to
     everything but ``lengths``, through both results; every sum is added up in a
-    fixed order.  Where a gradient is tracked, the states in front of every 8
+    fixed order.  All gradients are formed, whichever are asked for.  Where a gradient is tracked, the states in front of every 8
     steps are kept for it: T/8 * N * E * S floats for 16 states."""
     got = core.selective_scan(x, dt, a, b, c, skip, gate, dt_bias, bool(softplus), lengths, initial_state,
                               bool(return_state))
